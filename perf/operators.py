@@ -370,7 +370,7 @@ def _own_kv(s, dev):
 
 def _own_tree(s, dev):
     dev.tree_attn(s["q"], s["kc"], s["kp"], s["vc"], s["vp"], s["table"], s["len"], s["mask"],
-                  s["o"], lse=s["lse"])
+                  s["o"], s["dim"], lse=s["lse"])
     return s["o"], s["lse"]
 
 
