@@ -323,6 +323,138 @@ int nl_ternary_gemv_static_dev(const float *X, const uint32_t *WP,
                                uint32_t seq, uint32_t out, uint32_t cols,
                                void *stream);
 
+/* ---- speculative serving: Q/K norm + RoPE, quantised KV cache, tree attention - */
+
+/* Element types of the activations of the entry points below. */
+#define NL_F32 0
+#define NL_BF16 1
+
+/* Which values of a head the rotation pairs: (m, m + rot_dim/2), as rope-half
+ * (lisp/nelisp-gpu-kernels.el:857-882), or (2m, 2m + 1), as rope-apply. */
+#define NL_PAIRS_HALF 0
+#define NL_PAIRS_ADJACENT 1
+
+/* RMS norm of every query and key head and the position rotation, in one
+ * pass.  QKV holds N rows, X_STRIDE elements apart, that begin with
+ * [heads*head_dim q | kv_heads*head_dim k] (what follows, the values, is not
+ * read).  Q and K receive rows of heads*head_dim and kv_heads*head_dim
+ * elements, Q_STRIDE and K_STRIDE apart:
+ *   y = R(POS[row]) (x r o G),  r = 1 / sqrt(mean x^2 + EPS)
+ * per head, G being GQ or GK (f32 [head_dim]).  R turns the pairs of the
+ * first ROT_DIM values by the angles whose cosines and sines are rows of CO
+ * and SI (f32 [ROPE_ROWS x ROT_DIM/2], 16-byte aligned).  A row whose
+ * position is outside [0, ROPE_ROWS) is padding: its outputs are zeros.  Q
+ * and K may be the rows of QKV themselves.  Sums are f32 whatever DTYPE.
+ * Rows are 16-byte aligned; head_dim (at most 256) and rot_dim are multiples
+ * of 8 (f32) or 16 (bf16).  Does not synchronise. */
+int nl_qk_norm_rope_dev(int dtype, const void *QKV, uint64_t x_stride,
+                        const float *GQ, const float *GK, const float *CO,
+                        const float *SI, const int32_t *POS, void *Q,
+                        uint64_t q_stride, void *K, uint64_t k_stride,
+                        uint32_t n, uint32_t heads, uint32_t kv_heads,
+                        uint32_t head_dim, uint32_t rot_dim,
+                        uint32_t rope_rows, int pairs, float eps,
+                        void *stream);
+
+/* Its backward pass: from the saved QKV rows and the gradients DQ and DK of
+ * the two outputs, the gradient of the q and k part of the rows (DQKV rows,
+ * DX_STRIDE apart; the part of the values is not touched) and of the gains
+ * (f32 [head_dim], summed over rows and heads in a fixed order; zeros for no
+ * rows).  Padding rows give zeros.  WORKSPACE holds at least
+ * nl_qk_norm_rope_bwd_workspace_bytes(head_dim) bytes, 16-byte aligned, or is
+ * NULL for the library's own (calls that overlap in time must then not
+ * share it).  Does not synchronise. */
+size_t nl_qk_norm_rope_bwd_workspace_bytes(uint32_t head_dim);
+int nl_qk_norm_rope_bwd_dev(int dtype, const void *QKV, uint64_t x_stride,
+                            const float *GQ, const float *GK, const float *CO,
+                            const float *SI, const int32_t *POS,
+                            const void *DQ, uint64_t dq_stride, const void *DK,
+                            uint64_t dk_stride, void *DQKV, uint64_t dx_stride,
+                            float *DGQ, float *DGK, uint32_t n, uint32_t heads,
+                            uint32_t kv_heads, uint32_t head_dim,
+                            uint32_t rot_dim, uint32_t rope_rows, int pairs,
+                            float eps, void *workspace, size_t ws_bytes,
+                            void *stream);
+
+/* Formats of the quantised paged KV cache.  A cache is four device arrays,
+ * for the keys and for the values
+ *   codes  bytes [num_blocks][kv_heads][block_size][head_dim * bits / 8]
+ *   params words [num_blocks][kv_heads][block_size]
+ * (codes 16-byte aligned), and token slot s is offset s % block_size of block
+ * s / block_size.  Per head vector x, with fl one rounding to f32:
+ *   NL_KV_I8  s = fl(max|x|/127), code = 128 + rint(fl(x fl(127/max|x|))),
+ *             the word is s, the value s (code - 128);
+ *   NL_KV_I4  lo = min x rounded down to bf16, s = fl(fl(max x - lo)/15)
+ *             rounded up to bf16, code = min(15, rint(fl(fl(x-lo) fl(1/s)))),
+ *             element 2i in the low and 2i+1 in the high half of byte i, the
+ *             word is bf16 s below bf16 lo, the value s code + lo.
+ * A scale under 2^-112 becomes 0.  A vector that holds a NaN or an infinity
+ * has scale NaN and reads back, and attends, as NaN.  head_dim is 64, 128 or
+ * 256; block_size is any; slots fit int32 and num_blocks * kv_heads *
+ * block_size fits uint32. */
+#define NL_KV_I4 4
+#define NL_KV_I8 8
+
+/* Quantise N tokens' keys and values (rows of kv_heads*head_dim elements,
+ * 16-byte aligned, K_STRIDE and V_STRIDE apart) into slots SLOT[i].  A slot
+ * outside the pool is skipped; of tokens with the same slot one is kept, its
+ * key and value heads not necessarily of the same token.  Does not
+ * synchronise. */
+int nl_kv_append_dev(int fmt, int dtype, const void *K, uint64_t k_stride,
+                     const void *V, uint64_t v_stride, const int32_t *SLOT,
+                     void *KC, uint32_t *KP, void *VC, uint32_t *VP,
+                     uint32_t n, uint32_t kv_heads, uint32_t head_dim,
+                     uint32_t block_size, uint32_t num_blocks, void *stream);
+
+/* Read the slots back as values: rows of K and V.  A slot outside the pool
+ * reads as zeros.  Does not synchronise. */
+int nl_kv_read_dev(int fmt, int dtype, const int32_t *SLOT, const void *KC,
+                   const uint32_t *KP, const void *VC, const uint32_t *VP,
+                   void *K, uint64_t k_stride, void *V, uint64_t v_stride,
+                   uint32_t n, uint32_t kv_heads, uint32_t head_dim,
+                   uint32_t block_size, uint32_t num_blocks, void *stream);
+
+/* Move tokens inside the pool without requantising them, e.g. the accepted
+ * path of a draft tree to the end of its prefix: for each of BATCH sequences
+ * COUNT (at most 64) slots SRC -> DST (int32 [batch][count]).  All sources of
+ * a sequence are read before any of its destinations is written; a pair with
+ * a slot outside the pool is skipped; different sequences must not share
+ * slots.  Does not synchronise. */
+int nl_kv_move_dev(int fmt, const int32_t *SRC, const int32_t *DST, void *KC,
+                   uint32_t *KP, void *VC, uint32_t *VP, uint32_t batch,
+                   uint32_t count, uint32_t kv_heads, uint32_t head_dim,
+                   uint32_t block_size, uint32_t num_blocks, void *stream);
+
+/* Attention of a tree of NODES (at most 64) drafted tokens per sequence over
+ * the quantised cache; NODES 1 is an ordinary decode step.  Sequence b has
+ * LEN[b] prefix tokens (int32, taken as 0 if negative) and its nodes follow
+ * them, node j as token LEN[b] + j; token t is offset t % block_size of block
+ * TABLE[b][t / block_size] (int32 [batch][max_blocks]; a block outside the
+ * pool, or past max_blocks, holds no keys).  Node i attends to every prefix
+ * token and to the nodes j whose bit j of MASK[b][i] is set: its ancestors
+ * and itself.  A mask of 0 marks an unused node: its output is zeros and its
+ * LSE -inf, as for a node that finds no key.
+ *   O[b,i,h] = sum_t softmax_t(SCALE q.k_t) v_t,
+ *   LSE[b,i,h] = log sum_t exp(SCALE q.k_t)
+ * Q and O are rows (b, i) of heads*head_dim elements of DTYPE, 16-byte
+ * aligned, Q_STRIDE and O_STRIDE apart; query head h reads key head
+ * h / (heads/kv_heads); LSE is f32 [batch*nodes][heads] or NULL.  Products
+ * are exact in the codes and sums f32.  WORKSPACE holds at least
+ * nl_tree_attn_workspace_bytes(nodes, heads, kv_heads, head_dim) bytes,
+ * 16-byte aligned, or is NULL for the library's own (calls that overlap in
+ * time must then not share it).  Does not synchronise. */
+size_t nl_tree_attn_workspace_bytes(uint32_t nodes, uint32_t heads,
+                                    uint32_t kv_heads, uint32_t head_dim);
+int nl_tree_attn_dev(int fmt, int dtype, const void *Q, uint64_t q_stride,
+                     const void *KC, const uint32_t *KP, const void *VC,
+                     const uint32_t *VP, const int32_t *TABLE,
+                     const int32_t *LEN, const uint64_t *MASK, void *O,
+                     uint64_t o_stride, float *LSE, uint32_t batch,
+                     uint32_t nodes, uint32_t heads, uint32_t kv_heads,
+                     uint32_t head_dim, uint32_t block_size,
+                     uint32_t num_blocks, uint32_t max_blocks, float scale,
+                     void *workspace, size_t ws_bytes, void *stream);
+
 /* ---- the ternary decoder (tensor-parallel) --------------------------- */
 
 /* A LLaMA-style decoder with ternary linears (BitNet-b1.58-2B shaped): RMSNorm,

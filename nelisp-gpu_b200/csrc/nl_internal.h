@@ -67,6 +67,10 @@ extern const int kTrainOpsCount;
 int set_error(int code, const char *fmt, ...);
 int cuda_status(cudaError_t e, const char *what);
 
+// NL_OK once the context exists, creating it on the default device if it does
+// not: the first thing every entry point that launches work asks.
+int api_ready();
+
 // Bounded waits.  A kernel whose bounded wait gives up records it in a
 // host-mapped flag (wait_flag_device(), allocated by nl_init before any
 // capture); the synchronising entry points report and clear it.

@@ -285,6 +285,8 @@ int cuda_status(cudaError_t e, const char *what) {
                    cudaGetErrorString(e), cudaGetErrorName(e));
 }
 
+int api_ready() { return ensure_ready(); }
+
 void count_launches(uint64_t n) {
   if (g.capturing) g.capture_launches += n;
   else g.launches += n;

@@ -83,6 +83,17 @@ SIGNATURES = {
     "nl_ternary_gemv_static_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp]),
     "nl_decode_attn_rope_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32,
                                      ctypes.c_float, _vp]),
+    "nl_qk_norm_rope_dev": (_i, [_i, _vp, _u64] + [_vp] * 5 + [_vp, _u64, _vp, _u64] +
+                            [_u32] * 6 + [_i, ctypes.c_float, _vp]),
+    "nl_qk_norm_rope_bwd_workspace_bytes": (_sz, [_u32]),
+    "nl_qk_norm_rope_bwd_dev": (_i, [_i, _vp, _u64] + [_vp] * 5 + [_vp, _u64] * 3 + [_vp, _vp] +
+                                [_u32] * 6 + [_i, ctypes.c_float, _vp, _sz, _vp]),
+    "nl_kv_append_dev": (_i, [_i, _i, _vp, _u64, _vp, _u64] + [_vp] * 5 + [_u32] * 5 + [_vp]),
+    "nl_kv_read_dev": (_i, [_i, _i] + [_vp] * 5 + [_vp, _u64, _vp, _u64] + [_u32] * 5 + [_vp]),
+    "nl_kv_move_dev": (_i, [_i] + [_vp] * 6 + [_u32] * 6 + [_vp]),
+    "nl_tree_attn_workspace_bytes": (_sz, [_u32] * 4),
+    "nl_tree_attn_dev": (_i, [_i, _i, _vp, _u64] + [_vp] * 8 + [_u64, _vp] + [_u32] * 8 +
+                         [ctypes.c_float, _vp, _sz, _vp]),
     "nl_wait_status": (_i, []),
     "nl_upload_file_ternary": (_i, [ctypes.c_char_p, _u64, _u32, _u32, ctypes.c_int,
                                     ctypes.POINTER(_u32), ctypes.POINTER(_u32)]),
