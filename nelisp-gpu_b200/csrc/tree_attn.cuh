@@ -1,0 +1,889 @@
+// tree_attn.cuh -- attention of a tree of drafted tokens over the quantised
+// paged cache (kv_quant.cuh); one node is an ordinary decode step.
+//
+// For a query row q (a node and a head), over the keys t it sees,
+//   score_t = scale q.k_t,  o = sum_t softmax_t(score) v_t,
+// with k_t = s c (8 bits) or s c + lo (4 bits; c is then taken less 8, and lo
+// with 8 s more), so that
+//   q.k_t = s (q.c) + lo sum(q),   sum_t p_t v_t = sum_t (p_t s_t) c_t + sum_t p_t lo_t:
+// the matrix products run on the codes themselves, small integers that are
+// exact in float16, and the scales meet the scores and the weights in 32 bits.
+// The other operand is normalised to a power of two (a query row by its
+// largest value, the weights p_t s_t by the largest scale met so far) and
+// rounded to float16: one term (11 bits) where the output is bfloat16, whose
+// 8 bits hide it; a second term, the remainder (22 bits), where it is float32.
+//
+// The codes are the first operand of mma.sync m16n8k16 in both products --
+// 16 keys x 8 rows of scores, 16 columns x 8 rows of output -- so a decode
+// step with few rows wastes nothing: rows are padded to 8, not 16, and the
+// state of 8 rows is 32 registers at 128 columns.  The scores come out with a
+// key per lane group and leave as the second operand with a row per lane
+// group: one movmatrix per 8 x 8 weights.
+//
+// Rows of one key head -- nodes x the query heads that share it -- are taken
+// 8 NR WR at a time, an item: NR tiles of 8 rows a warp, WR warps for
+// different rows of the same keys.  The work is the list of the items' runs of
+// key tiles; every CTA takes an equal run of that list whatever the sequences'
+// lengths, keeps the softmax state of one item at a time, and writes the
+// output itself where it has the whole item, or a partial state that a second
+// kernel joins.  The WR warps of 32 keys share a cp.async ring, and nothing
+// else synchronises the CTA until an item ends.
+//
+// Key order.  Row r of a 16-key tile is key 4 (r % 8 / 2) + r % 2 + 2 (r / 8):
+// the second product then takes four successive value rows a lane.  The K
+// index of the score product is permuted so a lane's part of a key is whole
+// 16-byte chunks, and the columns of the second product so a lane's part of a
+// value row is contiguous.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kv_quant.cuh"
+
+namespace nl {
+
+constexpr int kTreeWarps = 4, kTreeThreads = 32 * kTreeWarps;
+constexpr int kTreeKeys = 32;              // keys of a warp's tile
+constexpr uint32_t kTreeMaxCtas = 148 * 4;
+// What an item costs besides its tiles (its queries, the ring's first fill,
+// the join), in tiles: the shares count it, or a CTA whose share is many short
+// items would end long after the others.
+constexpr uint32_t kTreeItemCost = 4;
+
+struct TreeArgs {
+  const void *q;
+  void *o;
+  float *lse;
+  const int32_t *table, *len;
+  const uint64_t *mask;
+  float *part_o, *part_ml;       // partial states: [2 * ctas][rows_at_once][HD], [..][2]
+  uint64_t q_stride, o_stride;
+  KvPool pool;
+  uint32_t batch, nodes, heads, group, rows, row_tiles, max_blocks, ctas;
+  uint32_t rows_at_once, tile;   // rows of an item; keys of a CTA's tile
+  uint32_t block_shift;          // log2(block_size), or 32 if it is not a power of two
+  float scale;                   // scale * log2(e)
+};
+
+// The launches for one head size (k_treeattn_h*.cu): NR and WR follow from
+// the rows.
+template <int HD> cudaError_t tree_attn_start(TreeArgs &a, bool bf16, cudaStream_t st);
+// Rows of an item for ROWS rows of a key head.
+uint32_t tree_rows_at_once(uint32_t rows, uint32_t head_dim);
+
+#ifdef NL_TREE_KERNELS
+namespace {
+
+constexpr uint32_t kNone = ~0u;
+
+// ---- the list of work -----------------------------------------------------
+
+__device__ __forceinline__ uint32_t prefix_of(const TreeArgs &a, uint32_t b) {
+  return (uint32_t)max(__ldg(a.len + b), 0);
+}
+// Tokens of sequence b that the table can hold.
+__device__ __forceinline__ uint32_t keys_of(const TreeArgs &a, uint32_t b) {
+  const uint64_t n = (uint64_t)prefix_of(a, b) + a.nodes;
+  const uint64_t most = (uint64_t)a.max_blocks * a.pool.block_size;
+  return (uint32_t)(n < most ? n : most);
+}
+// Tiles of one of its items: at least one, so that every row is written.
+__device__ __forceinline__ uint32_t tiles_of(const TreeArgs &a, uint32_t b) {
+  const uint32_t n = keys_of(a, b);
+  return n ? (n + a.tile - 1) / a.tile : 1u;
+}
+
+__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// The length of the list: an item counts its tiles and kTreeItemCost.
+__device__ __forceinline__ uint64_t all_cost(const TreeArgs &a) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint64_t v = 0;
+  for (uint32_t b = lane; b < a.batch; b += 32) v += tiles_of(a, b) + kTreeItemCost;
+  return warp_sum(v) * (a.pool.kv_heads * a.row_tiles);
+}
+// The sequence that place AT of the list falls into, and the places before it.
+__device__ __forceinline__ void locate(const TreeArgs &a, uint64_t at, uint32_t *b_out,
+                                       uint64_t *before_out) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t items = (uint64_t)a.pool.kv_heads * a.row_tiles;
+  uint64_t before = 0;
+  for (uint32_t base = 0; base < a.batch; base += 32) {
+    uint64_t mine = base + lane < a.batch ? (tiles_of(a, base + lane) + kTreeItemCost) * items : 0, end = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t up = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= (uint32_t)o) end += up;
+    }
+    end += before;
+    const uint32_t past = __ballot_sync(0xffffffffu, base + lane < a.batch && at < end);
+    if (past) {
+      const int first = __ffs(past) - 1;
+      *b_out = base + first;
+      *before_out = __shfl_sync(0xffffffffu, end - mine, first);
+      return;
+    }
+    before = __shfl_sync(0xffffffffu, end, 31);
+  }
+  *b_out = a.batch;
+  *before_out = before;
+}
+// CTA c of w takes the places [share(c), share(c + 1)).
+__device__ __forceinline__ uint64_t share(uint64_t total, uint32_t w, uint32_t c) {
+  return total / w * c + total % w * c / w;
+}
+__device__ __forceinline__ uint32_t owner(uint64_t total, uint32_t w, uint64_t at) {
+  uint32_t c = (uint32_t)((double)at * w / (double)total);
+  if (c >= w) c = w - 1;
+  while (c + 1 < w && share(total, w, c + 1) <= at) c++;
+  while (c > 0 && share(total, w, c) > at) c--;
+  return c;
+}
+
+// ---- small device helpers ---------------------------------------------------
+
+__device__ __forceinline__ uint32_t su32(const void *p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src),
+               "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src),
+               "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() {
+  asm volatile("cp.async.commit_group;\n" ::: "memory");
+}
+template <int N> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void mma16(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
+__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
+
+// The 8 x 8 matrix of 16-bit values whose row g, columns 2t and 2t + 1, lane
+// (g, t) holds, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
+}
+// o += codes x weights.  The tensor core cuts, not rounds, what it adds to an
+// accumulator, and over a long context that drifts; where the output is
+// float32 each 16 keys are summed apart and added in float32.
+template <int Terms, int NR>
+__device__ __forceinline__ void weigh(float (&o)[4], const uint4 &c,
+                                      const uint32_t (&p)[Terms][NR][2], int n) {
+  if (Terms == 1) {
+    mma16(o, c, p[0][n][0], p[0][n][1]);
+  } else {
+    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = Terms - 1; e >= 0; e--) mma16(d, c, p[e][n][0], p[e][n][1]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] += d[i];
+  }
+}
+
+// Two bytes u, v (0 .. 255) of W, placed as float16 1024 + u, 1024 + v by the
+// selector, less 1152: the signed codes u - 128, v - 128, exactly.
+__device__ __forceinline__ uint32_t codes8(uint32_t w, uint32_t sel) {
+  return h2(__hsub2(as_h2(__byte_perm(w, 0x64646464u, sel)), as_h2(0x64806480u)));
+}
+// The nibbles at bits 0 and 16 (4 and 20) of W, less 8, as float16.
+__device__ __forceinline__ uint32_t codes4_low(uint32_t w) {
+  return h2(__hsub2(as_h2((w & 0x000f000fu) | 0x64006400u), as_h2(0x64086408u)));
+}
+__device__ __forceinline__ uint32_t codes4_high(uint32_t w) {
+  return h2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), as_h2(0x2c002c00u),
+                    as_h2(0xd480d480u)));   // (1024 + 16 c) / 16 - 64 - 8
+}
+// Scale and offset of a parameter word.  Four-bit codes are used less 8, so
+// the offset is that of the middle of the range: with it at the low end the
+// two sums q.c and lo sum(q) would be large and of opposite signs.
+template <int BITS> __device__ __forceinline__ float scale_of(uint32_t w) {
+  return __uint_as_float(BITS == 8 ? w : w << 16);
+}
+__device__ __forceinline__ float middle_of(uint32_t w) {
+  return fmaf(8.0f, __uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// ---- geometry -----------------------------------------------------------------
+
+template <int HD, int BITS> struct Geo {
+  static constexpr int RB = HD * BITS / 8;            // bytes of a row
+  static constexpr int Chunks = RB / 16;
+  static constexpr int Steps = HD / 16;               // k16 steps of the score product
+  static constexpr int Words = HD * BITS / 128;       // words of a key a lane holds
+  static constexpr int MT = HD / 16;                  // 16-column tiles of the second product
+  static constexpr int Stage = 2 * kTreeKeys * RB + 2 * kTreeKeys * 4 + 16;   // codes, words, valid
+  // Byte of chunk c of key k: key rows read together by the lanes of a score
+  // tile (two apart) and value rows read together by those of the second
+  // product (four apart) are kept off each other's banks.
+  static __device__ __forceinline__ uint32_t k_at(uint32_t key, uint32_t c) {
+    return key * RB + (RB >= 128 ? c ^ ((key & 1) << 2) : c) * 16;
+  }
+  static __device__ __forceinline__ uint32_t v_at(uint32_t key, uint32_t c) {
+    return (((key * Chunks + c) ^ (((key >> 2) & 3) << 1))) * 16;
+  }
+  // Column d of the output that lane group g holds as its column nt.
+  static __device__ __forceinline__ uint32_t column(uint32_t g, uint32_t nt) {
+    if (HD == 256 && BITS == 8) return nt / 16 * 128 + 16 * g + nt % 16;
+    return HD / 8 * g + nt;
+  }
+  // Where element d of a query row goes among the operand fragments: step,
+  // lane of the quad, which of the two registers, which half.
+  static __device__ __forceinline__ void spot(uint32_t d, uint32_t *step, uint32_t *t, uint32_t *p,
+                                              uint32_t *i) {
+    if (BITS == 8) {
+      const uint32_t c = d / 16;
+      *t = c & 3;
+      *step = c / 4 * 4 + d % 16 / 4;
+      *p = d % 4 / 2;
+      *i = d % 2;
+    } else {
+      constexpr uint32_t per = HD == 64 ? 16 : 32;    // elements of a lane's contiguous part
+      const uint32_t c = d / per, e = d % 8;
+      *t = c & 3;
+      *step = 2 * (c / 4 * 4 + d % per / 8) + ((e >> 1) & 1);
+      *p = e & 1;
+      *i = e >> 2;
+    }
+  }
+};
+
+template <typename T, int HD, int BITS, int NR, int WR> struct Plan {
+  using G = Geo<HD, BITS>;
+  static constexpr int Terms = sizeof(T) == 4 ? 2 : 1;
+  static constexpr int WK = kTreeWarps / WR;                // warps with keys of their own
+  static constexpr int Rows = 8 * NR * WR, Tile = kTreeKeys * WK;
+  static constexpr int Q = Terms * Rows * HD * 2;           // query fragments
+  static constexpr int Stages = WR > 1 ? 4 : G::RB <= 64 ? 4 : G::RB <= 128 ? 3 : 2;
+  static constexpr int Ring = WK * Stages * G::Stage;
+  static constexpr int Pitch = HD + 4;                      // floats of a row when states are joined
+  static constexpr int Join = WK * Rows * Pitch * 4;        // over the fragments and the ring
+  // row factors, row sums, masks, per-warp (max, sum)
+  static constexpr int Small = Rows * 4 + Rows * 4 + Rows * 8 + WK * Rows * 8;
+  static constexpr int Bytes = Small + (Q + Ring > Join ? Q + Ring : Join);
+};
+
+template <typename T> __device__ __forceinline__ float load1(const T *p);
+template <> __device__ __forceinline__ float load1<float>(const float *p) { return __ldg(p); }
+template <> __device__ __forceinline__ float load1<__nv_bfloat16>(const __nv_bfloat16 *p) {
+  return __bfloat162float(__ldg(p));
+}
+__device__ __forceinline__ void store1(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <typename T, int HD, int BITS, int NR, int WR>
+__global__ void __launch_bounds__(kTreeThreads)
+tree_attn_kernel(const __grid_constant__ TreeArgs a) {
+  using G = Geo<HD, BITS>;
+  using P = Plan<T, HD, BITS, NR, WR>;
+  constexpr int Terms = P::Terms, WK = P::WK, Stages = P::Stages;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float *row_f = reinterpret_cast<float *>(smem);                    // factor of a row's scores
+  float *row_sum = row_f + P::Rows;                                  // sum of its query
+  uint64_t *row_mask = reinterpret_cast<uint64_t *>(row_sum + P::Rows);
+  float2 *ml = reinterpret_cast<float2 *>(row_mask + P::Rows);       // [WK][Rows]
+  uint8_t *qf = reinterpret_cast<uint8_t *>(ml + WK * P::Rows);
+  uint8_t *ring = qf + P::Q;
+  float *join = reinterpret_cast<float *>(qf);
+
+  pdl_trigger();
+  pdl_wait();
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t wr = warp % WR, wk = warp / WR;
+  const uint64_t total = all_cost(a);
+  const uint32_t workers = total < a.ctas ? (uint32_t)total : a.ctas;
+  if (blockIdx.x >= workers) return;
+  uint64_t at = share(total, workers, blockIdx.x);
+  const uint64_t end = share(total, workers, blockIdx.x + 1);
+  uint32_t b;
+  uint64_t before;
+  locate(a, at, &b, &before);
+  const uint32_t items = a.pool.kv_heads * a.row_tiles;
+  uint8_t *mine = ring + wk * (Stages * G::Stage);
+  const uint64_t used = a.nodes < 64 ? (1ull << a.nodes) - 1 : ~0ull;
+  // Byte of lane (row % 8, quad)'s fragment of a step: one tile of 8 rows
+  // (8 bytes) or two side by side (16).
+  auto fragment = [](uint32_t row, uint32_t step, uint32_t quad) {
+    const uint32_t l = (row & 7) * 4 + quad;
+    if (NR == 1) return ((row / 8 * G::Steps + step) * 32 + l) * 8;
+    return ((row / 16 * G::Steps + step) * 32 + l) * 16 + (row / 8 & 1) * 8;
+  };
+
+  while (at < end) {
+    // ---- the next item, or part of one ----
+    const uint32_t tiles = tiles_of(a, b), cost = tiles + kTreeItemCost;
+    if (at >= before + (uint64_t)cost * items) {
+      before += (uint64_t)cost * items;
+      b++;
+      continue;
+    }
+    const uint32_t item = (uint32_t)((at - before) / cost), c0 = (uint32_t)((at - before) % cost);
+    const uint32_t c1 = end - at < cost - c0 ? c0 + (uint32_t)(end - at) : cost;
+    at += c1 - c0;
+    if (c1 <= kTreeItemCost) continue;             // its share ends before the first tile
+    const uint32_t t0 = c0 > kTreeItemCost ? c0 - kTreeItemCost : 0, t1 = c1 - kTreeItemCost;
+    const uint32_t head = item / a.row_tiles, row0 = item % a.row_tiles * P::Rows;
+    const uint32_t prefix = prefix_of(a, b), keys = keys_of(a, b);
+
+    // ---- keys on their way ----
+    // The pool row of this lane's key of a tile, kNone where there is none.
+    auto find = [&](uint32_t tile) {
+      const uint32_t key = tile * P::Tile + wk * kTreeKeys + lane;
+      if (tile >= t1 || key >= keys) return kNone;
+      const uint32_t page = a.block_shift < 32 ? key >> a.block_shift : key / a.pool.block_size;
+      const uint32_t off = key - page * a.pool.block_size;
+      const uint32_t block = (uint32_t)__ldg(a.table + (uint64_t)b * a.max_blocks + page);
+      return block < a.pool.num_blocks ? kv_row(a.pool, block, off, head) : kNone;
+    };
+    auto request = [&](uint32_t row, uint32_t slot) {
+      const uint32_t valid = __ballot_sync(0xffffffffu, row != kNone);
+      uint8_t *st = mine + slot * G::Stage;
+      const uint32_t s0 = su32(st), words = s0 + 2 * kTreeKeys * G::RB;
+      const bool on = row != kNone;
+      if (WR == 1 || wr == 0) {
+        copy4(words + lane * 4, a.pool.param[0] + (on ? row : 0), on);
+        copy4(words + 128 + lane * 4, a.pool.param[1] + (on ? row : 0), on);
+        if (lane == 0) *reinterpret_cast<uint32_t *>(st + 2 * kTreeKeys * G::RB + 256) = valid;
+      }
+#pragma unroll
+      for (int i = 0; i < (G::Chunks + WR - 1) / WR; i++) {
+        const uint32_t n = (i * WR + wr) * 32 + lane;
+        if (G::Chunks % WR != 0 && n >= kTreeKeys * G::Chunks) break;   // the whole warp
+        const uint32_t k = n / G::Chunks, c = n % G::Chunks;
+        const uint32_t from = __shfl_sync(0xffffffffu, row, k);
+        const bool have = from != kNone;
+        const uint64_t byte = (uint64_t)(have ? from : 0) * G::RB + c * 16;
+        copy16(s0 + G::k_at(k, c), a.pool.code[0] + byte, have);
+        copy16(s0 + kTreeKeys * G::RB + G::v_at(k, c), a.pool.code[1] + byte, have);
+      }
+    };
+    __syncthreads();               // the last item's states are joined
+    uint32_t next = find(t0);
+#pragma unroll
+    for (int i = 0; i < Stages - 1; i++) {
+      if (t0 + i < t1) request(next, i);
+      copy_commit();
+      next = find(t0 + i + 1);
+    }
+
+    // ---- the query rows, as operand fragments: 8 threads a row ----
+    for (uint32_t r = threadIdx.x / 8; r < P::Rows; r += kTreeThreads / 8) {
+      constexpr int Per = HD / 8;
+      const uint32_t part = threadIdx.x % 8, row = row0 + r;
+      const bool live = row < a.rows;
+      const uint32_t node = live ? row / a.group : 0;
+      const T *q = (const T *)a.q + ((uint64_t)b * a.nodes + node) * a.q_stride +
+                   (uint64_t)(head * a.group + (live ? row % a.group : 0)) * HD + part * Per;
+      float v[Per], top = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < Per; i++) {
+        v[i] = live ? load1(q + i) : 0.0f;
+        top = fmaxf(top, fabsf(v[i]));
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // the power of two that brings the largest value to [2^13, 2^14)
+      int up = 140 - (int)(__float_as_uint(top) >> 23);
+      if (top == 0.0f || !(top < INFINITY)) up = 0;
+      up = min(up, 126);
+      const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+      for (int i = 0; i < Per; i++) {
+        v[i] *= mul;
+        sum += v[i];
+        uint32_t step, quad, p, half;
+        G::spot(part * Per + i, &step, &quad, &p, &half);
+        const uint32_t byte = fragment(r, step, quad) + p * 4 + half * 2;
+        const __half hi = __float2half_rn(v[i]);
+        *reinterpret_cast<__half *>(qf + byte) = hi;
+        if (Terms == 2)
+          *reinterpret_cast<__half *>(qf + P::Rows * HD * 2 + byte) =
+              __float2half_rn(v[i] - __half2float(hi));
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (part == 0) {
+        // never zero: a factor of zero would make NaN of a masked score
+        row_f[r] = fmaxf(a.scale * __uint_as_float((uint32_t)(127 - up) << 23), 1.17549435e-38f);
+        row_sum[r] = sum;
+        row_mask[r] = live ? a.mask[(uint64_t)b * a.nodes + node] & used : 0;
+      }
+    }
+    __syncthreads();
+
+    const uint32_t r0 = wr * (8 * NR) + 2 * t;      // rows r0 + 8 n and the next are this lane's
+    float o[G::MT][NR][4];
+#pragma unroll
+    for (int i = 0; i < G::MT; i++)
+#pragma unroll
+      for (int n = 0; n < NR; n++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
+    float m[NR][2], l[NR][2], base[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) m[n][r] = -INFINITY, l[n][r] = base[n][r] = 0.0f;
+    float vs = 1.0f;               // the weights are p s vs
+    uint32_t vlimit = 0;           // scales below these bits fit vs
+
+    for (uint32_t tile = t0; tile < t1; tile++) {
+      copy_wait<Stages - 2>();
+      if (WR == 1) __syncwarp();
+      else asm volatile("bar.sync %0, %1;\n" ::"r"(1 + wk), "n"(32 * WR) : "memory");
+      // the slot of the tile before this one: every warp of the ring is past it
+      if (tile + Stages - 1 < t1) request(next, (tile - t0 + Stages - 1) % Stages);
+      copy_commit();
+      next = find(tile + Stages);
+
+      const uint8_t *st = mine + (tile - t0) % Stages * G::Stage;
+      const uint8_t *kc = st, *vc = st + kTreeKeys * G::RB;
+      const uint32_t *kw = reinterpret_cast<const uint32_t *>(st + 2 * kTreeKeys * G::RB);
+      const uint32_t *vw = kw + 32;
+      const uint32_t valid = vw[32];
+      const uint32_t k0 = tile * P::Tile + wk * kTreeKeys;
+      const uint32_t krow = 4 * (g >> 1) + (g & 1);  // and two keys on
+
+      // scores of 32 keys x 8 NR rows, in units of the normalised queries
+      float s[2][NR][4];
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int n = 0; n < NR; n++) s[k][n][0] = s[k][n][1] = s[k][n][2] = s[k][n][3] = 0.0f;
+#pragma unroll
+      for (int h = 0; h < (G::Words + 3) / 4; h++) {
+        uint32_t w[2][2][4];
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            const uint32_t key = 16 * k + 2 * u + krow;
+            if (G::Words == 2) {
+              const uint2 x = *reinterpret_cast<const uint2 *>(kc + key * G::RB + t * 8);
+              w[k][u][0] = x.x; w[k][u][1] = x.y;
+            } else {
+              const uint4 x = *reinterpret_cast<const uint4 *>(kc + G::k_at(key, t + 4 * h));
+              w[k][u][0] = x.x; w[k][u][1] = x.y; w[k][u][2] = x.z; w[k][u][3] = x.w;
+            }
+          }
+#pragma unroll
+        for (int i = 0; i < (G::Words < 4 ? G::Words : 4); i++) {
+#pragma unroll
+          for (int half = 0; half < (BITS == 8 ? 1 : 2); half++) {
+            const int step = BITS == 8 ? 4 * h + i : 2 * (4 * h + i) + half;
+            uint32_t q[Terms][NR][2];
+#pragma unroll
+            for (int e = 0; e < Terms; e++) {
+              const uint8_t *from = qf + e * (P::Rows * HD * 2);
+              if (NR == 1) {
+                const uint2 x = *reinterpret_cast<const uint2 *>(from + fragment(8 * wr + g, step, t));
+                q[e][0][0] = x.x; q[e][0][1] = x.y;
+              } else {
+#pragma unroll
+                for (int n = 0; n < NR; n += 2) {
+                  const uint4 x = *reinterpret_cast<const uint4 *>(
+                      from + fragment(8 * NR * wr + 8 * n + g, step, t));
+                  q[e][n][0] = x.x; q[e][n][1] = x.y;
+                  q[e][n + 1 < NR ? n + 1 : 0][0] = x.z; q[e][n + 1 < NR ? n + 1 : 0][1] = x.w;
+                }
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              uint4 c;
+              if (BITS == 8) {
+                c = make_uint4(codes8(w[k][0][i], 0x4140), codes8(w[k][1][i], 0x4140),
+                               codes8(w[k][0][i], 0x4342), codes8(w[k][1][i], 0x4342));
+              } else {
+                const uint32_t x = half ? w[k][0][i] >> 8 : w[k][0][i];
+                const uint32_t y = half ? w[k][1][i] >> 8 : w[k][1][i];
+                c = make_uint4(codes4_low(x), codes4_low(y), codes4_high(x), codes4_high(y));
+              }
+#pragma unroll
+              for (int e = Terms - 1; e >= 0; e--)
+#pragma unroll
+                for (int n = 0; n < NR; n++) mma16(s[k][n], c, q[e][n][0], q[e][n][1]);
+            }
+          }
+        }
+      }
+
+      // scales, offsets and masks: s becomes the score over the row's factor
+      const bool whole = k0 + kTreeKeys <= prefix && valid == 0xffffffffu;
+      float f[NR][2], top[NR][2];
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const uint32_t wa = kw[16 * k + krow], wb = kw[16 * k + krow + 2];
+        const float sa = scale_of<BITS>(wa), sb = scale_of<BITS>(wb);
+        const float ma = middle_of(wa), mb = middle_of(wb);
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+          float2 sum = make_float2(0.0f, 0.0f);
+          if (BITS == 4) sum = *reinterpret_cast<const float2 *>(row_sum + r0 + 8 * n);
+          float (&x)[4] = s[k][n];
+          x[0] *= sa; x[1] *= sa; x[2] *= sb; x[3] *= sb;
+          if (BITS == 4) {
+            x[0] = fmaf(ma, sum.x, x[0]); x[1] = fmaf(ma, sum.y, x[1]);
+            x[2] = fmaf(mb, sum.x, x[2]); x[3] = fmaf(mb, sum.y, x[3]);
+          }
+        }
+      }
+      uint32_t see[NR][2];
+      if (!whole) {
+        const uint32_t pre = k0 >= prefix ? 0u
+                             : prefix - k0 >= 32 ? 0xffffffffu : (1u << (prefix - k0)) - 1u;
+#pragma unroll
+        for (int n = 0; n < NR; n++)
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            const uint64_t w = row_mask[r0 + 8 * n + r];
+            uint32_t nodes = 0;
+            if (k0 >= prefix) nodes = k0 - prefix < 64 ? (uint32_t)(w >> (k0 - prefix)) : 0u;
+            else if (prefix - k0 < 32) nodes = (uint32_t)(w << (prefix - k0));
+            see[n][r] = ((pre | nodes) & valid) >> krow;     // this lane's keys: 0, 2, 16, 18
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+              for (int u = 0; u < 2; u++)
+                if (!(see[n][r] >> (16 * k + 2 * u) & 1)) s[k][n][2 * u + r] = -INFINITY;
+          }
+      }
+      bool moved = false;
+#pragma unroll
+      for (int n = 0; n < NR; n++) {
+        const float2 ff = *reinterpret_cast<const float2 *>(row_f + r0 + 8 * n);
+        f[n][0] = ff.x; f[n][1] = ff.y;
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          float v = fmaxf(fmaxf(s[0][n][r], s[0][n][2 + r]), fmaxf(s[1][n][r], s[1][n][2 + r]));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          top[n][r] = fmaxf(v, m[n][r]);
+          moved |= top[n][r] != m[n][r];
+        }
+      }
+      // the largest finite scale of the values decides the weights' power of two
+      uint32_t big = BITS == 8 ? vw[lane] : vw[lane] << 16;
+      big = __reduce_max_sync(0xffffffffu, big < 0x7f800000u ? big : 0u);
+      float ratio = 1.0f;
+      if (big >= vlimit && big != 0) {
+        const uint32_t e = (big >> 23) + 1;             // scales below 2^(e - 127)
+        vlimit = e << 23;
+        const float next_vs = __uint_as_float((269u - e) << 23);   // to below 2^15
+        ratio = next_vs / vs;
+        vs = next_vs;
+        moved = true;
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+          float c[2];
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            const float keep = top[n][r] == m[n][r] ? 1.0f : ex2((m[n][r] - top[n][r]) * f[n][r]);
+            l[n][r] *= keep;
+            base[n][r] *= keep;
+            c[r] = keep * ratio;
+            m[n][r] = top[n][r];
+          }
+#pragma unroll
+          for (int i = 0; i < G::MT; i++) {
+            o[i][n][0] *= c[0]; o[i][n][1] *= c[1];
+            o[i][n][2] *= c[0]; o[i][n][3] *= c[1];
+          }
+        }
+      }
+
+      // weights, and the second product
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const uint32_t wa = vw[16 * k + krow], wb = vw[16 * k + krow + 2];
+        const float sc[2] = {scale_of<BITS>(wa) * vs, scale_of<BITS>(wb) * vs};
+        const float mid[2] = {middle_of(wa), middle_of(wb)};
+        uint32_t p[Terms][NR][2];
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+          float off[2];
+#pragma unroll
+          for (int r = 0; r < 2; r++) off[r] = m[n][r] == -INFINITY ? 0.0f : -m[n][r] * f[n][r];
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            float e[2];
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+              e[r] = ex2(fmaf(s[k][n][2 * u + r], f[n][r], off[r]));
+              l[n][r] += e[r];
+              const bool seen = whole || (see[n][r] >> (16 * k + 2 * u) & 1);
+              if (BITS == 4 && seen) base[n][r] = fmaf(e[r], mid[u], base[n][r]);
+              e[r] = seen ? e[r] * sc[u] : 0.0f;
+            }
+            const __half2 hi = __floats2half2_rn(e[0], e[1]);
+            p[0][n][u] = transpose8(h2(hi));
+            if (Terms == 2)
+              p[Terms - 1][n][u] = transpose8(
+                  h2(__floats2half2_rn(e[0] - __low2float(hi), e[1] - __high2float(hi))));
+          }
+        }
+        // a lane's part of the four value rows, in groups of 4 (8 bits) or 8
+        // (4 bits) columns a word
+        constexpr int VW = G::RB / 32;                   // words of a row a lane holds
+        constexpr int VL = VW < 4 ? VW : 4;              // at a time
+#pragma unroll
+        for (int h = 0; h < VW / VL; h++) {
+          uint32_t w[4][VL];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t key = 16 * k + 4 * t + i;
+            if (VW == 1) {
+              w[i][0] = *reinterpret_cast<const uint32_t *>(vc + G::v_at(key, g / 4) + g % 4 * 4);
+            } else if (VW == 2) {
+              const uint2 y = *reinterpret_cast<const uint2 *>(vc + G::v_at(key, g / 2) + g % 2 * 8);
+              w[i][0] = y.x; w[i][VL - 1] = y.y;
+            } else {
+              const uint4 y = *reinterpret_cast<const uint4 *>(vc + G::v_at(key, g + 8 * h));
+              w[i][0] = y.x; w[i][1 % VL] = y.y; w[i][2 % VL] = y.z; w[i][3 % VL] = y.w;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < VL; j++) {
+            if (BITS == 8) {
+#pragma unroll
+              for (int u = 0; u < 2; u++) {              // bytes 2u, 2u + 1
+                const uint32_t sel = u ? 0x7362 : 0x5140;
+                const uint32_t ab = __byte_perm(w[0][j], w[1][j], sel);
+                const uint32_t cd = __byte_perm(w[2][j], w[3][j], sel);
+                const uint4 c = make_uint4(codes8(ab, 0x4140), codes8(ab, 0x4342),
+                                           codes8(cd, 0x4140), codes8(cd, 0x4342));
+#pragma unroll
+                for (int n = 0; n < NR; n++)
+                  weigh<Terms, NR>(o[2 * (VL * h + j) + u][n], c, p, n);
+              }
+            } else {
+#pragma unroll
+              for (int u = 0; u < 4; u++) {              // byte u: columns 2u, 2u + 1
+                const uint32_t sel = u < 2 ? 0x5410 : 0x7632;
+                uint32_t ab = __byte_perm(w[0][j], w[1][j], sel);
+                uint32_t cd = __byte_perm(w[2][j], w[3][j], sel);
+                if (u & 1) ab >>= 8, cd >>= 8;
+                const uint4 c = make_uint4(codes4_low(ab), codes4_high(ab), codes4_low(cd),
+                                           codes4_high(cd));
+#pragma unroll
+                for (int n = 0; n < NR; n++)
+                  weigh<Terms, NR>(o[4 * (VL * h + j) + u][n], c, p, n);
+              }
+            }
+          }
+        }
+      }
+    }
+    copy_wait<0>();
+
+    // ---- join the warps' states ----
+#pragma unroll
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], x);
+          if (BITS == 4) base[n][r] += __shfl_xor_sync(0xffffffffu, base[n][r], x);
+        }
+        const uint32_t row = r0 + 8 * n + r;
+        const float mm = m[n][r] == -INFINITY ? m[n][r] : m[n][r] * row_f[row];
+        if (g == 0) ml[wk * P::Rows + row] = make_float2(mm, l[n][r]);
+      }
+    __syncthreads();               // every warp is done with the fragments and its ring
+    {
+      const float back = 1.0f / vs;
+#pragma unroll
+      for (int n = 0; n < NR; n++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          float *to = join + (wk * P::Rows + r0 + 8 * n + r) * P::Pitch;
+#pragma unroll
+          for (int i = 0; i < G::MT; i++)
+            *reinterpret_cast<float2 *>(to + G::column(g, 2 * i)) =
+                make_float2(fmaf(o[i][n][r], back, base[n][r]),
+                            fmaf(o[i][n][2 + r], back, base[n][r]));
+        }
+    }
+    __syncthreads();
+    for (uint32_t r = threadIdx.x / 8; r < P::Rows; r += kTreeThreads / 8) {
+      constexpr int Per = HD / 8;
+      const uint32_t part = threadIdx.x % 8, row = row0 + r;
+      float top = -INFINITY, sum = 0.0f, c[WK];
+#pragma unroll
+      for (int w = 0; w < WK; w++) top = fmaxf(top, ml[w * P::Rows + r].x);
+#pragma unroll
+      for (int w = 0; w < WK; w++) {
+        const float2 v = ml[w * P::Rows + r];
+        c[w] = v.x == -INFINITY ? 0.0f : ex2(v.x - top);
+        // a row of NaN scores has the maximum -inf and a sum that is NaN
+        if (v.x == -INFINITY && v.y != v.y) c[w] = 1.0f;
+        sum = fmaf(c[w], v.y, sum);
+      }
+      const bool part_of = !(t0 == 0 && t1 == tiles);
+      const uint32_t slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+      const bool empty = row_mask[r] == 0 || sum == 0.0f;
+      const float inv = 1.0f / sum;
+      const uint32_t node = row / a.group, h = head * a.group + row % a.group;
+      const uint64_t out_row = (uint64_t)b * a.nodes + node;
+#pragma unroll
+      for (int i = 0; i < Per; i++) {
+        const uint32_t d = i * 8 + part;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WK; w++)
+          v = c[w] == 0.0f ? v : fmaf(c[w], join[(w * P::Rows + r) * P::Pitch + d], v);
+        if (part_of) {
+          a.part_o[((uint64_t)slot * P::Rows + r) * HD + d] = v;
+        } else if (row < a.rows) {
+          store1((T *)a.o + out_row * a.o_stride + (uint64_t)h * HD + d, empty ? 0.0f : v * inv);
+        }
+      }
+      if (part == 0) {
+        if (part_of) {
+          a.part_ml[((uint64_t)slot * P::Rows + r) * 2] = top;
+          a.part_ml[((uint64_t)slot * P::Rows + r) * 2 + 1] = sum;
+        } else if (row < a.rows && a.lse) {
+          a.lse[out_row * a.heads + h] =
+              empty ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+        }
+      }
+    }
+  }
+}
+
+// Joins the partial states of the items that several CTAs share: a block per
+// output row.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kTreeThreads)
+tree_join_kernel(const __grid_constant__ TreeArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float red[kTreeWarps][HD + 2];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t h = blockIdx.x % a.heads, bn = blockIdx.x / a.heads;
+  const uint32_t b = bn / a.nodes, row = bn % a.nodes * a.group + h % a.group;
+  const uint64_t total = all_cost(a);
+  const uint32_t workers = total < a.ctas ? (uint32_t)total : a.ctas;
+  uint64_t before = 0;
+  {
+    for (uint32_t i = lane; i < b; i += 32) before += tiles_of(a, i) + kTreeItemCost;
+    before = warp_sum(before) * ((uint64_t)a.pool.kv_heads * a.row_tiles);
+  }
+  const uint32_t tiles = tiles_of(a, b);
+  const uint64_t s0 = before + kTreeItemCost +
+                      (uint64_t)(h / a.group * a.row_tiles + row / a.rows_at_once) *
+                          (tiles + kTreeItemCost);
+  const uint32_t c0 = owner(total, workers, s0), c1 = owner(total, workers, s0 + tiles - 1);
+  if (c0 == c1) return;
+  constexpr int Per = HD / 32;
+  float v[Per], m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < Per; i++) v[i] = 0.0f;
+  for (uint32_t c = c0 + warp; c <= c1; c += kTreeWarps) {
+    const uint64_t at =
+        (uint64_t)(2 * c + (c == c0 ? 1 : 0)) * a.rows_at_once + row % a.rows_at_once;
+    const float pm = a.part_ml[2 * at], pl = a.part_ml[2 * at + 1];
+    if (pm == -INFINITY && pl == 0.0f) continue;
+    const float top = fmaxf(m, pm);
+    const float old = m == top ? 1.0f : ex2(m - top), add = pm == top ? 1.0f : ex2(pm - top);
+    m = top;
+    l = fmaf(l, old, pl * add);
+#pragma unroll
+    for (int i = 0; i < Per; i++) v[i] = fmaf(v[i], old, a.part_o[at * HD + i * 32 + lane] * add);
+  }
+#pragma unroll
+  for (int i = 0; i < Per; i++) red[warp][i * 32 + lane] = v[i];
+  if (lane == 0) red[warp][HD] = m, red[warp][HD + 1] = l;
+  __syncthreads();
+  float top = -INFINITY, sum = 0.0f, c[kTreeWarps];
+#pragma unroll
+  for (int w = 0; w < kTreeWarps; w++) top = fmaxf(top, red[w][HD]);
+#pragma unroll
+  for (int w = 0; w < kTreeWarps; w++) {
+    c[w] = red[w][HD] == top ? 1.0f : ex2(red[w][HD] - top);
+    sum = fmaf(c[w], red[w][HD + 1], sum);
+  }
+  const uint64_t words = a.mask[bn] & (a.nodes < 64 ? (1ull << a.nodes) - 1 : ~0ull);
+  const bool empty = words == 0 || sum == 0.0f;
+  const float inv = 1.0f / sum;
+  for (uint32_t d = threadIdx.x; d < HD; d += kTreeThreads) {
+    float y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kTreeWarps; w++) y = fmaf(c[w], red[w][d], y);
+    store1((T *)a.o + (uint64_t)bn * a.o_stride + (uint64_t)h * HD + d, empty ? 0.0f : y * inv);
+  }
+  if (threadIdx.x == 0 && a.lse)
+    a.lse[(uint64_t)bn * a.heads + h] =
+        empty ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
+template <typename T, int HD, int BITS, int NR, int WR>
+cudaError_t start(TreeArgs &a, cudaStream_t st) {
+  using P = Plan<T, HD, BITS, NR, WR>;
+  static int per_sm = 0;
+  if (!per_sm) {
+    cudaError_t e = cudaFuncSetAttribute(tree_attn_kernel<T, HD, BITS, NR, WR>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, P::Bytes);
+    if (e != cudaSuccess) return e;
+    int n = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, tree_attn_kernel<T, HD, BITS, NR, WR>,
+                                                      kTreeThreads, P::Bytes);
+    if (e != cudaSuccess) return e;
+    per_sm = n < 1 ? 1 : n > 4 ? 4 : n;
+  }
+  a.ctas = 148u * per_sm;
+  a.tile = P::Tile;
+  cudaError_t e = launch_pdl(tree_attn_kernel<T, HD, BITS, NR, WR>, dim3(a.ctas),
+                             dim3(kTreeThreads), (size_t)P::Bytes, st, a);
+  if (e != cudaSuccess) return e;
+  count_launches(2);
+  return launch_pdl(tree_join_kernel<T, HD>, dim3(a.batch * a.nodes * a.heads), dim3(kTreeThreads),
+                    0, st, a);
+}
+template <typename T, int HD, int BITS>
+cudaError_t start_rows(TreeArgs &a, cudaStream_t st) {
+  constexpr int Most = HD == 256 ? 2 : 4;        // row tiles a warp has registers for
+  if (a.rows_at_once == 8) return start<T, HD, BITS, 1, 1>(a, st);
+  if (a.rows_at_once == 16) return start<T, HD, BITS, 2, 1>(a, st);
+  if (a.rows_at_once == 32) return start<T, HD, BITS, Most, 4 / Most>(a, st);
+  if (a.rows_at_once == 64) return start<T, HD, BITS, Most, 8 / Most>(a, st);
+  if constexpr (Most == 4) return start<T, HD, BITS, Most, 4>(a, st);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+template <int HD>
+cudaError_t tree_attn_start(TreeArgs &a, bool bf16, cudaStream_t st) {
+  if (a.pool.bits == 8)
+    return bf16 ? start_rows<__nv_bfloat16, HD, 8>(a, st) : start_rows<float, HD, 8>(a, st);
+  return bf16 ? start_rows<__nv_bfloat16, HD, 4>(a, st) : start_rows<float, HD, 4>(a, st);
+}
+#endif  // NL_TREE_KERNELS
+
+}  // namespace nl

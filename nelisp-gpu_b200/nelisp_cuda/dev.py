@@ -30,9 +30,13 @@ def _p(t):
 
 
 def _stream(stream=None):
+    """The cudaStream_t of STREAM, or of torch's current stream on the
+    library's device (read raw: building a Stream object for it costs more
+    than the rest of a call)."""
+    if stream is not None:
+        return stream.cuda_stream
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return ctypes.c_void_p(s.cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _check_tensor(t, dtype_name):
