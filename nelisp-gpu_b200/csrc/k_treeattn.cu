@@ -2,7 +2,7 @@
 // the quantised paged cache.  The kernels are in tree_attn.cuh, compiled per
 // head size in k_treeattn_h*.cu.
 
-#include "tree_attn.cuh"
+#include "tree_work.cuh"
 
 namespace nl {
 
@@ -73,7 +73,9 @@ extern "C" int nl_tree_attn_dev(int fmt, int dtype, const void *Q, uint64_t q_st
   a.q_stride = q_stride; a.o_stride = o_stride;
   a.batch = batch; a.nodes = nodes; a.heads = heads; a.group = heads / kv_heads;
   a.rows = a.group * nodes;
-  a.rows_at_once = tree_rows_at_once(a.rows, head_dim);
+  const bool bf16 = dtype == NL_BF16;
+  const uint32_t umma_rows = tree_umma_rows(a, bf16);
+  a.rows_at_once = umma_rows ? umma_rows : tree_rows_at_once(a.rows, head_dim);
   a.row_tiles = (a.rows + a.rows_at_once - 1) / a.rows_at_once;
   a.block_shift = 32;
   for (uint32_t s = 0; s < 32; s++)
@@ -84,10 +86,17 @@ extern "C" int nl_tree_attn_dev(int fmt, int dtype, const void *Q, uint64_t q_st
     for (int i = 0; i < 2; i++)
       a.pool.code[i] = (uint8_t *)workspace, a.pool.param[i] = (uint32_t *)workspace;
   a.part_o = (float *)workspace;
-  a.part_ml = a.part_o + (size_t)2 * kTreeMaxCtas * a.rows_at_once * head_dim;
-  const bool bf16 = dtype == NL_BF16;
-  return cuda_status(head_dim == 64    ? tree_attn_start<64>(a, bf16, st)
-                     : head_dim == 128 ? tree_attn_start<128>(a, bf16, st)
-                                       : tree_attn_start<256>(a, bf16, st),
-                     what);
+  // sized by the rows of tree_rows_at_once; the tcgen05 form's 2 x 148 items of
+  // up to 128 rows, of more than 16, fit its 2 x 592 of at least 32
+  a.part_ml = a.part_o +
+              (size_t)2 * kTreeMaxCtas * tree_rows_at_once(a.rows, head_dim) * head_dim;
+  cudaError_t e = umma_rows         ? tree_umma_start(a, st)
+                  : head_dim == 64  ? tree_attn_start<64>(a, bf16, st)
+                  : head_dim == 128 ? tree_attn_start<128>(a, bf16, st)
+                                    : tree_attn_start<256>(a, bf16, st);
+  if (e == cudaSuccess)
+    e = head_dim == 64    ? tree_join_start<64>(a, bf16, st)
+        : head_dim == 128 ? tree_join_start<128>(a, bf16, st)
+                          : tree_join_start<256>(a, bf16, st);
+  return cuda_status(e, what);
 }

@@ -1,7 +1,7 @@
 // k_treeattn_h64.cu -- tree attention for heads of 64 values.
-#define NL_TREE_KERNELS
 #include "tree_attn.cuh"
 
 namespace nl {
 template cudaError_t tree_attn_start<64>(TreeArgs &a, bool bf16, cudaStream_t st);
+template cudaError_t tree_join_start<64>(TreeArgs &a, bool bf16, cudaStream_t st);
 }

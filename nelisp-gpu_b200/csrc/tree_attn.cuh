@@ -36,196 +36,14 @@
 // value row is contiguous.
 #pragma once
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-#include <stdint.h>
-
-#include "kv_quant.cuh"
+#define NL_TREE_KERNELS
+#include "tree_work.cuh"
 
 namespace nl {
+namespace {
 
 constexpr int kTreeWarps = 4, kTreeThreads = 32 * kTreeWarps;
 constexpr int kTreeKeys = 32;              // keys of a warp's tile
-constexpr uint32_t kTreeMaxCtas = 148 * 4;
-// What an item costs besides its tiles (its queries, the ring's first fill,
-// the join), in tiles: the shares count it, or a CTA whose share is many short
-// items would end long after the others.
-constexpr uint32_t kTreeItemCost = 4;
-
-struct TreeArgs {
-  const void *q;
-  void *o;
-  float *lse;
-  const int32_t *table, *len;
-  const uint64_t *mask;
-  float *part_o, *part_ml;       // partial states: [2 * ctas][rows_at_once][HD], [..][2]
-  uint64_t q_stride, o_stride;
-  KvPool pool;
-  uint32_t batch, nodes, heads, group, rows, row_tiles, max_blocks, ctas;
-  uint32_t rows_at_once, tile;   // rows of an item; keys of a CTA's tile
-  uint32_t block_shift;          // log2(block_size), or 32 if it is not a power of two
-  float scale;                   // scale * log2(e)
-};
-
-// The launches for one head size (k_treeattn_h*.cu): NR and WR follow from
-// the rows.
-template <int HD> cudaError_t tree_attn_start(TreeArgs &a, bool bf16, cudaStream_t st);
-// Rows of an item for ROWS rows of a key head.
-uint32_t tree_rows_at_once(uint32_t rows, uint32_t head_dim);
-
-#ifdef NL_TREE_KERNELS
-namespace {
-
-constexpr uint32_t kNone = ~0u;
-
-// ---- the list of work -----------------------------------------------------
-
-__device__ __forceinline__ uint32_t prefix_of(const TreeArgs &a, uint32_t b) {
-  return (uint32_t)max(__ldg(a.len + b), 0);
-}
-// Tokens of sequence b that the table can hold.
-__device__ __forceinline__ uint32_t keys_of(const TreeArgs &a, uint32_t b) {
-  const uint64_t n = (uint64_t)prefix_of(a, b) + a.nodes;
-  const uint64_t most = (uint64_t)a.max_blocks * a.pool.block_size;
-  return (uint32_t)(n < most ? n : most);
-}
-// Tiles of one of its items: at least one, so that every row is written.
-__device__ __forceinline__ uint32_t tiles_of(const TreeArgs &a, uint32_t b) {
-  const uint32_t n = keys_of(a, b);
-  return n ? (n + a.tile - 1) / a.tile : 1u;
-}
-
-__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-// The length of the list: an item counts its tiles and kTreeItemCost.
-__device__ __forceinline__ uint64_t all_cost(const TreeArgs &a) {
-  const uint32_t lane = threadIdx.x & 31;
-  uint64_t v = 0;
-  for (uint32_t b = lane; b < a.batch; b += 32) v += tiles_of(a, b) + kTreeItemCost;
-  return warp_sum(v) * (a.pool.kv_heads * a.row_tiles);
-}
-// The sequence that place AT of the list falls into, and the places before it.
-__device__ __forceinline__ void locate(const TreeArgs &a, uint64_t at, uint32_t *b_out,
-                                       uint64_t *before_out) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t items = (uint64_t)a.pool.kv_heads * a.row_tiles;
-  uint64_t before = 0;
-  for (uint32_t base = 0; base < a.batch; base += 32) {
-    uint64_t mine = base + lane < a.batch ? (tiles_of(a, base + lane) + kTreeItemCost) * items : 0, end = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t up = __shfl_up_sync(0xffffffffu, end, o);
-      if (lane >= (uint32_t)o) end += up;
-    }
-    end += before;
-    const uint32_t past = __ballot_sync(0xffffffffu, base + lane < a.batch && at < end);
-    if (past) {
-      const int first = __ffs(past) - 1;
-      *b_out = base + first;
-      *before_out = __shfl_sync(0xffffffffu, end - mine, first);
-      return;
-    }
-    before = __shfl_sync(0xffffffffu, end, 31);
-  }
-  *b_out = a.batch;
-  *before_out = before;
-}
-// CTA c of w takes the places [share(c), share(c + 1)).
-__device__ __forceinline__ uint64_t share(uint64_t total, uint32_t w, uint32_t c) {
-  return total / w * c + total % w * c / w;
-}
-__device__ __forceinline__ uint32_t owner(uint64_t total, uint32_t w, uint64_t at) {
-  uint32_t c = (uint32_t)((double)at * w / (double)total);
-  if (c >= w) c = w - 1;
-  while (c + 1 < w && share(total, w, c + 1) <= at) c++;
-  while (c > 0 && share(total, w, c) > at) c--;
-  return c;
-}
-
-// ---- small device helpers ---------------------------------------------------
-
-__device__ __forceinline__ uint32_t su32(const void *p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src),
-               "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void *src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src),
-               "r"(on ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() {
-  asm volatile("cp.async.commit_group;\n" ::: "memory");
-}
-template <int N> __device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ void mma16(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};\n"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
-__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
-
-// The 8 x 8 matrix of 16-bit values whose row g, columns 2t and 2t + 1, lane
-// (g, t) holds, transposed.
-__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
-  return r;
-}
-// o += codes x weights.  The tensor core cuts, not rounds, what it adds to an
-// accumulator, and over a long context that drifts; where the output is
-// float32 each 16 keys are summed apart and added in float32.
-template <int Terms, int NR>
-__device__ __forceinline__ void weigh(float (&o)[4], const uint4 &c,
-                                      const uint32_t (&p)[Terms][NR][2], int n) {
-  if (Terms == 1) {
-    mma16(o, c, p[0][n][0], p[0][n][1]);
-  } else {
-    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int e = Terms - 1; e >= 0; e--) mma16(d, c, p[e][n][0], p[e][n][1]);
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] += d[i];
-  }
-}
-
-// Two bytes u, v (0 .. 255) of W, placed as float16 1024 + u, 1024 + v by the
-// selector, less 1152: the signed codes u - 128, v - 128, exactly.
-__device__ __forceinline__ uint32_t codes8(uint32_t w, uint32_t sel) {
-  return h2(__hsub2(as_h2(__byte_perm(w, 0x64646464u, sel)), as_h2(0x64806480u)));
-}
-// The nibbles at bits 0 and 16 (4 and 20) of W, less 8, as float16.
-__device__ __forceinline__ uint32_t codes4_low(uint32_t w) {
-  return h2(__hsub2(as_h2((w & 0x000f000fu) | 0x64006400u), as_h2(0x64086408u)));
-}
-__device__ __forceinline__ uint32_t codes4_high(uint32_t w) {
-  return h2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), as_h2(0x2c002c00u),
-                    as_h2(0xd480d480u)));   // (1024 + 16 c) / 16 - 64 - 8
-}
-// Scale and offset of a parameter word.  Four-bit codes are used less 8, so
-// the offset is that of the middle of the range: with it at the low end the
-// two sums q.c and lo sum(q) would be large and of opposite signs.
-template <int BITS> __device__ __forceinline__ float scale_of(uint32_t w) {
-  return __uint_as_float(BITS == 8 ? w : w << 16);
-}
-__device__ __forceinline__ float middle_of(uint32_t w) {
-  return fmaf(8.0f, __uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
 
 // ---- geometry -----------------------------------------------------------------
 
@@ -334,7 +152,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
 
   while (at < end) {
     // ---- the next item, or part of one ----
-    const uint32_t tiles = tiles_of(a, b), cost = tiles + kTreeItemCost;
+    const uint32_t tiles = tiles_of(a, b), cost = tiles + a.item_cost;
     if (at >= before + (uint64_t)cost * items) {
       before += (uint64_t)cost * items;
       b++;
@@ -343,8 +161,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
     const uint32_t item = (uint32_t)((at - before) / cost), c0 = (uint32_t)((at - before) % cost);
     const uint32_t c1 = end - at < cost - c0 ? c0 + (uint32_t)(end - at) : cost;
     at += c1 - c0;
-    if (c1 <= kTreeItemCost) continue;             // its share ends before the first tile
-    const uint32_t t0 = c0 > kTreeItemCost ? c0 - kTreeItemCost : 0, t1 = c1 - kTreeItemCost;
+    if (c1 <= a.item_cost) continue;             // its share ends before the first tile
+    const uint32_t t0 = c0 > a.item_cost ? c0 - a.item_cost : 0, t1 = c1 - a.item_cost;
     const uint32_t head = item / a.row_tiles, row0 = item % a.row_tiles * P::Rows;
     const uint32_t prefix = prefix_of(a, b), keys = keys_of(a, b);
 
@@ -791,13 +609,13 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
   const uint32_t workers = total < a.ctas ? (uint32_t)total : a.ctas;
   uint64_t before = 0;
   {
-    for (uint32_t i = lane; i < b; i += 32) before += tiles_of(a, i) + kTreeItemCost;
+    for (uint32_t i = lane; i < b; i += 32) before += tiles_of(a, i) + a.item_cost;
     before = warp_sum(before) * ((uint64_t)a.pool.kv_heads * a.row_tiles);
   }
   const uint32_t tiles = tiles_of(a, b);
-  const uint64_t s0 = before + kTreeItemCost +
+  const uint64_t s0 = before + a.item_cost +
                       (uint64_t)(h / a.group * a.row_tiles + row / a.rows_at_once) *
-                          (tiles + kTreeItemCost);
+                          (tiles + a.item_cost);
   const uint32_t c0 = owner(total, workers, s0), c1 = owner(total, workers, s0 + tiles - 1);
   if (c0 == c1) return;
   constexpr int Per = HD / 32;
@@ -858,12 +676,11 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
   }
   a.ctas = 148u * per_sm;
   a.tile = P::Tile;
+  a.item_cost = 4 * WR;          // about 512 keys
   cudaError_t e = launch_pdl(tree_attn_kernel<T, HD, BITS, NR, WR>, dim3(a.ctas),
                              dim3(kTreeThreads), (size_t)P::Bytes, st, a);
-  if (e != cudaSuccess) return e;
-  count_launches(2);
-  return launch_pdl(tree_join_kernel<T, HD>, dim3(a.batch * a.nodes * a.heads), dim3(kTreeThreads),
-                    0, st, a);
+  count_launches(1);
+  return e;
 }
 template <typename T, int HD, int BITS>
 cudaError_t start_rows(TreeArgs &a, cudaStream_t st) {
@@ -884,6 +701,13 @@ cudaError_t tree_attn_start(TreeArgs &a, bool bf16, cudaStream_t st) {
     return bf16 ? start_rows<__nv_bfloat16, HD, 8>(a, st) : start_rows<float, HD, 8>(a, st);
   return bf16 ? start_rows<__nv_bfloat16, HD, 4>(a, st) : start_rows<float, HD, 4>(a, st);
 }
-#endif  // NL_TREE_KERNELS
+
+template <int HD>
+cudaError_t tree_join_start(TreeArgs &a, bool bf16, cudaStream_t st) {
+  const dim3 grid(a.batch * a.nodes * a.heads), block(kTreeThreads);
+  count_launches(1);
+  return bf16 ? launch_pdl(tree_join_kernel<__nv_bfloat16, HD>, grid, block, 0, st, a)
+              : launch_pdl(tree_join_kernel<float, HD>, grid, block, 0, st, a);
+}
 
 }  // namespace nl

@@ -1,0 +1,201 @@
+// tree_work.cuh -- what the kernels of the tree attention share: their
+// arguments, the list of work and how CTAs divide it, and the codes as float16.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kv_quant.cuh"
+
+namespace nl {
+
+constexpr uint32_t kTreeMaxCtas = 148 * 4;
+
+struct TreeArgs {
+  const void *q;
+  void *o;
+  float *lse;
+  const int32_t *table, *len;
+  const uint64_t *mask;
+  float *part_o, *part_ml;       // partial states: [2 * ctas][rows_at_once][HD], [..][2]
+  uint64_t q_stride, o_stride;
+  KvPool pool;
+  uint32_t batch, nodes, heads, group, rows, row_tiles, max_blocks, ctas;
+  uint32_t rows_at_once, tile;   // rows of an item; keys of a CTA's tile
+  // What an item costs besides its tiles (its queries, the first fill, the
+  // join), in tiles: the shares count it, or a CTA whose share is many short
+  // items would end long after the others.
+  uint32_t item_cost;
+  uint32_t block_shift;          // log2(block_size), or 32 if it is not a power of two
+  float scale;                   // scale * log2(e)
+};
+
+// The launches for one head size (k_treeattn_h*.cu): NR and WR follow from
+// the rows.
+template <int HD> cudaError_t tree_attn_start(TreeArgs &a, bool bf16, cudaStream_t st);
+// The joining kernel alone.
+template <int HD> cudaError_t tree_join_start(TreeArgs &a, bool bf16, cudaStream_t st);
+// The tcgen05 form (k_treeattn_umma.cu): the rows of an item it would take, or
+// 0 where it does not apply, and its launch.
+uint32_t tree_umma_rows(const TreeArgs &a, bool bf16);
+cudaError_t tree_umma_start(TreeArgs &a, cudaStream_t st);
+
+#ifdef NL_TREE_KERNELS
+namespace {
+
+constexpr uint32_t kNone = ~0u;
+
+// ---- the list of work -----------------------------------------------------
+
+__device__ __forceinline__ uint32_t prefix_of(const TreeArgs &a, uint32_t b) {
+  return (uint32_t)max(__ldg(a.len + b), 0);
+}
+// Tokens of sequence b that the table can hold.
+__device__ __forceinline__ uint32_t keys_of(const TreeArgs &a, uint32_t b) {
+  const uint64_t n = (uint64_t)prefix_of(a, b) + a.nodes;
+  const uint64_t most = (uint64_t)a.max_blocks * a.pool.block_size;
+  return (uint32_t)(n < most ? n : most);
+}
+// Tiles of one of its items: at least one, so that every row is written.
+__device__ __forceinline__ uint32_t tiles_of(const TreeArgs &a, uint32_t b) {
+  const uint32_t n = keys_of(a, b);
+  return n ? (n + a.tile - 1) / a.tile : 1u;
+}
+
+__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// The length of the list: an item counts its tiles and its own cost.
+__device__ __forceinline__ uint64_t all_cost(const TreeArgs &a) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint64_t v = 0;
+  for (uint32_t b = lane; b < a.batch; b += 32) v += tiles_of(a, b) + a.item_cost;
+  return warp_sum(v) * (a.pool.kv_heads * a.row_tiles);
+}
+// The sequence that place AT of the list falls into, and the places before it.
+__device__ __forceinline__ void locate(const TreeArgs &a, uint64_t at, uint32_t *b_out,
+                                       uint64_t *before_out) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t items = (uint64_t)a.pool.kv_heads * a.row_tiles;
+  uint64_t before = 0;
+  for (uint32_t base = 0; base < a.batch; base += 32) {
+    uint64_t mine = base + lane < a.batch ? (tiles_of(a, base + lane) + a.item_cost) * items : 0, end = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t up = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= (uint32_t)o) end += up;
+    }
+    end += before;
+    const uint32_t past = __ballot_sync(0xffffffffu, base + lane < a.batch && at < end);
+    if (past) {
+      const int first = __ffs(past) - 1;
+      *b_out = base + first;
+      *before_out = __shfl_sync(0xffffffffu, end - mine, first);
+      return;
+    }
+    before = __shfl_sync(0xffffffffu, end, 31);
+  }
+  *b_out = a.batch;
+  *before_out = before;
+}
+// CTA c of w takes the places [share(c), share(c + 1)).
+__device__ __forceinline__ uint64_t share(uint64_t total, uint32_t w, uint32_t c) {
+  return total / w * c + total % w * c / w;
+}
+__device__ __forceinline__ uint32_t owner(uint64_t total, uint32_t w, uint64_t at) {
+  uint32_t c = (uint32_t)((double)at * w / (double)total);
+  if (c >= w) c = w - 1;
+  while (c + 1 < w && share(total, w, c + 1) <= at) c++;
+  while (c > 0 && share(total, w, c) > at) c--;
+  return c;
+}
+
+// ---- small device helpers ---------------------------------------------------
+
+__device__ __forceinline__ uint32_t su32(const void *p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src),
+               "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src),
+               "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() {
+  asm volatile("cp.async.commit_group;\n" ::: "memory");
+}
+template <int N> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void mma16(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
+__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
+
+// The 8 x 8 matrix of 16-bit values whose row g, columns 2t and 2t + 1, lane
+// (g, t) holds, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
+}
+// o += codes x weights.  The tensor core cuts, not rounds, what it adds to an
+// accumulator, and over a long context that drifts; where the output is
+// float32 each 16 keys are summed apart and added in float32.
+template <int Terms, int NR>
+__device__ __forceinline__ void weigh(float (&o)[4], const uint4 &c,
+                                      const uint32_t (&p)[Terms][NR][2], int n) {
+  if (Terms == 1) {
+    mma16(o, c, p[0][n][0], p[0][n][1]);
+  } else {
+    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = Terms - 1; e >= 0; e--) mma16(d, c, p[e][n][0], p[e][n][1]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] += d[i];
+  }
+}
+
+// Two bytes u, v (0 .. 255) of W, placed as float16 1024 + u, 1024 + v by the
+// selector, less 1152: the signed codes u - 128, v - 128, exactly.
+__device__ __forceinline__ uint32_t codes8(uint32_t w, uint32_t sel) {
+  return h2(__hsub2(as_h2(__byte_perm(w, 0x64646464u, sel)), as_h2(0x64806480u)));
+}
+// The nibbles at bits 0 and 16 (4 and 20) of W, less 8, as float16.
+__device__ __forceinline__ uint32_t codes4_low(uint32_t w) {
+  return h2(__hsub2(as_h2((w & 0x000f000fu) | 0x64006400u), as_h2(0x64086408u)));
+}
+__device__ __forceinline__ uint32_t codes4_high(uint32_t w) {
+  return h2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), as_h2(0x2c002c00u),
+                    as_h2(0xd480d480u)));   // (1024 + 16 c) / 16 - 64 - 8
+}
+// Scale and offset of a parameter word.  Four-bit codes are used less 8, so
+// the offset is that of the middle of the range: with it at the low end the
+// two sums q.c and lo sum(q) would be large and of opposite signs.
+template <int BITS> __device__ __forceinline__ float scale_of(uint32_t w) {
+  return __uint_as_float(BITS == 8 ? w : w << 16);
+}
+__device__ __forceinline__ float middle_of(uint32_t w) {
+  return fmaf(8.0f, __uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+}  // namespace
+#endif  // NL_TREE_KERNELS
+
+}  // namespace nl
