@@ -8,29 +8,28 @@
 // with float32 accumulators in TMEM.  A score arrives with its key's thread:
 // the key's scale is a register, and no row maximum is taken at all in the
 // usual tile -- weights are formed against each row's reference, the maximum
-// of the keys up to the last time one exceeded it by 2^8 (a vote over the CTA
-// per tile), and float16 has the room: scales are brought below 2^7.
+// of the keys up to the last time one exceeded it by 2^8 (a vote of the 128
+// threads per tile), and float16 has the room: scales are brought below 2^7.
 //
-// 16 warps, one CTA per SM, tiles of 128 keys:
-//   warps 0-7   two groups, half the rows each, a thread per key: scores from
-//               TMEM, weights to shared memory (the N x 128 operand with N
-//               contiguous), sums of the weights in registers; at the end of
-//               an item the output from TMEM, a thread per value;
-//   warps 8-11  codes to float16, a thread per key: keys to a TMEM stage,
-//               values to a shared-memory stage ([key][value], read as V^T);
-//   warp 12     TMA of the code tiles, one box per run of a page;
-//   warp 13     allocates TMEM and issues the MMAs of both products;
-//               warps 14 and 15 have nothing to do.
-// The 128 registers a thread of the launch are shared out anew: 168 for the
-// score warps, which hold the sums of their rows, 104 for warps 8-11, 72 for
-// warps 12-15 (2 x 168 + 104 + 72 = 4 x 128).
+// 20 warps, one CTA per SM, tiles of 128 keys:
+//   warps 0-7   two groups that take the tiles in turn, a thread per key:
+//               scores from TMEM, weights to shared memory (the N x 128 operand
+//               with N contiguous), sums of the weights in registers.  Each
+//               group has its own references, sums and output accumulator, so
+//               they wait for each other only at the end of an item, where the
+//               two outputs are read, a thread per value, and joined;
+//   warps 8-11  key codes to float16 in a TMEM stage, a thread per key;
+//   warps 12-15 value codes to float16 in a shared-memory stage ([key][value],
+//               read as V^T), a thread per key;
+//   warp 16     TMA of the code tiles, one box per run of a page;
+//   warp 17     allocates TMEM and issues the MMAs of the scores;
+//   warps 18,19 issue those of the output, a group's each: one thread would
+//               need longer to issue all of a tile's than they run.
+// The 96 registers a thread of the launch are shared out anew: 152 for the
+// score warps, which hold the sums of their rows, 56, 72 and 48 for the others
+// (2 x 152 + 56 + 72 + 48 = 5 x 96).
 // The stages run on over the end of an item: the next item's codes are on
 // their way and converted while the last one's output is written.
-//
-// Per tile of 128 keys and heads of 128, shared memory moves about 1400 (N =
-// 64, 8 bits) cycles' worth at 128 bytes each, DRAM 1445 at the SM's share of
-// the copy rate, so the two are in balance there; with 4 bits or 128 rows the
-// shared memory and the score arithmetic bound it.
 //
 // Every wait is bounded.  One that gives up sets the library's wait flag, and
 // its thread then waits no more but runs on to the end: no barrier of the CTA
@@ -44,7 +43,7 @@
 namespace nl {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr int kSoft = 256;                 // threads of the score warps
 constexpr int kTileKeys = 128;
 constexpr uint32_t kWaitRounds = 4096, kSuspendNs = 1000000;
@@ -54,26 +53,27 @@ template <int HD, int BITS, int N> struct Plan {
   static constexpr int RB = HD * BITS / 8;
   static constexpr int Chunks = RB / 16;
   static constexpr int Codes = kTileKeys * RB;               // one side's codes of a tile
-  static constexpr int Stages = 2 * Codes * 3 <= 48 * 1024 ? 3 : N == 64 ? 3 : 2;
+  static constexpr int Stages = 3;
   static constexpr int VTile = HD * kTileKeys * 2;            // values as float16
-  static constexpr int PBufs = N == 64 ? 2 : 1;
-  static constexpr int PTile = N * kTileKeys * 2;
+  static constexpr int PTile = 128 * kTileKeys;               // weights, rows of 128 bytes
   static constexpr int QTile = N * HD * 2;
   // offsets from a 1024-byte boundary
-  static constexpr int V = Stages * 2 * Codes, P = V + 2 * VTile, Q = P + PBufs * PTile;
-  static constexpr int Ref = Q + QTile;                       // float2 per row
-  static constexpr int Sum = Ref + N * 8;                     // floats
-  static constexpr int Keep = Sum + N * 4;
-  static constexpr int Masks = Keep + N * 4;
+  static constexpr int V = Stages * 2 * Codes, P = V + 2 * VTile, Q = P + 2 * PTile;
+  static constexpr int Factor = Q + QTile;                    // floats
+  static constexpr int Sum = Factor + N * 4;
+  static constexpr int Ref = Sum + N * 4;                     // [2][N]
+  static constexpr int Keep = Ref + 2 * N * 4;                // [2][N]
+  static constexpr int Masks = Keep + 2 * N * 4;
   static constexpr int Offs = Masks + N * 8;                  // output offsets
-  static constexpr int Warp = Offs + N * 8;                   // [4][N] floats
-  static constexpr int Bars = Warp + 4 * N * 4;
+  static constexpr int Warp = Offs + N * 8;                   // [8][N]
+  static constexpr int Base = Warp + 8 * N * 4;               // [8][N] (4 bits)
+  static constexpr int Bars = Base + (BITS == 4 ? 8 * N * 4 : 0);
   static constexpr int Used = Bars + 256 + 1024;
   static constexpr int Bytes = Used > 120 * 1024 ? Used : 120 * 1024;   // one CTA per SM (TMEM)
-  // TMEM columns
+  // TMEM columns: two stages of keys and of scores, two outputs
   static constexpr uint32_t KCols = HD / 2;
   static constexpr uint32_t TK = 0, TS = 2 * KCols, TO = TS + 2 * N;
-  static_assert(TO + N <= 512 && Used <= 227 * 1024, "tile");
+  static_assert(TO + 2 * N <= 512 && Used <= 227 * 1024, "tile");
 };
 
 __device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) {
@@ -120,14 +120,29 @@ __device__ __forceinline__ void fence_async() {
 __device__ __forceinline__ void soft_sync() {
   asm volatile("bar.sync 1, %0;\n" ::"n"(kSoft) : "memory");
 }
-// Whether any of the score warps' threads says so.
-__device__ __forceinline__ bool soft_any(bool v) {
+// The same for the 128 threads of one group, and whether any of them says so.
+__device__ __forceinline__ void group_sync(uint32_t group) {
+  asm volatile("bar.sync %0, 128;\n" ::"r"(2 + group) : "memory");
+}
+__device__ __forceinline__ bool group_any(uint32_t group, bool v) {
   uint32_t r;
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, %2, p;\n"
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 128, p;\n"
       " selp.u32 %0, 1, 0, q;\n}\n"
-      : "=r"(r) : "r"((uint32_t)v), "n"(kSoft) : "memory");
+      : "=r"(r) : "r"((uint32_t)v), "r"(2 + group) : "memory");
   return r != 0;
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
   asm volatile(
@@ -151,6 +166,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) 
       "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
       "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
       "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+      "%13,%14,%15,%16};\n" ::"r"(at),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
@@ -208,6 +232,48 @@ __device__ __forceinline__ void expand(uint32_t w, uint32_t *to) {
   }
 }
 
+// Two floats at a time.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(Pair v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// The largest over a warp's lanes of each of 32 values: lane i gets that of v[i].
+__device__ __forceinline__ float tops32(float (&v)[32]) {
+  const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool high = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; i++) {
+      const float give = high ? v[i] : v[i + o], keep = high ? v[i + o] : v[i];
+      v[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o));
+    }
+  }
+  return v[0];
+}
 // The sum over a warp's lanes of each of 32 values: lane i gets that of v[i].
 __device__ __forceinline__ float sums32(float (&v)[32]) {
   const uint32_t lane = threadIdx.x & 31;
@@ -266,42 +332,44 @@ __global__ void __launch_bounds__(kThreads, 1)
 tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, uint32_t box, int *err) {
   using L = Plan<HD, BITS, N>;
-  constexpr int Half = N / 2;                // rows of a group of score warps
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                             ~(uintptr_t)1023);
   const uint32_t s0 = su32(sm);
-  float2 *ref = reinterpret_cast<float2 *>(sm + L::Ref);      // a row's factor, -reference
+  float *factor = reinterpret_cast<float *>(sm + L::Factor);  // of a row's scores
   float *qsum = reinterpret_cast<float *>(sm + L::Sum);       // the sum of its query
-  float *keep = reinterpret_cast<float *>(sm + L::Keep);      // what a new reference leaves of sums
+  float *refs = reinterpret_cast<float *>(sm + L::Ref);       // less a group's reference
+  float *keeps = reinterpret_cast<float *>(sm + L::Keep);     // what a new one leaves of the sums
   uint64_t *masks = reinterpret_cast<uint64_t *>(sm + L::Masks);
   uint64_t *offs = reinterpret_cast<uint64_t *>(sm + L::Offs);
   float *warp_part = reinterpret_cast<float *>(sm + L::Warp);
+  float *warp_base = reinterpret_cast<float *>(sm + L::Base);
   const uint32_t bars = s0 + L::Bars;
   const uint32_t full = bars, empty = bars + 24, kready = bars + 48, qkdone = bars + 64,
                  sfree = bars + 80, vready = bars + 96, pready = bars + 112, pvdone = bars + 128,
                  qready = bars + 144;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + L::Bars + 160);
-  uint32_t *vote = tmem_slot + 1;            // the largest scale of a tile
+  uint32_t *votes = tmem_slot + 1;           // the largest scale of a group's tile
+  float *backs = reinterpret_cast<float *>(tmem_slot + 3);   // a group's 1 / vs
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::Stages; i++) {
       bar_init(full + 8 * i, 1);
-      bar_init(empty + 8 * i, 4);
+      bar_init(empty + 8 * i, 8);
     }
     for (int i = 0; i < 2; i++) {
       bar_init(kready + 8 * i, 4);
       bar_init(qkdone + 8 * i, 1);
-      bar_init(sfree + 8 * i, 8);
+      bar_init(sfree + 8 * i, 4);
       bar_init(vready + 8 * i, 4);
-      bar_init(pready + 8 * i, 8);
+      bar_init(pready + 8 * i, 4);
       bar_init(pvdone + 8 * i, 1);
     }
     bar_init(qready, 8);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 13) {
+  if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
                      su32(tmem_slot)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
@@ -317,9 +385,9 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
   Walk w;
   if (w.begin(a)) {
     uint32_t it = 0;                         // tiles so far, over all items
-    if (warp >= 12) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
-      if (warp == 12) {
+    if (warp >= 16) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
+      if (warp == 16) {
         // ---- TMA of the codes: a run of BOX keys of a page at a time, one lane each ----
         const uint32_t runs = kTileKeys / box;
         while (w.next(a)) {
@@ -350,150 +418,168 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         alive = true;
         for (uint32_t i = it > (uint32_t)L::Stages ? it - L::Stages : 0; i < it; i++)
           bar_wait(full + 8 * (i % L::Stages), i / L::Stages & 1, alive, err);
-      } else if (warp == 13) {
-        // ---- the MMAs: scores of tile i, then the output of tile i - 1 ----
+      } else if (warp == 17) {
+        // ---- the score products ----
         uint32_t item = 0;
-        bool owed = false, first = true;       // a second product not issued yet; its item's first
-        auto second = [&](uint32_t i, bool fresh) {
-          const uint32_t st = i & 1;
-          bar_wait(vready + 8 * st, i >> 1 & 1, alive, err);
-          bar_wait(pready + 8 * st, i >> 1 & 1, alive, err);
-          fence_after();
-          const uint32_t v0 = s0 + L::V + st * L::VTile;
-          const uint32_t p0 = s0 + L::P + (L::PBufs == 2 ? st * L::PTile : 0);
-  #pragma unroll
-          for (int k = 0; k < kTileKeys / 16; k++)
-            mma_ss(tmem + L::TO, smem_desc(v0 + 2048 * k, HD == 128 ? kTileKeys * 128 : 0),
-                   smem_desc(p0 + 2048 * k, kTileKeys * 128), instr_desc<N, true>(),
-                   fresh && k == 0 ? 0u : 1u);
-          mma_commit(pvdone + 8 * st);
-        };
         while (w.next(a)) {
-          if (owed && lane == 0) second(it - 1, first);
-          owed = false;
-          first = true;
-          if (lane == 0) bar_wait(qready, item & 1, alive, err);
-          item++;
-          for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
-            if (lane == 0) {
-              const uint32_t st = it & 1;
-              bar_wait(kready + 8 * st, it >> 1 & 1, alive, err);
-              bar_wait(sfree + 8 * st, (it >> 1 & 1) ^ 1, alive, err);
+          if (lane == 0) {
+            bar_wait(qready, item & 1, alive, err);
+            for (uint32_t i = it; i < it + (w.t1 - w.t0); i++) {
+              const uint32_t st = i & 1, ph = i >> 1 & 1;
+              bar_wait(kready + 8 * st, ph, alive, err);
+              bar_wait(sfree + 8 * st, ph ^ 1, alive, err);
               fence_after();
-  #pragma unroll
+              const uint64_t q = smem_desc(s0 + L::Q, 16);
+#pragma unroll
               for (int k = 0; k < HD / 16; k++)
                 mma_ts(tmem + L::TS + st * N, tmem + L::TK + st * L::KCols + 8 * k,
-                       smem_desc(s0 + L::Q + k / 4 * (N * 128) + k % 4 * 32, 16),
-                       instr_desc<N, false>(), k ? 1u : 0u);
+                       q + (k / 4 * (N * 128) + k % 4 * 32) / 16, instr_desc<N, false>(),
+                       k ? 1u : 0u);
               mma_commit(qkdone + 8 * st);
-              if (owed) {
-                second(it - 1, first);
-                first = false;
-              }
             }
-            owed = true;
           }
           __syncwarp();
+          it += w.t1 - w.t0;
+          item++;
         }
-        if (owed && lane == 0) second(it - 1, first);
-        __syncwarp();
+      } else {
+        // ---- the output products, each group's into its own accumulator ----
+        const uint32_t st = warp - 18;
+        while (w.next(a)) {
+          if (lane == 0) {
+            const uint32_t i0 = it + ((it ^ st) & 1);
+            for (uint32_t i = i0; i < it + (w.t1 - w.t0); i += 2) {
+              const uint32_t ph = i >> 1 & 1;
+              bar_wait(vready + 8 * st, ph, alive, err);
+              bar_wait(pready + 8 * st, ph, alive, err);
+              fence_after();
+              // 16 keys on is 2048 bytes on: 128 in a descriptor's address field
+              const uint64_t v = smem_desc(s0 + L::V + st * L::VTile,
+                                           HD == 128 ? kTileKeys * 128 : 0);
+              const uint64_t p = smem_desc(s0 + L::P + st * L::PTile, 16);
+#pragma unroll
+              for (int k = 0; k < kTileKeys / 16; k++)
+                mma_ss(tmem + L::TO + st * N, v + 128 * k, p + 128 * k, instr_desc<N, true>(),
+                       k == 0 && i == i0 ? 0u : 1u);
+              mma_commit(pvdone + 8 * st);
+            }
+          }
+          __syncwarp();
+          it += w.t1 - w.t0;
+        }
       }
     } else if (warp >= 8) {
-      // ---- codes to float16, a thread per key ----
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
-      const uint32_t tid = threadIdx.x - kSoft;
-      const uint32_t quad = (warp & 3) * 32, key = quad + lane;    // its TMEM lane
-      while (w.next(a)) {
-        for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
-          const uint32_t st = it % L::Stages, h = it & 1;
-          const uint8_t *kc = sm + st * (2 * L::Codes), *vc = kc + L::Codes;
-          bar_wait(full + 8 * st, it / L::Stages & 1, alive, err);
-          bar_wait(qkdone + 8 * h, (it >> 1 & 1) ^ 1, alive, err);
-          fence_after();
-          // byte of chunk c of a key's row, swizzled by the copy over the row's bytes
-          auto chunk = [](uint32_t k, uint32_t c) {
-            const uint32_t x = L::RB == 128 ? k & 7 : L::RB == 64 ? k >> 1 & 3 : k >> 2 & 1;
-            return k * L::RB + ((c ^ x) << 4);
-          };
-          constexpr int Each = BITS == 8 ? 4 : 2;       // chunks that make 32 TMEM columns
+      // byte of chunk c of a key's row, swizzled by the copy over the row's bytes
+      const uint32_t quad = (warp & 3) * 32, key = quad + lane;
+      const uint32_t x = L::RB == 128 ? key & 7 : L::RB == 64 ? key >> 1 & 3 : key >> 2 & 1;
+      const uint32_t from = key * L::RB + (x << 4);
+      if (warp < 12) {
+        // ---- keys, to TMEM.  (Codes left 1024 too large, with that much of the
+        // query's sum taken off the scores, would halve the work here, but the
+        // cut sums of the tensor core then cost the scores 5 bits.) ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
+        while (w.next(a)) {
+          for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
+            const uint32_t st = it % L::Stages, h = it & 1;
+            const uint8_t *kc = sm + st * (2 * L::Codes);
+            bar_wait(full + 8 * st, it / L::Stages & 1, alive, err);
+            bar_wait(qkdone + 8 * h, (it >> 1 & 1) ^ 1, alive, err);
+            fence_after();
+            constexpr int Each = BITS == 8 ? 2 : 1;       // chunks that make 16 TMEM columns
+            constexpr int W = BITS == 8 ? 2 : 4;          // columns a word makes
 #pragma unroll
-          for (int c0 = 0; c0 < L::Chunks; c0 += Each) {
-            uint32_t v[32];
+            for (int c0 = 0; c0 < L::Chunks; c0 += Each) {
+              uint32_t v[16];
 #pragma unroll
-            for (int c = 0; c < Each; c++) {
-              const uint4 x = *reinterpret_cast<const uint4 *>(kc + chunk(key, c0 + c));
-              constexpr int W = BITS == 8 ? 2 : 4;
-              uint32_t *to = v + c * 4 * W;
-              expand<BITS>(x.x, to); expand<BITS>(x.y, to + W);
-              expand<BITS>(x.z, to + 2 * W); expand<BITS>(x.w, to + 3 * W);
+              for (int c = 0; c < Each; c++) {
+                const uint4 y = *reinterpret_cast<const uint4 *>(kc + (from ^ ((c0 + c) << 4)));
+                uint32_t *to = v + c * 4 * W;
+                expand<BITS>(y.x, to); expand<BITS>(y.y, to + W);
+                expand<BITS>(y.z, to + 2 * W); expand<BITS>(y.w, to + 3 * W);
+              }
+              tmem_st16(tmem + (quad << 16) + L::TK + h * L::KCols + c0 / Each * 16, v);
             }
-            tmem_st32(tmem + (quad << 16) + L::TK + h * L::KCols + c0 / Each * 32, v);
-          }
-          tmem_wait_st();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(kready + 8 * h);
-          // values: 16-byte chunks in turn, so that neither the reads nor the
-          // writes of eight lanes share a bank
-          bar_wait(pvdone + 8 * h, (it >> 1 & 1) ^ 1, alive, err);
-          uint8_t *vt = sm + L::V + h * L::VTile;
-#pragma unroll
-          for (int i = 0; i < L::Chunks; i++) {
-            const uint32_t n = i * 128 + tid, k = n / L::Chunks, c = n % L::Chunks;
-            const uint4 x = *reinterpret_cast<const uint4 *>(vc + chunk(k, c));
-            constexpr int Out = BITS == 8 ? 2 : 4;      // chunks of float16 it makes
-            uint32_t v[4 * Out];
-            if (BITS == 8) {
-              expand<8>(x.x, v); expand<8>(x.y, v + 2); expand<8>(x.z, v + 4); expand<8>(x.w, v + 6);
-            } else {
-              expand<4>(x.x, v); expand<4>(x.y, v + 4);
-              expand<4>(x.z, v + 8 % (4 * Out)); expand<4>(x.w, v + 12 % (4 * Out));
-            }
-            const uint32_t block = c * Out / 8, oc = c * Out % 8;
-            uint8_t *row = vt + block * (kTileKeys * 128) + k * 128;
-            const uint32_t turn = BITS == 8 ? block : block ^ ((k & 1) << 1);
-#pragma unroll
-            for (int s = 0; s < Out; s++) {
-              uint4 y = make_uint4(v[4 * s], v[4 * s + 1], v[4 * s + 2], v[4 * s + 3]);
-#pragma unroll
-              for (int u = 0; u < Out; u++)
-                if ((s ^ turn) == (uint32_t)u)
-                  y = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-              *reinterpret_cast<uint4 *>(row + (((oc + (s ^ turn)) ^ (k & 7)) << 4)) = y;
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              bar_arrive(kready + 8 * h);
+              bar_arrive(empty + 8 * st);
             }
           }
-          fence_async();
-          __syncwarp();
-          if (lane == 0) {
-            bar_arrive(vready + 8 * h);
-            bar_arrive(empty + 8 * st);
+        }
+      } else {
+        // ---- values: the signed codes, to shared memory; eight lanes' rows are
+        // swizzled apart, so neither reads nor writes share a bank ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        const uint32_t row = key * 128 + ((key & 7) << 4);
+        while (w.next(a)) {
+          for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
+            const uint32_t st = it % L::Stages, h = it & 1;
+            const uint8_t *vc = sm + st * (2 * L::Codes) + L::Codes;
+            uint8_t *vt = sm + L::V + h * L::VTile;
+            bar_wait(full + 8 * st, it / L::Stages & 1, alive, err);
+            bar_wait(pvdone + 8 * h, (it >> 1 & 1) ^ 1, alive, err);
+#pragma unroll 2
+            for (int c = 0; c < L::Chunks; c++) {
+              const uint4 y = *reinterpret_cast<const uint4 *>(vc + (from ^ (c << 4)));
+              constexpr int Out = BITS == 8 ? 2 : 4;      // chunks of float16 it makes
+              const uint32_t in[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+              for (int s = 0; s < Out; s++) {
+                uint32_t v[4];
+                if (BITS == 8) {
+                  expand<8>(in[2 * s % 4], v);
+                  expand<8>(in[(2 * s + 1) % 4], v + 2);
+                } else {
+                  expand<4>(in[s], v);
+                }
+                const int oc = c * Out + s;
+                *reinterpret_cast<uint4 *>(vt + oc / 8 * (kTileKeys * 128) +
+                                           (row ^ ((oc & 7) << 4))) =
+                    make_uint4(v[0], v[1], v[2], v[3]);
+              }
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+              bar_arrive(vready + 8 * h);
+              bar_arrive(empty + 8 * st);
+            }
           }
         }
       }
     } else {
       // ---- scores to weights, a thread per key; half the rows a group ----
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 152;\n");
       const uint32_t group = warp >> 2, quad = (warp & 3) * 32, mykey = quad + lane;
-      const uint32_t tid = threadIdx.x, n0 = group * Half;
+      const uint32_t tid = threadIdx.x;
+      float *ref = refs + group * N, *keep = keeps + group * N;
+      uint32_t *vote = votes + group;
       const uint64_t used = a.nodes < 64 ? (1ull << a.nodes) - 1 : ~0ull;
       while (w.next(a)) {
         const uint32_t prefix = prefix_of(a, w.b), keys = keys_of(a, w.b);
+        const uint32_t mine0 = w.t0 + ((it ^ group) & 1);        // this group's first tile
         // the parameter words of this thread's key of a tile, found a tile ahead
+        auto page_of = [&](uint32_t key) {
+          return a.block_shift < 32 ? key >> a.block_shift : key / a.pool.block_size;
+        };
         auto block_of = [&](uint32_t tile) {
           const uint32_t key = tile * kTileKeys + mykey;
           if (tile >= w.t1 || key >= keys) return kNone;
-          return (uint32_t)__ldg(a.table + (uint64_t)w.b * a.max_blocks + key / a.pool.block_size);
+          return (uint32_t)__ldg(a.table + (uint64_t)w.b * a.max_blocks + page_of(key));
         };
         auto words_of = [&](uint32_t tile, uint32_t block, uint32_t *kw, uint32_t *vw) {
           *kw = *vw = 0;
           if (block >= a.pool.num_blocks) return false;
+          const uint32_t key = tile * kTileKeys + mykey;
           const uint32_t row =
-              kv_row(a.pool, block, (tile * kTileKeys + mykey) % a.pool.block_size, w.head);
+              kv_row(a.pool, block, key - page_of(key) * a.pool.block_size, w.head);
           *kw = __ldg(a.pool.param[0] + row);
           *vw = __ldg(a.pool.param[1] + row);
           return true;
         };
-        uint32_t block1 = block_of(w.t0), kw1, vw1;
+        uint32_t block1 = block_of(mine0), kw1, vw1;
 
         // the queries of the item, float16, K-major
         {
@@ -541,8 +627,9 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           for (int o = Lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
           if (part == 0) {
             // a factor is never zero: it would make NaN of a masked score
-            ref[n] = make_float2(fmaxf(a.scale * __uint_as_float((uint32_t)(127 - up) << 23),
-                                       1.17549435e-38f), kFar);
+            factor[n] = fmaxf(a.scale * __uint_as_float((uint32_t)(127 - up) << 23),
+                              1.17549435e-38f);
+            refs[n] = refs[N + n] = kFar;
             qsum[n] = sum;
             masks[n] = live ? a.mask[out_row] & used : 0;
             offs[n] = live ? out_row * a.o_stride + (uint64_t)col * HD : ~0ull;
@@ -552,174 +639,165 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         soft_sync();
         if (lane == 0) bar_arrive(qready);
 
-        float l[Half], base[BITS == 4 ? Half : 1];
+        constexpr int NB = BITS == 4 ? N / 2 : 1;
+        Pair l[N / 2], base[NB];
 #pragma unroll
-        for (int i = 0; i < Half; i++) l[i] = 0.0f;
-        if (BITS == 4) {
-#pragma unroll
-          for (int i = 0; i < Half; i++) base[i] = 0.0f;
-        }
+        for (int i = 0; i < N / 2; i++) l[i] = base[i % NB] = 0;
         float vs = 1.0f;
         uint32_t vlimit = 0;
-        bool have1 = words_of(w.t0, block1, &kw1, &vw1);
-        block1 = block_of(w.t0 + 1);
+        bool have1 = words_of(mine0, block1, &kw1, &vw1);
+        block1 = block_of(mine0 + 2);
 
-        for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
-          const uint32_t st = it & 1;
+        for (uint32_t tile = mine0; tile < w.t1; tile += 2) {
+          const uint32_t i0 = it + (tile - w.t0), st = group, ph = i0 >> 1 & 1;
           const bool have = have1;
           const uint32_t kw = kw1, vw = vw1;
-          have1 = words_of(tile + 1, block1, &kw1, &vw1);
-          block1 = block_of(tile + 2);
-          const float sk = scale_of<BITS>(kw), mk = middle_of(kw);
-          const float sv = scale_of<BITS>(vw), mv = middle_of(vw);
+          have1 = words_of(tile + 2, block1, &kw1, &vw1);
+          block1 = block_of(tile + 4);
+          const float sk = scale_of<BITS>(kw);
+          const float mk = middle_of(kw);
+          const Pair sk2 = pair(sk, sk), mk2 = pair(mk, mk);
+          const float sv = scale_of<BITS>(vw);
+          // (a value that is NaN reaches the output by its weight alone)
+          const float mv = BITS == 4 && sv == sv ? middle_of(vw) : 0.0f;
           const uint32_t vbits = __float_as_uint(sv) < 0x7f800000u ? __float_as_uint(sv) : 0u;
           const uint32_t key = tile * kTileKeys + mykey;
           // tiles of prefix keys that all exist need no masks
           const bool whole = __all_sync(0xffffffffu, have && key < prefix);
-          // whether row n sees this key
-          auto seen = [&](uint32_t n) {
-            return have && (key < prefix ? masks[n] != 0
-                                         : key - prefix < 64 && (masks[n] >> (key - prefix) & 1));
-          };
-          // the scores of 32 rows from n: over the rows' references, in powers of two
-          auto score = [&](uint32_t (&s)[32], uint32_t n) {
+          // the scores of 32 rows from n on this key, in powers of two: over the
+          // rows' references (less 0) or as they are
+          auto score = [&](uint32_t (&s)[32], uint32_t n, bool over_ref) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              if (BITS == 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(qsum + n + i);
-                q[0] = x.x; q[1] = x.y; q[2] = x.z; q[3] = x.w;
-              }
+              float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (BITS == 4) q = *reinterpret_cast<const float4 *>(qsum + n + i);
+              const float4 f = *reinterpret_cast<const float4 *>(factor + n + i);
+              float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (over_ref) r = *reinterpret_cast<const float4 *>(ref + n + i);
 #pragma unroll
               for (int j = 0; j < 4; j += 2) {
-                const float4 r = *reinterpret_cast<const float4 *>(ref + n + i + j);
-                float x = __uint_as_float(s[i + j]) * sk, y = __uint_as_float(s[i + j + 1]) * sk;
-                if (BITS == 4) x = fmaf(mk, q[j], x), y = fmaf(mk, q[j + 1], y);
-                s[i + j] = __float_as_uint(fmaf(x, r.x, r.y));
-                s[i + j + 1] = __float_as_uint(fmaf(y, r.z, r.w));
+                Pair x = pair(__uint_as_float(s[i + j]), __uint_as_float(s[i + j + 1]));
+                x = mul2(x, sk2);
+                if (BITS == 4) x = fma2(mk2, j ? pair(q.z, q.w) : pair(q.x, q.y), x);
+                x = fma2(x, j ? pair(f.z, f.w) : pair(f.x, f.y), j ? pair(r.z, r.w) : pair(r.x, r.y));
+                const float2 y = unpair(x);
+                s[i + j] = __float_as_uint(y.x);
+                s[i + j + 1] = __float_as_uint(y.y);
               }
             }
             if (!whole) {
 #pragma unroll
-              for (int i = 0; i < 32; i++)
-                if (!seen(n + i)) s[i] = 0xff800000u;        // -inf
-            }
-          };
-          bar_wait(qkdone + 8 * st, it >> 1 & 1, alive, err);
-          fence_after();
-          const uint32_t ts = tmem + (quad << 16) + L::TS + st * N + n0;
-          uint32_t s[32];
-          bool over = vbits >= vlimit && vbits != 0;
-#pragma unroll
-          for (int c = 0; c < Half / 32; c++) {
-            tmem_ld32(ts + 32 * c, s);
-            score(s, n0 + 32 * c);
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 32; i++) top = fmaxf(top, __uint_as_float(s[i]));
-            over |= top > 8.0f;
-          }
-          if (soft_any(over)) {
-            // ---- new references: the maxima of the keys so far ----
-#pragma unroll
-            for (int c = 0; c < Half / 32; c++) {
-              tmem_ld32(ts + 32 * c, s);
-#pragma unroll
               for (int i = 0; i < 32; i++) {
-                const uint32_t n = n0 + 32 * c + i;
-                float x = __uint_as_float(s[i]) * sk;
-                if (BITS == 4) x = fmaf(mk, qsum[n], x);
-                x *= ref[n].x;
-                if (!whole && !seen(n)) x = -INFINITY;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1)
-                  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                if (lane == 0) warp_part[(warp & 3) * N + n] = x;
+                const uint64_t m = masks[n + i];
+                const bool seen = have && (key < prefix ? m != 0
+                                                        : key - prefix < 64 && (m >> (key - prefix) & 1));
+                if (!seen) s[i] = 0xff800000u;             // -inf
               }
             }
-            if (tid == 0) *vote = 0;
-            soft_sync();
+          };
+          bar_wait(qkdone + 8 * st, ph, alive, err);
+          fence_after();
+          const uint32_t ts = tmem + (quad << 16) + L::TS + st * N;
+          uint32_t s[32];
+          for (bool again = false;; again = true) {
+            bool over = vbits >= vlimit && vbits != 0;
+            // the last 32 rows stay in registers for their weights
+#pragma unroll
+            for (int c = 0; c < N / 32; c++) {
+              tmem_ld32(ts + 32 * c, s);
+              score(s, 32 * c, true);
+              float top = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 32; i++) top = fmaxf(top, __uint_as_float(s[i]));
+              over |= top > 8.0f;
+            }
+            if (again || !group_any(group, over)) break;
+            // ---- new references: the maxima of the keys so far ----
+#pragma unroll 1
+            for (int c = 0; c < N / 32; c++) {
+              tmem_ld32(ts + 32 * c, s);
+              score(s, 32 * c, false);
+              float x[32];
+#pragma unroll
+              for (int i = 0; i < 32; i++) x[i] = __uint_as_float(s[i]);
+              warp_part[warp * N + 32 * c + lane] = tops32(x);
+            }
+            if ((warp & 3) == 0 && lane == 0) *vote = 0;
+            group_sync(group);
             const uint32_t top_bits = __reduce_max_sync(0xffffffffu, vbits);
-            if (group == 0 && lane == 0) atomicMax(vote, top_bits);
-            soft_sync();
+            if (lane == 0) atomicMax(vote, top_bits);
+            if (mykey < N) {
+              const float *p = warp_part + group * 4 * N + mykey;
+              const float top = fmaxf(fmaxf(p[0], p[N]), fmaxf(p[2 * N], p[3 * N]));
+              const float old = -ref[mykey];                 // -kFar: no key met yet
+              keep[mykey] = top > old ? ex2(old - top) : 1.0f;
+              if (top > old) ref[mykey] = -top;
+            }
+            group_sync(group);
             float ratio = 1.0f;
             const uint32_t big = *vote;
             if (big >= vlimit && big != 0) {
-              const uint32_t e = (big >> 23) + 1;           // scales below 2^(e - 127)
+              const uint32_t e = (big >> 23) + 1;            // scales below 2^(e - 127)
               vlimit = e << 23;
               const float next_vs = __uint_as_float((261u - e) << 23);   // to below 2^7
               ratio = next_vs / vs;
               vs = next_vs;
             }
-            if (tid < N) {
-              const float top = fmaxf(fmaxf(warp_part[tid], warp_part[N + tid]),
-                                      fmaxf(warp_part[2 * N + tid], warp_part[3 * N + tid]));
-              const float old = -ref[tid].y;                 // -kFar: no key met yet
-              keep[tid] = top > old ? ex2(old - top) : 1.0f;
-              if (top > old) ref[tid].y = -top;
-            }
-            soft_sync();
             // the sums, and the output so far once its last product is done
 #pragma unroll
-            for (int i = 0; i < Half; i++) {
-              const float k = keep[n0 + i];
-              l[i] *= k;
-              if (BITS == 4) base[i % (BITS == 4 ? Half : 1)] *= k;
+            for (int i = 0; i < N / 2; i++) {
+              const float2 k = *reinterpret_cast<const float2 *>(keep + 2 * i);
+              l[i] = mul2(l[i], pair(k.x, k.y));
+              if (BITS == 4) base[i % NB] = mul2(base[i % NB], pair(k.x, k.y));
             }
-            if (tile > w.t0) {
-              bar_wait(pvdone + 8 * ((it - 1) & 1), (it - 1) >> 1 & 1, alive, err);
+            if (tile > mine0) {
+              bar_wait(pvdone + 8 * st, ph ^ 1, alive, err);
               fence_after();
-              const uint32_t to = tmem + (quad << 16) + L::TO + n0;
-#pragma unroll
-              for (int c = 0; c < Half / 32; c++) {
-                uint32_t o[32];
-                tmem_ld32(to + 32 * c, o);
+              const uint32_t to = tmem + (quad << 16) + L::TO + st * N;
+#pragma unroll 1
+              for (int c = 0; c < N / 32; c++) {
+                tmem_ld32(to + 32 * c, s);
 #pragma unroll
                 for (int i = 0; i < 32; i++)
-                  o[i] = __float_as_uint(__uint_as_float(o[i]) * (keep[n0 + 32 * c + i] * ratio));
-                tmem_st32(to + 32 * c, o);
+                  s[i] = __float_as_uint(__uint_as_float(s[i]) * (keep[32 * c + i] * ratio));
+                tmem_st32(to + 32 * c, s);
               }
               tmem_wait_st();
-            }
-            if (Half == 32) {
-              tmem_ld32(ts, s);
-              score(s, n0);
             }
           }
           // ---- the weights ----
           const float wv = sv * vs;
-          if (L::PBufs == 2) bar_wait(pvdone + 8 * st, (it >> 1 & 1) ^ 1, alive, err);
-          else if (it) bar_wait(pvdone + 8 * ((it - 1) & 1), (it - 1) >> 1 & 1, alive, err);
-          uint8_t *pt = sm + L::P + (L::PBufs == 2 ? st * L::PTile : 0) + mykey * 128;
+          const bool odd = !(fabsf(wv) < INFINITY);
+          const Pair wv2 = pair(wv, wv), mv2 = pair(mv, mv);
+          bar_wait(pvdone + 8 * st, ph ^ 1, alive, err);       // the buffer's last reader
+          uint8_t *pt = sm + L::P + st * L::PTile + mykey * 128;
 #pragma unroll
-          for (int c = 0; c < Half / 32; c++) {
-            if (Half > 32) {
+          for (int c = N / 32 - 1; c >= 0; c--) {
+            if (c < N / 32 - 1) {
               tmem_ld32(ts + 32 * c, s);
-              score(s, n0 + 32 * c);
+              score(s, 32 * c, true);
             }
             uint32_t p[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float e[2];
-#pragma unroll
-              for (int j = 0; j < 2; j++) {
-                const int n = 32 * c + i + j;
-                const float x = __uint_as_float(s[i + j]);
-                e[j] = ex2(x);
-                l[n] += e[j];
-                // an unseen key's value may be NaN
-                const bool in = whole || x != -INFINITY;
-                if (BITS == 4 && in) base[n % (BITS == 4 ? Half : 1)] =
-                    fmaf(e[j], mv, base[n % (BITS == 4 ? Half : 1)]);
-                e[j] = in ? e[j] * wv : 0.0f;
-              }
-              p[i / 2] = h2(__floats2half2_rn(e[0], e[1]));
+            for (int i = 0; i < 16; i++) {
+              const int n = 16 * c + i;
+              const Pair e = pair(ex2(__uint_as_float(s[2 * i])), ex2(__uint_as_float(s[2 * i + 1])));
+              l[n] = add2(l[n], e);
+              const float2 y = unpair(mul2(e, wv2));
+              if (BITS == 4) base[n % NB] = fma2(e, mv2, base[n % NB]);
+              p[i] = h2(__floats2half2_rn(y.x, y.y));
             }
-            const uint32_t n = n0 + 32 * c;
-            uint8_t *to = pt + n / 64 * (kTileKeys * 128);
+            if (odd) {
+              // this key's value is NaN: to the rows that see it, and to no other
+#pragma unroll
+              for (int i = 0; i < 16; i++) {
+                const bool in0 = s[2 * i] != 0xff800000u, in1 = s[2 * i + 1] != 0xff800000u;
+                p[i] = (in0 ? 0x7e00u : 0u) | (in1 ? 0x7e000000u : 0u);
+              }
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++)
-              *reinterpret_cast<uint4 *>(to + (((n % 64 / 8 + j) ^ (mykey & 7)) << 4)) =
+              *reinterpret_cast<uint4 *>(pt + (((4 * c + j) ^ (mykey & 7)) << 4)) =
                   make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
           }
           fence_before();
@@ -731,79 +809,106 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           }
         }
 
-        // ---- the end of the item: sums over the keys, and the output ----
+        // ---- the end of the item: the groups' sums over their keys, joined, and
+        // the output ----
+        const uint32_t n_tiles = w.t1 - w.t0, last = it + n_tiles - 1;
         const bool part_of = !(w.t0 == 0 && w.t1 == w.tiles);
         const uint32_t slot = 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0);
+        const bool has[2] = {n_tiles > 1 || (it & 1) == 0, n_tiles > 1 || (it & 1) == 1};
 #pragma unroll
-        for (int c = 0; c < Half / 32; c++) {
+        for (int c = 0; c < N / 32; c++) {
           float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; i++) v[i] = l[32 * c + i];
-          warp_part[(warp & 3) * N + n0 + 32 * c + lane] = sums32(v);
+          for (int i = 0; i < 16; i++) {
+            const float2 y = unpair(l[16 * c + i]);
+            v[2 * i] = y.x;
+            v[2 * i + 1] = y.y;
+          }
+          warp_part[warp * N + 32 * c + lane] = sums32(v);
+          if (BITS == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const float2 y = unpair(base[(16 * c + i) % NB]);
+              v[2 * i] = y.x;
+              v[2 * i + 1] = y.y;
+            }
+            warp_base[warp * N + 32 * c + lane] = sums32(v);
+          }
         }
+        if (quad == 0 && lane == 0) backs[group] = 1.0f / vs;
         soft_sync();
         if (tid < N) {
-          const float sum = (warp_part[tid] + warp_part[N + tid]) +
-                            (warp_part[2 * N + tid] + warp_part[3 * N + tid]);
-          const bool empty = masks[tid] == 0 || sum == 0.0f;
-          const float top = ref[tid].y == kFar ? -INFINITY : -ref[tid].y;
+          float top[2], sum[2], mid[2] = {0.0f, 0.0f}, c[2], all = 0.0f;
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            const float *p = warp_part + u * 4 * N + tid, *q = warp_base + u * 4 * N + tid;
+            sum[u] = (p[0] + p[N]) + (p[2 * N] + p[3 * N]);
+            if (BITS == 4) mid[u] = (q[0] + q[N]) + (q[2 * N] + q[3 * N]);
+            top[u] = refs[u * N + tid] == kFar ? -INFINITY : -refs[u * N + tid];
+          }
+          const float most = fmaxf(top[0], top[1]);
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            c[u] = top[u] == -INFINITY ? 0.0f : ex2(top[u] - most);
+            if (sum[u] != sum[u]) c[u] = 1.0f;       // NaN scores may have left no maximum
+            all = fmaf(c[u], sum[u], all);
+          }
+          const bool empty = masks[tid] == 0 || all == 0.0f;
           const uint32_t row = w.row0 + tid;
           if (part_of) {
-            a.part_ml[((uint64_t)slot * N + tid) * 2] = top;
-            a.part_ml[((uint64_t)slot * N + tid) * 2 + 1] = sum;
+            a.part_ml[((uint64_t)slot * N + tid) * 2] = most;
+            a.part_ml[((uint64_t)slot * N + tid) * 2 + 1] = all;
           } else if (row < a.rows && a.lse) {
             a.lse[((uint64_t)w.b * a.nodes + row / a.group) * a.heads + w.head * a.group +
-                  row % a.group] = empty ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+                  row % a.group] = empty ? -INFINITY : (most + log2f(all)) * 0.6931471805599453f;
           }
-          // what the output is multiplied by: 0 stands for a row without keys
-          keep[tid] = part_of ? 1.0f : empty ? 0.0f : 1.0f / sum;
-          qsum[tid] = 0.0f;
-        }
-        if (BITS == 4) {
-          soft_sync();                       // the sums of the weights are read
+          // what the outputs are multiplied by: 0 where there is nothing to read
+          const float by = part_of ? 1.0f : empty ? 0.0f : 1.0f / all;
+          float add = 0.0f;
 #pragma unroll
-          for (int c = 0; c < Half / 32; c++) {
-            float v[32];
-#pragma unroll
-            for (int i = 0; i < 32; i++) v[i] = base[(32 * c + i) % (BITS == 4 ? Half : 1)];
-            warp_part[(warp & 3) * N + n0 + 32 * c + lane] = sums32(v);
+          for (int u = 0; u < 2; u++) {
+            const float k = has[u] && !(empty && !part_of) ? c[u] * by : 0.0f;
+            keeps[u * N + tid] = k * backs[u];
+            if (k != 0.0f) add = fmaf(k, mid[u], add);
           }
-          soft_sync();
-          if (tid < N)
-            qsum[tid] = (warp_part[tid] + warp_part[N + tid]) +
-                        (warp_part[2 * N + tid] + warp_part[3 * N + tid]);
+          qsum[tid] = add;
         }
         soft_sync();
-        bar_wait(pvdone + 8 * ((it - 1) & 1), (it - 1) >> 1 & 1, alive, err);
+        bar_wait(pvdone + 8 * (last & 1), last >> 1 & 1, alive, err);
+        if (n_tiles > 1) bar_wait(pvdone + 8 * (last - 1 & 1), (last - 1) >> 1 & 1, alive, err);
         fence_after();
-        const float back = 1.0f / vs;
         const uint32_t d = natural<BITS>(mykey);       // the value this TMEM lane holds
-#pragma unroll
-        for (int c = 0; c < Half / 32; c++) {
-          uint32_t o[32];
-          tmem_ld32(tmem + (quad << 16) + L::TO + n0 + 32 * c, o);
+#pragma unroll 1
+        for (uint32_t n0 = group * (N / 2); n0 < (group + 1) * (N / 2); n0 += 16) {
+          uint32_t o[2][16];
+          tmem_ld16(tmem + (quad << 16) + L::TO + n0, o[0]);
+          tmem_ld16(tmem + (quad << 16) + L::TO + N + n0, o[1]);
+          tmem_wait_ld();
           if (HD == 128 || quad < 64) {
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
-              const uint32_t n = n0 + 32 * c + i;
-              const float v = fmaf(__uint_as_float(o[i]), back, qsum[n]), by = keep[n];
-              if (part_of) {
-                a.part_o[((uint64_t)slot * N + n) * HD + d] = v;
-              } else if (offs[n] != ~0ull) {
-                ((__nv_bfloat16 *)a.o)[offs[n] + d] =
-                    __float2bfloat16_rn(by == 0.0f ? 0.0f : v * by);
+            for (int i = 0; i < 16; i++) {
+              const uint32_t n = n0 + i;
+              float v = qsum[n];
+#pragma unroll
+              for (int u = 0; u < 2; u++) {
+                const float k = keeps[u * N + n];
+                if (k != 0.0f) v = fmaf(__uint_as_float(o[u][i]), k, v);
               }
+              if (part_of) a.part_o[((uint64_t)slot * N + n) * HD + d] = v;
+              else if (offs[n] != ~0ull)
+                ((__nv_bfloat16 *)a.o)[offs[n] + d] = __float2bfloat16_rn(v);
             }
           }
         }
         fence_before();
         soft_sync();                         // the rows are read: the next item may write them
+        it += n_tiles;
       }
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 17) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
   }
@@ -861,7 +966,7 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
   }
   a.ctas = 148;
   a.tile = kTileKeys;
-  a.item_cost = 4;
+  a.item_cost = 12;
   int *err = wait_flag_device();
   if (!err) return cudaErrorMemoryAllocation;
   count_launches(1);
@@ -876,14 +981,14 @@ uint32_t tree_umma_rows(const TreeArgs &a, bool bf16) {
       (uint64_t)a.pool.num_blocks * a.pool.kv_heads * a.pool.block_size > INT32_MAX ||
       !a.pool.num_blocks || (uint64_t)a.batch * a.nodes * a.heads >= kNone || !encode_fn())
     return 0;
-  return a.pool.bits == 8 && a.rows > 64 ? 128 : 64;
+  return a.pool.bits == 8 && a.rows > 32 ? 64 : 32;
 }
 
 cudaError_t tree_umma_start(TreeArgs &a, cudaStream_t st) {
   const bool h128 = a.pool.head_dim == 128;
-  if (a.pool.bits == 4) return h128 ? start<128, 4, 64>(a, st) : start<64, 4, 64>(a, st);
-  if (a.rows_at_once == 64) return h128 ? start<128, 8, 64>(a, st) : start<64, 8, 64>(a, st);
-  return h128 ? start<128, 8, 128>(a, st) : start<64, 8, 128>(a, st);
+  if (a.pool.bits == 4) return h128 ? start<128, 4, 32>(a, st) : start<64, 4, 32>(a, st);
+  if (a.rows_at_once == 32) return h128 ? start<128, 8, 32>(a, st) : start<64, 8, 32>(a, st);
+  return h128 ? start<128, 8, 64>(a, st) : start<64, 8, 64>(a, st);
 }
 
 }  // namespace nl
