@@ -12,19 +12,20 @@
 // threads per tile), and float16 has the room: scales are brought below 2^7.
 //
 // 20 warps, one CTA per SM, tiles of 128 keys:
-//   warps 0-7   two groups that take the tiles in turn, a thread per key:
-//               scores from TMEM, weights to shared memory (the N x 128 operand
-//               with N contiguous), sums of the weights in registers.  Each
-//               group has its own references, sums and output accumulator, so
-//               they wait for each other only at the end of an item, where the
-//               two outputs are read, a thread per value, and joined;
+//   warps 0-7   two groups, half the rows each, a thread per key: scores from
+//               TMEM, weights to shared memory (the N x 128 operand with N
+//               contiguous), sums of the weights in registers; at the end of
+//               an item the output, a thread per value.  A group has its own
+//               references and votes, so the two do not wait for each other;
 //   warps 8-11  key codes to float16 in a TMEM stage, a thread per key;
 //   warps 12-15 value codes to float16 in a shared-memory stage ([key][value],
 //               read as V^T), a thread per key;
 //   warp 16     TMA of the code tiles, one box per run of a page;
 //   warp 17     allocates TMEM and issues the MMAs of the scores;
-//   warps 18,19 issue those of the output, a group's each: one thread would
-//               need longer to issue all of a tile's than they run.
+//   warp 18     issues those of the output (warp 19 has nothing to do).  Both
+//               run as whole warps of which one thread issues, so that the
+//               descriptors are formed in uniform registers: from a single
+//               thread's branch the issue of a tile took longer than its work.
 // The 96 registers a thread of the launch are shared out anew: 152 for the
 // score warps, which hold the sums of their rows, 56, 72 and 48 for the others
 // (2 x 152 + 56 + 72 + 48 = 5 x 96).
@@ -46,7 +47,7 @@ namespace {
 constexpr int kThreads = 640;
 constexpr int kSoft = 256;                 // threads of the score warps
 constexpr int kTileKeys = 128;
-constexpr uint32_t kWaitRounds = 4096, kSuspendNs = 1000000;
+constexpr uint32_t kWaitTries = 1u << 22;
 constexpr float kFar = 1.0e30f;            // a row that has met no key: -reference
 
 template <int HD, int BITS, int N> struct Plan {
@@ -61,19 +62,19 @@ template <int HD, int BITS, int N> struct Plan {
   static constexpr int V = Stages * 2 * Codes, P = V + 2 * VTile, Q = P + 2 * PTile;
   static constexpr int Factor = Q + QTile;                    // floats
   static constexpr int Sum = Factor + N * 4;
-  static constexpr int Ref = Sum + N * 4;                     // [2][N]
-  static constexpr int Keep = Ref + 2 * N * 4;                // [2][N]
-  static constexpr int Masks = Keep + 2 * N * 4;
+  static constexpr int Ref = Sum + N * 4;
+  static constexpr int Keep = Ref + N * 4;
+  static constexpr int Masks = Keep + N * 4;
   static constexpr int Offs = Masks + N * 8;                  // output offsets
-  static constexpr int Warp = Offs + N * 8;                   // [8][N]
-  static constexpr int Base = Warp + 8 * N * 4;               // [8][N] (4 bits)
-  static constexpr int Bars = Base + (BITS == 4 ? 8 * N * 4 : 0);
+  static constexpr int Warp = Offs + N * 8;                   // [4][N]
+  static constexpr int Base = Warp + 4 * N * 4;               // [4][N] (4 bits)
+  static constexpr int Bars = Base + (BITS == 4 ? 4 * N * 4 : 0);
   static constexpr int Used = Bars + 256 + 1024;
   static constexpr int Bytes = Used > 120 * 1024 ? Used : 120 * 1024;   // one CTA per SM (TMEM)
-  // TMEM columns: two stages of keys and of scores, two outputs
+  // TMEM columns: two stages of keys and of scores, the output
   static constexpr uint32_t KCols = HD / 2;
   static constexpr uint32_t TK = 0, TS = 2 * KCols, TO = TS + 2 * N;
-  static_assert(TO + 2 * N <= 512 && Used <= 227 * 1024, "tile");
+  static_assert(TO + N <= 512 && Used <= 227 * 1024, "tile");
 };
 
 __device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) {
@@ -87,14 +88,17 @@ __device__ __forceinline__ void bar_arrive(uint32_t b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(b) : "memory");
 }
 // A bounded wait; ALIVE goes false when one gives up, and no later one waits.
+// Without a suspend-time hint: with one a waiter may sleep on, and a tile
+// passes through ten waits.
 __device__ __forceinline__ void bar_wait(uint32_t b, uint32_t parity, bool &alive, int *err) {
   if (!alive) return;
-  for (uint32_t i = 0; i < kWaitRounds; i++) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kWaitTries; i++) {
     uint32_t done;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done) : "r"(b), "r"(parity), "r"(kSuspendNs) : "memory");
+        : "=r"(done) : "r"(b), "r"(parity) : "memory");
     if (done) return;
   }
   report_wait_timeout(err);
@@ -180,6 +184,18 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) 
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
 }
+template <int H> __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&v)[H]) {
+  if constexpr (H == 32) {
+    tmem_ld32(at, v);
+  } else {
+    tmem_ld16(at, v);
+    tmem_wait_ld();
+  }
+}
+template <int H> __device__ __forceinline__ void tmem_st(uint32_t at, const uint32_t (&v)[H]) {
+  if constexpr (H == 32) tmem_st32(at, v);
+  else tmem_st16(at, v);
+}
 // Shared-memory operands in the 128-byte swizzle, rows of 128 bytes in groups
 // of eight 1024 bytes apart: rows of the M or N index with 64 K values
 // (K-major), or rows of the K index with 64 M or N values, 64-value blocks
@@ -193,23 +209,33 @@ template <int N, bool MN> constexpr uint32_t instr_desc() {
   return (1u << 4) | (MN ? (1u << 15) | (1u << 16) : 0u) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+// Issued by the thread whose ME is set; every lane comes here with the same
+// operands.
+__device__ __forceinline__ uint32_t elect() {
+  uint32_t me;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(me));
+  return me;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t me, uint32_t d, uint32_t a, uint64_t b,
+                                       uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(me));
 }
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(
-                   bar) : "memory");
+__device__ __forceinline__ void mma_ss(uint32_t me, uint32_t d, uint64_t a, uint64_t b,
+                                       uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(me));
+}
+__device__ __forceinline__ void mma_commit(uint32_t me, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
+          bar), "r"(me) : "memory");
 }
 
 // The order in which a word's codes leave the conversion: natural for 8 bits;
@@ -260,33 +286,30 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   return r;
 }
 
-// The largest over a warp's lanes of each of 32 values: lane i gets that of v[i].
-__device__ __forceinline__ float tops32(float (&v)[32]) {
+// The largest, or the sum, over a warp's lanes of each of H values: lane i < H
+// gets that of v[i].
+template <int H, bool SUM> __device__ __forceinline__ float across(uint32_t (&v)[H]) {
   const uint32_t lane = threadIdx.x & 31;
+  auto join = [](float x, float y) { return SUM ? x + y : fmaxf(x, y); };
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = H / 2; o > 0; o >>= 1) {
     const bool high = lane & o;
 #pragma unroll
     for (int i = 0; i < o; i++) {
-      const float give = high ? v[i] : v[i + o], keep = high ? v[i + o] : v[i];
-      v[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o));
+      const uint32_t give = high ? v[i] : v[i + o], have = high ? v[i + o] : v[i];
+      v[i] = __float_as_uint(join(__uint_as_float(have),
+                                  __uint_as_float(__shfl_xor_sync(0xffffffffu, give, o))));
     }
   }
-  return v[0];
+  float r = __uint_as_float(v[0]);
+  if (H == 16) r = join(r, __shfl_xor_sync(0xffffffffu, r, 16));
+  return r;
 }
-// The sum over a warp's lanes of each of 32 values: lane i gets that of v[i].
-__device__ __forceinline__ float sums32(float (&v)[32]) {
-  const uint32_t lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const bool high = lane & o;
-#pragma unroll
-    for (int i = 0; i < o; i++) {
-      const float give = high ? v[i] : v[i + o], keep = high ? v[i + o] : v[i];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-    }
-  }
-  return v[0];
+template <int H> __device__ __forceinline__ float tops(uint32_t (&v)[H]) {
+  return across<H, false>(v);
+}
+template <int H> __device__ __forceinline__ float sums(uint32_t (&v)[H]) {
+  return across<H, true>(v);
 }
 
 // The walk over the parts of items that a CTA has, the same in every role.
@@ -332,14 +355,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, uint32_t box, int *err) {
   using L = Plan<HD, BITS, N>;
+  constexpr int H = N / 2;                   // rows of a group of score warps
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                             ~(uintptr_t)1023);
   const uint32_t s0 = su32(sm);
   float *factor = reinterpret_cast<float *>(sm + L::Factor);  // of a row's scores
   float *qsum = reinterpret_cast<float *>(sm + L::Sum);       // the sum of its query
-  float *refs = reinterpret_cast<float *>(sm + L::Ref);       // less a group's reference
-  float *keeps = reinterpret_cast<float *>(sm + L::Keep);     // what a new one leaves of the sums
+  float *ref = reinterpret_cast<float *>(sm + L::Ref);        // less its reference
+  float *keep = reinterpret_cast<float *>(sm + L::Keep);      // what a new one leaves of the sums
   uint64_t *masks = reinterpret_cast<uint64_t *>(sm + L::Masks);
   uint64_t *offs = reinterpret_cast<uint64_t *>(sm + L::Offs);
   float *warp_part = reinterpret_cast<float *>(sm + L::Warp);
@@ -350,7 +374,6 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
                  qready = bars + 144;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + L::Bars + 160);
   uint32_t *votes = tmem_slot + 1;           // the largest scale of a group's tile
-  float *backs = reinterpret_cast<float *>(tmem_slot + 3);   // a group's 1 / vs
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -361,9 +384,9 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
     for (int i = 0; i < 2; i++) {
       bar_init(kready + 8 * i, 4);
       bar_init(qkdone + 8 * i, 1);
-      bar_init(sfree + 8 * i, 4);
+      bar_init(sfree + 8 * i, 8);
       bar_init(vready + 8 * i, 4);
-      bar_init(pready + 8 * i, 4);
+      bar_init(pready + 8 * i, 8);
       bar_init(pvdone + 8 * i, 1);
     }
     bar_init(qready, 8);
@@ -420,52 +443,44 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           bar_wait(full + 8 * (i % L::Stages), i / L::Stages & 1, alive, err);
       } else if (warp == 17) {
         // ---- the score products ----
+        const uint32_t me = elect();
         uint32_t item = 0;
         while (w.next(a)) {
-          if (lane == 0) {
-            bar_wait(qready, item & 1, alive, err);
-            for (uint32_t i = it; i < it + (w.t1 - w.t0); i++) {
-              const uint32_t st = i & 1, ph = i >> 1 & 1;
-              bar_wait(kready + 8 * st, ph, alive, err);
-              bar_wait(sfree + 8 * st, ph ^ 1, alive, err);
-              fence_after();
-              const uint64_t q = smem_desc(s0 + L::Q, 16);
-#pragma unroll
-              for (int k = 0; k < HD / 16; k++)
-                mma_ts(tmem + L::TS + st * N, tmem + L::TK + st * L::KCols + 8 * k,
-                       q + (k / 4 * (N * 128) + k % 4 * 32) / 16, instr_desc<N, false>(),
-                       k ? 1u : 0u);
-              mma_commit(qkdone + 8 * st);
-            }
-          }
-          __syncwarp();
-          it += w.t1 - w.t0;
+          bar_wait(qready, item & 1, alive, err);
           item++;
-        }
-      } else {
-        // ---- the output products, each group's into its own accumulator ----
-        const uint32_t st = warp - 18;
-        while (w.next(a)) {
-          if (lane == 0) {
-            const uint32_t i0 = it + ((it ^ st) & 1);
-            for (uint32_t i = i0; i < it + (w.t1 - w.t0); i += 2) {
-              const uint32_t ph = i >> 1 & 1;
-              bar_wait(vready + 8 * st, ph, alive, err);
-              bar_wait(pready + 8 * st, ph, alive, err);
-              fence_after();
-              // 16 keys on is 2048 bytes on: 128 in a descriptor's address field
-              const uint64_t v = smem_desc(s0 + L::V + st * L::VTile,
-                                           HD == 128 ? kTileKeys * 128 : 0);
-              const uint64_t p = smem_desc(s0 + L::P + st * L::PTile, 16);
+          for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
+            const uint32_t st = it & 1, ph = it >> 1 & 1;
+            bar_wait(kready + 8 * st, ph, alive, err);
+            bar_wait(sfree + 8 * st, ph ^ 1, alive, err);
+            fence_after();
+            const uint64_t q = smem_desc(s0 + L::Q, 16);
 #pragma unroll
-              for (int k = 0; k < kTileKeys / 16; k++)
-                mma_ss(tmem + L::TO + st * N, v + 128 * k, p + 128 * k, instr_desc<N, true>(),
-                       k == 0 && i == i0 ? 0u : 1u);
-              mma_commit(pvdone + 8 * st);
-            }
+            for (int k = 0; k < HD / 16; k++)
+              mma_ts(me, tmem + L::TS + st * N, tmem + L::TK + st * L::KCols + 8 * k,
+                     q + (k / 4 * (N * 128) + k % 4 * 32) / 16, instr_desc<N, false>(),
+                     k ? 1u : 0u);
+            mma_commit(me, qkdone + 8 * st);
           }
-          __syncwarp();
-          it += w.t1 - w.t0;
+        }
+      } else if (warp == 18) {
+        // ---- the output products ----
+        const uint32_t me = elect();
+        while (w.next(a)) {
+          for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
+            const uint32_t st = it & 1, ph = it >> 1 & 1;
+            bar_wait(vready + 8 * st, ph, alive, err);
+            bar_wait(pready + 8 * st, ph, alive, err);
+            fence_after();
+            // 16 keys on is 2048 bytes on: 128 in a descriptor's address field
+            const uint64_t v = smem_desc(s0 + L::V + st * L::VTile,
+                                         HD == 128 ? kTileKeys * 128 : 0);
+            const uint64_t p = smem_desc(s0 + L::P + st * L::PTile, 16);
+#pragma unroll
+            for (int k = 0; k < kTileKeys / 16; k++)
+              mma_ss(me, tmem + L::TO, v + 128 * k, p + 128 * k, instr_desc<N, true>(),
+                     k == 0 && tile == w.t0 ? 0u : 1u);
+            mma_commit(me, pvdone + 8 * st);
+          }
         }
       }
     } else if (warp >= 8) {
@@ -554,12 +569,11 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
       asm volatile("setmaxnreg.inc.sync.aligned.u32 152;\n");
       const uint32_t group = warp >> 2, quad = (warp & 3) * 32, mykey = quad + lane;
       const uint32_t tid = threadIdx.x;
-      float *ref = refs + group * N, *keep = keeps + group * N;
+      const uint32_t n0 = group * H;
       uint32_t *vote = votes + group;
       const uint64_t used = a.nodes < 64 ? (1ull << a.nodes) - 1 : ~0ull;
       while (w.next(a)) {
         const uint32_t prefix = prefix_of(a, w.b), keys = keys_of(a, w.b);
-        const uint32_t mine0 = w.t0 + ((it ^ group) & 1);        // this group's first tile
         // the parameter words of this thread's key of a tile, found a tile ahead
         auto page_of = [&](uint32_t key) {
           return a.block_shift < 32 ? key >> a.block_shift : key / a.pool.block_size;
@@ -579,7 +593,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           *vw = __ldg(a.pool.param[1] + row);
           return true;
         };
-        uint32_t block1 = block_of(mine0), kw1, vw1;
+        uint32_t block1 = block_of(w.t0), kw1, vw1;
 
         // the queries of the item, float16, K-major
         {
@@ -629,7 +643,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             // a factor is never zero: it would make NaN of a masked score
             factor[n] = fmaxf(a.scale * __uint_as_float((uint32_t)(127 - up) << 23),
                               1.17549435e-38f);
-            refs[n] = refs[N + n] = kFar;
+            ref[n] = kFar;
             qsum[n] = sum;
             masks[n] = live ? a.mask[out_row] & used : 0;
             offs[n] = live ? out_row * a.o_stride + (uint64_t)col * HD : ~0ull;
@@ -639,21 +653,21 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         soft_sync();
         if (lane == 0) bar_arrive(qready);
 
-        constexpr int NB = BITS == 4 ? N / 2 : 1;
-        Pair l[N / 2], base[NB];
+        constexpr int NB = BITS == 4 ? H / 2 : 1;
+        Pair l[H / 2], base[NB];
 #pragma unroll
-        for (int i = 0; i < N / 2; i++) l[i] = base[i % NB] = 0;
+        for (int i = 0; i < H / 2; i++) l[i] = base[i % NB] = 0;
         float vs = 1.0f;
         uint32_t vlimit = 0;
-        bool have1 = words_of(mine0, block1, &kw1, &vw1);
-        block1 = block_of(mine0 + 2);
+        bool have1 = words_of(w.t0, block1, &kw1, &vw1);
+        block1 = block_of(w.t0 + 1);
 
-        for (uint32_t tile = mine0; tile < w.t1; tile += 2) {
-          const uint32_t i0 = it + (tile - w.t0), st = group, ph = i0 >> 1 & 1;
+        for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
+          const uint32_t st = it & 1, ph = it >> 1 & 1;
           const bool have = have1;
           const uint32_t kw = kw1, vw = vw1;
-          have1 = words_of(tile + 2, block1, &kw1, &vw1);
-          block1 = block_of(tile + 4);
+          have1 = words_of(tile + 1, block1, &kw1, &vw1);
+          block1 = block_of(tile + 2);
           const float sk = scale_of<BITS>(kw);
           const float mk = middle_of(kw);
           const Pair sk2 = pair(sk, sk), mk2 = pair(mk, mk);
@@ -664,11 +678,12 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           const uint32_t key = tile * kTileKeys + mykey;
           // tiles of prefix keys that all exist need no masks
           const bool whole = __all_sync(0xffffffffu, have && key < prefix);
-          // the scores of 32 rows from n on this key, in powers of two: over the
-          // rows' references (less 0) or as they are
-          auto score = [&](uint32_t (&s)[32], uint32_t n, bool over_ref) {
+          // the scores of the group's rows on this key, in powers of two: over the
+          // rows' references, or as they are
+          auto score = [&](uint32_t (&s)[H], bool over_ref) {
+            const uint32_t n = n0;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
+            for (int i = 0; i < H; i += 4) {
               float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
               if (BITS == 4) q = *reinterpret_cast<const float4 *>(qsum + n + i);
               const float4 f = *reinterpret_cast<const float4 *>(factor + n + i);
@@ -686,8 +701,8 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
               }
             }
             if (!whole) {
-#pragma unroll
-              for (int i = 0; i < 32; i++) {
+#pragma unroll 8
+              for (int i = 0; i < H; i++) {
                 const uint64_t m = masks[n + i];
                 const bool seen = have && (key < prefix ? m != 0
                                                         : key - prefix < 64 && (m >> (key - prefix) & 1));
@@ -697,41 +712,31 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           };
           bar_wait(qkdone + 8 * st, ph, alive, err);
           fence_after();
-          const uint32_t ts = tmem + (quad << 16) + L::TS + st * N;
-          uint32_t s[32];
+          const uint32_t ts = tmem + (quad << 16) + L::TS + st * N + n0;
+          uint32_t s[H];
           for (bool again = false;; again = true) {
-            bool over = vbits >= vlimit && vbits != 0;
-            // the last 32 rows stay in registers for their weights
+            tmem_ld<H>(ts, s);
+            score(s, true);
+            float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < N / 32; c++) {
-              tmem_ld32(ts + 32 * c, s);
-              score(s, 32 * c, true);
-              float top = -INFINITY;
-#pragma unroll
-              for (int i = 0; i < 32; i++) top = fmaxf(top, __uint_as_float(s[i]));
-              over |= top > 8.0f;
-            }
+            for (int i = 0; i < H; i++) top = fmaxf(top, __uint_as_float(s[i]));
+            const bool over = top > 8.0f || (vbits >= vlimit && vbits != 0);
             if (again || !group_any(group, over)) break;
             // ---- new references: the maxima of the keys so far ----
-#pragma unroll 1
-            for (int c = 0; c < N / 32; c++) {
-              tmem_ld32(ts + 32 * c, s);
-              score(s, 32 * c, false);
-              float x[32];
-#pragma unroll
-              for (int i = 0; i < 32; i++) x[i] = __uint_as_float(s[i]);
-              warp_part[warp * N + 32 * c + lane] = tops32(x);
-            }
-            if ((warp & 3) == 0 && lane == 0) *vote = 0;
+            tmem_ld<H>(ts, s);
+            score(s, false);
+            const float mine = tops<H>(s);
+            if (lane < H) warp_part[(warp & 3) * N + n0 + lane] = mine;
+            if (quad == 0 && lane == 0) *vote = 0;
             group_sync(group);
             const uint32_t top_bits = __reduce_max_sync(0xffffffffu, vbits);
             if (lane == 0) atomicMax(vote, top_bits);
-            if (mykey < N) {
-              const float *p = warp_part + group * 4 * N + mykey;
-              const float top = fmaxf(fmaxf(p[0], p[N]), fmaxf(p[2 * N], p[3 * N]));
-              const float old = -ref[mykey];                 // -kFar: no key met yet
-              keep[mykey] = top > old ? ex2(old - top) : 1.0f;
-              if (top > old) ref[mykey] = -top;
+            if (mykey < H) {
+              const float *p = warp_part + n0 + mykey;
+              const float most = fmaxf(fmaxf(p[0], p[N]), fmaxf(p[2 * N], p[3 * N]));
+              const float old = -ref[n0 + mykey];            // -kFar: no key met yet
+              keep[n0 + mykey] = most > old ? ex2(old - most) : 1.0f;
+              if (most > old) ref[n0 + mykey] = -most;
             }
             group_sync(group);
             float ratio = 1.0f;
@@ -745,61 +750,51 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             }
             // the sums, and the output so far once its last product is done
 #pragma unroll
-            for (int i = 0; i < N / 2; i++) {
-              const float2 k = *reinterpret_cast<const float2 *>(keep + 2 * i);
+            for (int i = 0; i < H / 2; i++) {
+              const float2 k = *reinterpret_cast<const float2 *>(keep + n0 + 2 * i);
               l[i] = mul2(l[i], pair(k.x, k.y));
               if (BITS == 4) base[i % NB] = mul2(base[i % NB], pair(k.x, k.y));
             }
-            if (tile > mine0) {
-              bar_wait(pvdone + 8 * st, ph ^ 1, alive, err);
+            if (tile > w.t0) {
+              bar_wait(pvdone + 8 * (st ^ 1), (it - 1) >> 1 & 1, alive, err);
               fence_after();
-              const uint32_t to = tmem + (quad << 16) + L::TO + st * N;
-#pragma unroll 1
-              for (int c = 0; c < N / 32; c++) {
-                tmem_ld32(to + 32 * c, s);
+              const uint32_t to = tmem + (quad << 16) + L::TO + n0;
+              tmem_ld<H>(to, s);
 #pragma unroll
-                for (int i = 0; i < 32; i++)
-                  s[i] = __float_as_uint(__uint_as_float(s[i]) * (keep[32 * c + i] * ratio));
-                tmem_st32(to + 32 * c, s);
-              }
+              for (int i = 0; i < H; i++)
+                s[i] = __float_as_uint(__uint_as_float(s[i]) * (keep[n0 + i] * ratio));
+              tmem_st<H>(to, s);
               tmem_wait_st();
             }
           }
           // ---- the weights ----
           const float wv = sv * vs;
+          // an unseen key's value may be NaN
           const bool odd = !(fabsf(wv) < INFINITY);
           const Pair wv2 = pair(wv, wv), mv2 = pair(mv, mv);
           bar_wait(pvdone + 8 * st, ph ^ 1, alive, err);       // the buffer's last reader
           uint8_t *pt = sm + L::P + st * L::PTile + mykey * 128;
+          uint32_t p[H / 2];
 #pragma unroll
-          for (int c = N / 32 - 1; c >= 0; c--) {
-            if (c < N / 32 - 1) {
-              tmem_ld32(ts + 32 * c, s);
-              score(s, 32 * c, true);
-            }
-            uint32_t p[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const int n = 16 * c + i;
-              const Pair e = pair(ex2(__uint_as_float(s[2 * i])), ex2(__uint_as_float(s[2 * i + 1])));
-              l[n] = add2(l[n], e);
-              const float2 y = unpair(mul2(e, wv2));
-              if (BITS == 4) base[n % NB] = fma2(e, mv2, base[n % NB]);
-              p[i] = h2(__floats2half2_rn(y.x, y.y));
-            }
-            if (odd) {
-              // this key's value is NaN: to the rows that see it, and to no other
-#pragma unroll
-              for (int i = 0; i < 16; i++) {
-                const bool in0 = s[2 * i] != 0xff800000u, in1 = s[2 * i + 1] != 0xff800000u;
-                p[i] = (in0 ? 0x7e00u : 0u) | (in1 ? 0x7e000000u : 0u);
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              *reinterpret_cast<uint4 *>(pt + (((4 * c + j) ^ (mykey & 7)) << 4)) =
-                  make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+          for (int i = 0; i < H / 2; i++) {
+            const Pair e = pair(ex2(__uint_as_float(s[2 * i])), ex2(__uint_as_float(s[2 * i + 1])));
+            l[i] = add2(l[i], e);
+            const float2 y = unpair(mul2(e, wv2));
+            if (BITS == 4) base[i % NB] = fma2(e, mv2, base[i % NB]);
+            p[i] = h2(__floats2half2_rn(y.x, y.y));
           }
+          if (odd) {
+            // this key's value is NaN: to the rows that see it, and to no other
+#pragma unroll
+            for (int i = 0; i < H / 2; i++) {
+              const bool in0 = s[2 * i] != 0xff800000u, in1 = s[2 * i + 1] != 0xff800000u;
+              p[i] = (in0 ? 0x7e00u : 0u) | (in1 ? 0x7e000000u : 0u);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < H / 8; j++)
+            *reinterpret_cast<uint4 *>(pt + (((n0 / 8 + j) ^ (mykey & 7)) << 4)) =
+                make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
           fence_before();
           fence_async();
           __syncwarp();
@@ -809,100 +804,71 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           }
         }
 
-        // ---- the end of the item: the groups' sums over their keys, joined, and
-        // the output ----
-        const uint32_t n_tiles = w.t1 - w.t0, last = it + n_tiles - 1;
+        // ---- the end of the item: sums over the keys, and the output ----
         const bool part_of = !(w.t0 == 0 && w.t1 == w.tiles);
         const uint32_t slot = 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0);
-        const bool has[2] = {n_tiles > 1 || (it & 1) == 0, n_tiles > 1 || (it & 1) == 1};
+        {
+          uint32_t v[H];
 #pragma unroll
-        for (int c = 0; c < N / 32; c++) {
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float2 y = unpair(l[16 * c + i]);
-            v[2 * i] = y.x;
-            v[2 * i + 1] = y.y;
+          for (int i = 0; i < H / 2; i++) {
+            const float2 y = unpair(l[i]);
+            v[2 * i] = __float_as_uint(y.x);
+            v[2 * i + 1] = __float_as_uint(y.y);
           }
-          warp_part[warp * N + 32 * c + lane] = sums32(v);
+          const float sum = sums<H>(v);
+          if (lane < H) warp_part[(warp & 3) * N + n0 + lane] = sum;
           if (BITS == 4) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const float2 y = unpair(base[(16 * c + i) % NB]);
-              v[2 * i] = y.x;
-              v[2 * i + 1] = y.y;
+            for (int i = 0; i < H / 2; i++) {
+              const float2 y = unpair(base[i % NB]);
+              v[2 * i] = __float_as_uint(y.x);
+              v[2 * i + 1] = __float_as_uint(y.y);
             }
-            warp_base[warp * N + 32 * c + lane] = sums32(v);
+            const float mid = sums<H>(v);
+            if (lane < H) warp_base[(warp & 3) * N + n0 + lane] = mid;
           }
         }
-        if (quad == 0 && lane == 0) backs[group] = 1.0f / vs;
-        soft_sync();
-        if (tid < N) {
-          float top[2], sum[2], mid[2] = {0.0f, 0.0f}, c[2], all = 0.0f;
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            const float *p = warp_part + u * 4 * N + tid, *q = warp_base + u * 4 * N + tid;
-            sum[u] = (p[0] + p[N]) + (p[2 * N] + p[3 * N]);
-            if (BITS == 4) mid[u] = (q[0] + q[N]) + (q[2 * N] + q[3 * N]);
-            top[u] = refs[u * N + tid] == kFar ? -INFINITY : -refs[u * N + tid];
-          }
-          const float most = fmaxf(top[0], top[1]);
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            c[u] = top[u] == -INFINITY ? 0.0f : ex2(top[u] - most);
-            if (sum[u] != sum[u]) c[u] = 1.0f;       // NaN scores may have left no maximum
-            all = fmaf(c[u], sum[u], all);
-          }
-          const bool empty = masks[tid] == 0 || all == 0.0f;
-          const uint32_t row = w.row0 + tid;
+        group_sync(group);
+        if (mykey < H) {
+          const uint32_t n = n0 + mykey, row = w.row0 + n;
+          const float *p = warp_part + n, *q = warp_base + n;
+          const float sum = (p[0] + p[N]) + (p[2 * N] + p[3 * N]);
+          const bool empty = masks[n] == 0 || sum == 0.0f;
+          const float top = ref[n] == kFar ? -INFINITY : -ref[n];
           if (part_of) {
-            a.part_ml[((uint64_t)slot * N + tid) * 2] = most;
-            a.part_ml[((uint64_t)slot * N + tid) * 2 + 1] = all;
+            a.part_ml[((uint64_t)slot * N + n) * 2] = top;
+            a.part_ml[((uint64_t)slot * N + n) * 2 + 1] = sum;
           } else if (row < a.rows && a.lse) {
             a.lse[((uint64_t)w.b * a.nodes + row / a.group) * a.heads + w.head * a.group +
-                  row % a.group] = empty ? -INFINITY : (most + log2f(all)) * 0.6931471805599453f;
+                  row % a.group] = empty ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
           }
-          // what the outputs are multiplied by: 0 where there is nothing to read
-          const float by = part_of ? 1.0f : empty ? 0.0f : 1.0f / all;
-          float add = 0.0f;
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            const float k = has[u] && !(empty && !part_of) ? c[u] * by : 0.0f;
-            keeps[u * N + tid] = k * backs[u];
-            if (k != 0.0f) add = fmaf(k, mid[u], add);
-          }
-          qsum[tid] = add;
+          // what the output is multiplied by, 0 for a row without keys, and what
+          // the offsets add to it
+          const float by = part_of ? 1.0f : empty ? 0.0f : 1.0f / sum;
+          keep[n] = by / vs;
+          qsum[n] = BITS == 4 && by != 0.0f ? by * ((q[0] + q[N]) + (q[2 * N] + q[3 * N])) : 0.0f;
         }
-        soft_sync();
-        bar_wait(pvdone + 8 * (last & 1), last >> 1 & 1, alive, err);
-        if (n_tiles > 1) bar_wait(pvdone + 8 * (last - 1 & 1), (last - 1) >> 1 & 1, alive, err);
+        group_sync(group);
+        bar_wait(pvdone + 8 * (it - 1 & 1), (it - 1) >> 1 & 1, alive, err);
         fence_after();
         const uint32_t d = natural<BITS>(mykey);       // the value this TMEM lane holds
-#pragma unroll 1
-        for (uint32_t n0 = group * (N / 2); n0 < (group + 1) * (N / 2); n0 += 16) {
-          uint32_t o[2][16];
-          tmem_ld16(tmem + (quad << 16) + L::TO + n0, o[0]);
-          tmem_ld16(tmem + (quad << 16) + L::TO + N + n0, o[1]);
-          tmem_wait_ld();
+        {
+          uint32_t o[H];
+          tmem_ld<H>(tmem + (quad << 16) + L::TO + n0, o);
           if (HD == 128 || quad < 64) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
+            float *part = a.part_o + ((uint64_t)slot * N + n0) * HD + d;
+#pragma unroll 8
+            for (int i = 0; i < H; i++) {
               const uint32_t n = n0 + i;
-              float v = qsum[n];
-#pragma unroll
-              for (int u = 0; u < 2; u++) {
-                const float k = keeps[u * N + n];
-                if (k != 0.0f) v = fmaf(__uint_as_float(o[u][i]), k, v);
-              }
-              if (part_of) a.part_o[((uint64_t)slot * N + n) * HD + d] = v;
-              else if (offs[n] != ~0ull)
-                ((__nv_bfloat16 *)a.o)[offs[n] + d] = __float2bfloat16_rn(v);
+              const float k = keep[n], v = k == 0.0f ? 0.0f : fmaf(__uint_as_float(o[i]), k, qsum[n]);
+              const uint64_t at = offs[n];
+              if (part_of) part[i * HD] = v;
+              else if (at != ~0ull) ((__nv_bfloat16 *)a.o)[at + d] = __float2bfloat16_rn(v);
             }
           }
         }
         fence_before();
         soft_sync();                         // the rows are read: the next item may write them
-        it += n_tiles;
       }
     }
   }
@@ -981,13 +947,17 @@ uint32_t tree_umma_rows(const TreeArgs &a, bool bf16) {
       (uint64_t)a.pool.num_blocks * a.pool.kv_heads * a.pool.block_size > INT32_MAX ||
       !a.pool.num_blocks || (uint64_t)a.batch * a.nodes * a.heads >= kNone || !encode_fn())
     return 0;
-  return a.pool.bits == 8 && a.rows > 32 ? 64 : 32;
+  return a.rows > 32 ? 64 : 32;
 }
 
 cudaError_t tree_umma_start(TreeArgs &a, cudaStream_t st) {
   const bool h128 = a.pool.head_dim == 128;
-  if (a.pool.bits == 4) return h128 ? start<128, 4, 32>(a, st) : start<64, 4, 32>(a, st);
-  if (a.rows_at_once == 32) return h128 ? start<128, 8, 32>(a, st) : start<64, 8, 32>(a, st);
+  const bool few = a.rows_at_once == 32;
+  if (a.pool.bits == 4) {
+    if (few) return h128 ? start<128, 4, 32>(a, st) : start<64, 4, 32>(a, st);
+    return h128 ? start<128, 4, 64>(a, st) : start<64, 4, 64>(a, st);
+  }
+  if (few) return h128 ? start<128, 8, 32>(a, st) : start<64, 8, 32>(a, st);
   return h128 ? start<128, 8, 64>(a, st) : start<64, 8, 64>(a, st);
 }
 
