@@ -701,7 +701,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
               }
             }
             if (!whole) {
-#pragma unroll 8
+#pragma unroll
               for (int i = 0; i < H; i++) {
                 const uint64_t m = masks[n + i];
                 const bool seen = have && (key < prefix ? m != 0
@@ -857,7 +857,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           tmem_ld<H>(tmem + (quad << 16) + L::TO + n0, o);
           if (HD == 128 || quad < 64) {
             float *part = a.part_o + ((uint64_t)slot * N + n0) * HD + d;
-#pragma unroll 8
+#pragma unroll
             for (int i = 0; i < H; i++) {
               const uint32_t n = n0 + i;
               const float k = keep[n], v = k == 0.0f ? 0.0f : fmaf(__uint_as_float(o[i]), k, qsum[n]);
