@@ -11,24 +11,23 @@
 // of the keys up to the last time one exceeded it by 2^8 (a vote of the 128
 // threads per tile), and float16 has the room: scales are brought below 2^7.
 //
-// 20 warps, one CTA per SM, tiles of 128 keys:
-//   warps 0-7   two groups, half the rows each, a thread per key: scores from
+// One CTA per SM, tiles of 128 keys, a warp group (four warps) per role:
+//   N / 16 groups of score warps, 16 rows each, a thread per key: scores from
 //               TMEM, weights to shared memory (the N x 128 operand with N
 //               contiguous), sums of the weights in registers; at the end of
 //               an item the output, a thread per value.  A group has its own
-//               references and votes, so the two do not wait for each other;
-//   warps 8-11  key codes to float16 in a TMEM stage, a thread per key;
-//   warps 12-15 value codes to float16 in a shared-memory stage ([key][value],
-//               read as V^T), a thread per key;
-//   warp 16     TMA of the code tiles, one box per run of a page;
-//   warp 17     allocates TMEM and issues the MMAs of the scores;
-//   warp 18     issues those of the output (warp 19 has nothing to do).  Both
+//               references and votes, so they do not wait for each other;
+//   keys        codes to float16 in a TMEM stage, a thread per key, and the
+//               keys' parameter words to shared memory;
+//   values      codes to float16 in a shared-memory stage ([key][value], read
+//               as V^T), a thread per key;
+//   control     one warp for the TMA of the code tiles, one box per run of a
+//               page; one that allocates TMEM and issues the MMAs of the scores;
+//               one that issues those of the output (and one idle).  The two
 //               run as whole warps of which one thread issues, so that the
 //               descriptors are formed in uniform registers: from a single
 //               thread's branch the issue of a tile took longer than its work.
-// The 96 registers a thread of the launch are shared out anew: 152 for the
-// score warps, which hold the sums of their rows, 56, 72 and 48 for the others
-// (2 x 152 + 56 + 72 + 48 = 5 x 96).
+// The registers of the launch are shared out anew among the roles.
 // The stages run on over the end of an item: the next item's codes are on
 // their way and converted while the last one's output is written.
 //
@@ -44,13 +43,17 @@
 namespace nl {
 namespace {
 
-constexpr int kThreads = 640;
-constexpr int kSoft = 256;                 // threads of the score warps
+constexpr int H = 16;                      // rows of a group of score warps
 constexpr int kTileKeys = 128;
 constexpr uint32_t kWaitTries = 1u << 22;
 constexpr float kFar = 1.0e30f;            // a row that has met no key: -reference
 
 template <int HD, int BITS, int N> struct Plan {
+  static constexpr int Groups = N / H;
+  static constexpr int Soft = 128 * Groups;                   // threads of the score warps
+  static constexpr int Threads = Soft + 3 * 128;
+  static constexpr int Regs = 65536 / Threads / 8 * 8;        // a thread, at launch
+  static constexpr int RegsSoft = (Regs * (Groups + 3) - 56 - 56 - 40) / Groups / 8 * 8;
   static constexpr int RB = HD * BITS / 8;
   static constexpr int Chunks = RB / 16;
   static constexpr int Codes = kTileKeys * RB;               // one side's codes of a tile
@@ -68,7 +71,8 @@ template <int HD, int BITS, int N> struct Plan {
   static constexpr int Offs = Masks + N * 8;                  // output offsets
   static constexpr int Warp = Offs + N * 8;                   // [4][N]
   static constexpr int Base = Warp + 4 * N * 4;               // [4][N] (4 bits)
-  static constexpr int Bars = Base + (BITS == 4 ? 4 * N * 4 : 0);
+  static constexpr int Words = Base + (BITS == 4 ? 4 * N * 4 : 0);   // [4][128] uint4
+  static constexpr int Bars = Words + 4 * kTileKeys * 16;
   static constexpr int Used = Bars + 256 + 1024;
   static constexpr int Bytes = Used > 120 * 1024 ? Used : 120 * 1024;   // one CTA per SM (TMEM)
   // TMEM columns: two stages of keys and of scores, the output
@@ -121,8 +125,8 @@ __device__ __forceinline__ void fence_after() {
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
 }
-__device__ __forceinline__ void soft_sync() {
-  asm volatile("bar.sync 1, %0;\n" ::"n"(kSoft) : "memory");
+template <int THREADS> __device__ __forceinline__ void soft_sync() {
+  asm volatile("bar.sync 1, %0;\n" ::"n"(THREADS) : "memory");
 }
 // The same for the 128 threads of one group, and whether any of them says so.
 __device__ __forceinline__ void group_sync(uint32_t group) {
@@ -144,33 +148,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
         "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
         "=r"(v[14]), "=r"(v[15])
       : "r"(at));
-}
-__device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
-      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
-        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(at));
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
-      "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(
-          at),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
-      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
-      "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile(
@@ -183,18 +161,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) 
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-}
-template <int H> __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&v)[H]) {
-  if constexpr (H == 32) {
-    tmem_ld32(at, v);
-  } else {
-    tmem_ld16(at, v);
-    tmem_wait_ld();
-  }
-}
-template <int H> __device__ __forceinline__ void tmem_st(uint32_t at, const uint32_t (&v)[H]) {
-  if constexpr (H == 32) tmem_st32(at, v);
-  else tmem_st16(at, v);
 }
 // Shared-memory operands in the 128-byte swizzle, rows of 128 bytes in groups
 // of eight 1024 bytes apart: rows of the M or N index with 64 K values
@@ -286,9 +252,9 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   return r;
 }
 
-// The largest, or the sum, over a warp's lanes of each of H values: lane i < H
-// gets that of v[i].
-template <int H, bool SUM> __device__ __forceinline__ float across(uint32_t (&v)[H]) {
+// The largest, or the sum, over a warp's lanes of each of 16 values: lanes i and
+// i + 16 get that of v[i].
+template <bool SUM> __device__ __forceinline__ float across(uint32_t (&v)[H]) {
   const uint32_t lane = threadIdx.x & 31;
   auto join = [](float x, float y) { return SUM ? x + y : fmaxf(x, y); };
 #pragma unroll
@@ -301,15 +267,8 @@ template <int H, bool SUM> __device__ __forceinline__ float across(uint32_t (&v)
                                   __uint_as_float(__shfl_xor_sync(0xffffffffu, give, o))));
     }
   }
-  float r = __uint_as_float(v[0]);
-  if (H == 16) r = join(r, __shfl_xor_sync(0xffffffffu, r, 16));
-  return r;
-}
-template <int H> __device__ __forceinline__ float tops(uint32_t (&v)[H]) {
-  return across<H, false>(v);
-}
-template <int H> __device__ __forceinline__ float sums(uint32_t (&v)[H]) {
-  return across<H, true>(v);
+  const float r = __uint_as_float(v[0]);
+  return join(r, __shfl_xor_sync(0xffffffffu, r, 16));
 }
 
 // The walk over the parts of items that a CTA has, the same in every role.
@@ -351,11 +310,10 @@ struct Walk {
 };
 
 template <int HD, int BITS, int N>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Plan<HD, BITS, N>::Threads, 1)
 tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, uint32_t box, int *err) {
   using L = Plan<HD, BITS, N>;
-  constexpr int H = N / 2;                   // rows of a group of score warps
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                             ~(uintptr_t)1023);
@@ -369,12 +327,15 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
   float *warp_part = reinterpret_cast<float *>(sm + L::Warp);
   float *warp_base = reinterpret_cast<float *>(sm + L::Base);
   const uint32_t bars = s0 + L::Bars;
-  const uint32_t full = bars, empty = bars + 24, kready = bars + 48, qkdone = bars + 64,
-                 sfree = bars + 80, vready = bars + 96, pready = bars + 112, pvdone = bars + 128,
-                 qready = bars + 144;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + L::Bars + 160);
+  const uint32_t full = bars, empty = bars + 24, kready = bars + 48, qkdone = bars + 80,
+                 sfree = bars + 96, vready = bars + 112, pready = bars + 128, pvdone = bars + 144,
+                 qready = bars + 160;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + L::Bars + 176);
   uint32_t *votes = tmem_slot + 1;           // the largest scale of a group's tile
+  uint4 *words = reinterpret_cast<uint4 *>(sm + L::Words);
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // 0: the score groups; then keys, values, control
+  const uint32_t role = warp < 4 * L::Groups ? 0 : warp / 4 - L::Groups + 1;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::Stages; i++) {
@@ -382,17 +343,19 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
       bar_init(empty + 8 * i, 8);
     }
     for (int i = 0; i < 2; i++) {
-      bar_init(kready + 8 * i, 4);
       bar_init(qkdone + 8 * i, 1);
-      bar_init(sfree + 8 * i, 8);
+      bar_init(sfree + 8 * i, 4 * L::Groups);
       bar_init(vready + 8 * i, 4);
-      bar_init(pready + 8 * i, 8);
+      bar_init(pready + 8 * i, 4 * L::Groups);
       bar_init(pvdone + 8 * i, 1);
     }
-    bar_init(qready, 8);
+    // four: a score warp may come to wait for a tile's keys when those two
+    // tiles on are ready too, and a phase must not be taken for the next
+    for (int i = 0; i < 4; i++) bar_init(kready + 8 * i, 4);
+    bar_init(qready, 4 * L::Groups);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 17) {
+  if (role == 3 && warp % 4 == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
                      su32(tmem_slot)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
@@ -408,9 +371,9 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
   Walk w;
   if (w.begin(a)) {
     uint32_t it = 0;                         // tiles so far, over all items
-    if (warp >= 16) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
-      if (warp == 16) {
+    if (role == 3) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
+      if (warp % 4 == 0) {
         // ---- TMA of the codes: a run of BOX keys of a page at a time, one lane each ----
         const uint32_t runs = kTileKeys / box;
         while (w.next(a)) {
@@ -441,7 +404,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         alive = true;
         for (uint32_t i = it > (uint32_t)L::Stages ? it - L::Stages : 0; i < it; i++)
           bar_wait(full + 8 * (i % L::Stages), i / L::Stages & 1, alive, err);
-      } else if (warp == 17) {
+      } else if (warp % 4 == 1) {
         // ---- the score products ----
         const uint32_t me = elect();
         uint32_t item = 0;
@@ -450,7 +413,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           item++;
           for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
             const uint32_t st = it & 1, ph = it >> 1 & 1;
-            bar_wait(kready + 8 * st, ph, alive, err);
+            bar_wait(kready + 8 * (it & 3), it >> 2 & 1, alive, err);
             bar_wait(sfree + 8 * st, ph ^ 1, alive, err);
             fence_after();
             const uint64_t q = smem_desc(s0 + L::Q, 16);
@@ -462,7 +425,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             mma_commit(me, qkdone + 8 * st);
           }
         }
-      } else if (warp == 18) {
+      } else if (warp % 4 == 2) {
         // ---- the output products ----
         const uint32_t me = elect();
         while (w.next(a)) {
@@ -483,19 +446,34 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           }
         }
       }
-    } else if (warp >= 8) {
+    } else if (role) {
       // byte of chunk c of a key's row, swizzled by the copy over the row's bytes
       const uint32_t quad = (warp & 3) * 32, key = quad + lane;
       const uint32_t x = L::RB == 128 ? key & 7 : L::RB == 64 ? key >> 1 & 3 : key >> 2 & 1;
       const uint32_t from = key * L::RB + (x << 4);
-      if (warp < 12) {
+      if (role == 1) {
         // ---- keys, to TMEM.  (Codes left 1024 too large, with that much of the
         // query's sum taken off the scores, would halve the work here, but the
         // cut sums of the tensor core then cost the scores 5 bits.) ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
         while (w.next(a)) {
+          const uint32_t keys = keys_of(a, w.b);
           for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
             const uint32_t st = it % L::Stages, h = it & 1;
+            // the parameter words of this thread's key, and whether there is one
+            uint4 word = make_uint4(0, 0, 0, 0);
+            const uint32_t token = tile * kTileKeys + key;
+            if (token < keys) {
+              const uint32_t page =
+                  a.block_shift < 32 ? token >> a.block_shift : token / a.pool.block_size;
+              const uint32_t block = (uint32_t)__ldg(a.table + (uint64_t)w.b * a.max_blocks + page);
+              if (block < a.pool.num_blocks) {
+                const uint32_t row = kv_row(a.pool, block, token - page * a.pool.block_size, w.head);
+                word.x = __ldg(a.pool.param[0] + row);
+                word.y = __ldg(a.pool.param[1] + row);
+                word.z = 1;
+              }
+            }
             const uint8_t *kc = sm + st * (2 * L::Codes);
             bar_wait(full + 8 * st, it / L::Stages & 1, alive, err);
             bar_wait(qkdone + 8 * h, (it >> 1 & 1) ^ 1, alive, err);
@@ -514,11 +492,14 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
               }
               tmem_st16(tmem + (quad << 16) + L::TK + h * L::KCols + c0 / Each * 16, v);
             }
+            // four tiles of them: the product just waited for was issued after every
+            // score warp was past the tile before its stage's last
+            words[(it & 3) * kTileKeys + key] = word;
             tmem_wait_st();
             fence_before();
             __syncwarp();
             if (lane == 0) {
-              bar_arrive(kready + 8 * h);
+              bar_arrive(kready + 8 * (it & 3));
               bar_arrive(empty + 8 * st);
             }
           }
@@ -526,7 +507,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
       } else {
         // ---- values: the signed codes, to shared memory; eight lanes' rows are
         // swizzled apart, so neither reads nor writes share a bank ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
         const uint32_t row = key * 128 + ((key & 7) << 4);
         while (w.next(a)) {
           for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
@@ -566,38 +547,18 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
       }
     } else {
       // ---- scores to weights, a thread per key; half the rows a group ----
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 152;\n");
+      if constexpr (L::RegsSoft >= L::Regs)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(L::RegsSoft));
       const uint32_t group = warp >> 2, quad = (warp & 3) * 32, mykey = quad + lane;
       const uint32_t tid = threadIdx.x;
-      const uint32_t n0 = group * H;
+      const uint32_t n0 = group * H;         // its first row
       uint32_t *vote = votes + group;
       const uint64_t used = a.nodes < 64 ? (1ull << a.nodes) - 1 : ~0ull;
       while (w.next(a)) {
-        const uint32_t prefix = prefix_of(a, w.b), keys = keys_of(a, w.b);
-        // the parameter words of this thread's key of a tile, found a tile ahead
-        auto page_of = [&](uint32_t key) {
-          return a.block_shift < 32 ? key >> a.block_shift : key / a.pool.block_size;
-        };
-        auto block_of = [&](uint32_t tile) {
-          const uint32_t key = tile * kTileKeys + mykey;
-          if (tile >= w.t1 || key >= keys) return kNone;
-          return (uint32_t)__ldg(a.table + (uint64_t)w.b * a.max_blocks + page_of(key));
-        };
-        auto words_of = [&](uint32_t tile, uint32_t block, uint32_t *kw, uint32_t *vw) {
-          *kw = *vw = 0;
-          if (block >= a.pool.num_blocks) return false;
-          const uint32_t key = tile * kTileKeys + mykey;
-          const uint32_t row =
-              kv_row(a.pool, block, key - page_of(key) * a.pool.block_size, w.head);
-          *kw = __ldg(a.pool.param[0] + row);
-          *vw = __ldg(a.pool.param[1] + row);
-          return true;
-        };
-        uint32_t block1 = block_of(w.t0), kw1, vw1;
-
+        const uint32_t prefix = prefix_of(a, w.b);
         // the queries of the item, float16, K-major
         {
-          constexpr int Per = N * HD / kSoft, Lanes = HD / Per;      // values a thread takes
+          constexpr int Per = N * HD / L::Soft, Lanes = HD / Per;      // values a thread takes
           const uint32_t n = tid / Lanes, part = tid % Lanes, row = w.row0 + n;
           const bool live = row < a.rows;
           const uint32_t node = live ? row / a.group : 0;
@@ -650,7 +611,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           }
         }
         fence_async();
-        soft_sync();
+        soft_sync<L::Soft>();
         if (lane == 0) bar_arrive(qready);
 
         constexpr int NB = BITS == 4 ? H / 2 : 1;
@@ -659,15 +620,13 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         for (int i = 0; i < H / 2; i++) l[i] = base[i % NB] = 0;
         float vs = 1.0f;
         uint32_t vlimit = 0;
-        bool have1 = words_of(w.t0, block1, &kw1, &vw1);
-        block1 = block_of(w.t0 + 1);
 
         for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
           const uint32_t st = it & 1, ph = it >> 1 & 1;
-          const bool have = have1;
-          const uint32_t kw = kw1, vw = vw1;
-          have1 = words_of(tile + 1, block1, &kw1, &vw1);
-          block1 = block_of(tile + 2);
+          bar_wait(kready + 8 * (it & 3), it >> 2 & 1, alive, err);
+          const uint4 word = words[(it & 3) * kTileKeys + mykey];
+          const uint32_t kw = word.x, vw = word.y;
+          const bool have = word.z != 0;
           const float sk = scale_of<BITS>(kw);
           const float mk = middle_of(kw);
           const Pair sk2 = pair(sk, sk), mk2 = pair(mk, mk);
@@ -715,7 +674,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           const uint32_t ts = tmem + (quad << 16) + L::TS + st * N + n0;
           uint32_t s[H];
           for (bool again = false;; again = true) {
-            tmem_ld<H>(ts, s);
+            tmem_ld16(ts, s);
             score(s, true);
             float top = -INFINITY;
 #pragma unroll
@@ -723,9 +682,9 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             const bool over = top > 8.0f || (vbits >= vlimit && vbits != 0);
             if (again || !group_any(group, over)) break;
             // ---- new references: the maxima of the keys so far ----
-            tmem_ld<H>(ts, s);
+            tmem_ld16(ts, s);
             score(s, false);
-            const float mine = tops<H>(s);
+            const float mine = across<false>(s);
             if (lane < H) warp_part[(warp & 3) * N + n0 + lane] = mine;
             if (quad == 0 && lane == 0) *vote = 0;
             group_sync(group);
@@ -759,11 +718,11 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
               bar_wait(pvdone + 8 * (st ^ 1), (it - 1) >> 1 & 1, alive, err);
               fence_after();
               const uint32_t to = tmem + (quad << 16) + L::TO + n0;
-              tmem_ld<H>(to, s);
+              tmem_ld16(to, s);
 #pragma unroll
               for (int i = 0; i < H; i++)
                 s[i] = __float_as_uint(__uint_as_float(s[i]) * (keep[n0 + i] * ratio));
-              tmem_st<H>(to, s);
+              tmem_st16(to, s);
               tmem_wait_st();
             }
           }
@@ -815,7 +774,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             v[2 * i] = __float_as_uint(y.x);
             v[2 * i + 1] = __float_as_uint(y.y);
           }
-          const float sum = sums<H>(v);
+          const float sum = across<true>(v);
           if (lane < H) warp_part[(warp & 3) * N + n0 + lane] = sum;
           if (BITS == 4) {
 #pragma unroll
@@ -824,7 +783,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
               v[2 * i] = __float_as_uint(y.x);
               v[2 * i + 1] = __float_as_uint(y.y);
             }
-            const float mid = sums<H>(v);
+            const float mid = across<true>(v);
             if (lane < H) warp_base[(warp & 3) * N + n0 + lane] = mid;
           }
         }
@@ -854,7 +813,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         const uint32_t d = natural<BITS>(mykey);       // the value this TMEM lane holds
         {
           uint32_t o[H];
-          tmem_ld<H>(tmem + (quad << 16) + L::TO + n0, o);
+          tmem_ld16(tmem + (quad << 16) + L::TO + n0, o);
           if (HD == 128 || quad < 64) {
             float *part = a.part_o + ((uint64_t)slot * N + n0) * HD + d;
 #pragma unroll
@@ -868,13 +827,13 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           }
         }
         fence_before();
-        soft_sync();                         // the rows are read: the next item may write them
+        soft_sync<L::Soft>();                         // the rows are read: the next item may write them
       }
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == 17) {
+  if (role == 3 && warp % 4 == 1) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
   }
@@ -936,7 +895,7 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
   int *err = wait_flag_device();
   if (!err) return cudaErrorMemoryAllocation;
   count_launches(1);
-  return launch_pdl(tree_umma_kernel<HD, BITS, N>, dim3(a.ctas), dim3(kThreads), (size_t)L::Bytes,
+  return launch_pdl(tree_umma_kernel<HD, BITS, N>, dim3(a.ctas), dim3(L::Threads), (size_t)L::Bytes,
                     st, a, map[0], map[1], box, err);
 }
 
