@@ -594,8 +594,10 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   }
 }
 
-// Joins the partial states of the items that several CTAs share: a block per
-// output row.
+// Joins the partial states of the items that several CTAs share.  The shares'
+// boundaries are the only places where an item can be cut: block (c, y) joins
+// four rows of the item that boundary c + 1 cuts, if it is the first to cut it.
+// A warp takes a row while the parts are few, the block a row at a time else.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTreeThreads)
 tree_join_kernel(const __grid_constant__ TreeArgs a) {
@@ -603,61 +605,102 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
   pdl_wait();
   __shared__ float red[kTreeWarps][HD + 2];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t h = blockIdx.x % a.heads, bn = blockIdx.x / a.heads;
-  const uint32_t b = bn / a.nodes, row = bn % a.nodes * a.group + h % a.group;
   const uint64_t total = all_cost(a);
-  const uint32_t workers = total < a.ctas ? (uint32_t)total : a.ctas;
-  uint64_t before = 0;
-  {
-    for (uint32_t i = lane; i < b; i += 32) before += tiles_of(a, i) + a.item_cost;
-    before = warp_sum(before) * ((uint64_t)a.pool.kv_heads * a.row_tiles);
-  }
-  const uint32_t tiles = tiles_of(a, b);
-  const uint64_t s0 = before + a.item_cost +
-                      (uint64_t)(h / a.group * a.row_tiles + row / a.rows_at_once) *
-                          (tiles + a.item_cost);
-  const uint32_t c0 = owner(total, workers, s0), c1 = owner(total, workers, s0 + tiles - 1);
-  if (c0 == c1) return;
+  const uint32_t workers = total < a.ctas ? (uint32_t)total : a.ctas, cut = blockIdx.x + 1;
+  if (cut >= workers) return;
+  const uint64_t at = share(total, workers, cut);
+  uint32_t b;
+  uint64_t before;
+  locate(a, at, &b, &before);
+  const uint32_t tiles = tiles_of(a, b), cost = tiles + a.item_cost;
+  const uint32_t off = (uint32_t)((at - before) % cost), item = (uint32_t)((at - before) / cost);
+  const uint64_t s0 = at - off + a.item_cost;     // the item's first tile
+  if (off <= a.item_cost || share(total, workers, cut - 1) > s0) return;
+  const uint32_t c0 = cut - 1, c1 = owner(total, workers, s0 + tiles - 1);
+  const uint32_t head = item / a.row_tiles, row0 = item % a.row_tiles * a.rows_at_once;
   constexpr int Per = HD / 32;
-  float v[Per], m = -INFINITY, l = 0.0f;
+  const bool alone = c1 - c0 < 32;                // a warp per row
+  for (uint32_t r = alone ? warp : 0; r < 4; r += alone ? 4 : 1) {
+    const uint32_t here = blockIdx.y * 4 + r, row = row0 + here;
+    if (row >= a.rows) break;                      // of the warp, or of the block
+    float v[Per], m = -INFINITY, l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < Per; i++) v[i] = 0.0f;
-  for (uint32_t c = c0 + warp; c <= c1; c += kTreeWarps) {
-    const uint64_t at =
-        (uint64_t)(2 * c + (c == c0 ? 1 : 0)) * a.rows_at_once + row % a.rows_at_once;
-    const float pm = a.part_ml[2 * at], pl = a.part_ml[2 * at + 1];
-    if (pm == -INFINITY && pl == 0.0f) continue;
-    const float top = fmaxf(m, pm);
-    const float old = m == top ? 1.0f : ex2(m - top), add = pm == top ? 1.0f : ex2(pm - top);
-    m = top;
-    l = fmaf(l, old, pl * add);
+    for (int i = 0; i < Per; i++) v[i] = 0.0f;
+    // 32 parts at a time: a lane finds the weight of one
+    const uint32_t step = alone ? 1 : kTreeWarps;
+    for (uint32_t c = c0 + (alone ? 0 : warp); c <= c1; c += 32 * step) {
+      const uint32_t mine = c + lane * step;
+      float pm = -INFINITY, pl = 0.0f;
+      if (mine <= c1) {
+        const uint64_t from = (uint64_t)(2 * mine + (mine == c0 ? 1 : 0)) * a.rows_at_once + here;
+        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * from);
+        pm = ml.x;
+        pl = ml.y;
+      }
+      float top = fmaxf(m, pm);
 #pragma unroll
-    for (int i = 0; i < Per; i++) v[i] = fmaf(v[i], old, a.part_o[at * HD + i * 32 + lane] * add);
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // a part without keys weighs nothing; one of NaN may have left no maximum
+      const float by = pm == -INFINITY && pl == 0.0f ? 0.0f : pm == top ? 1.0f : ex2(pm - top);
+      const float old = m == top ? 1.0f : ex2(m - top);
+      float sum = by == 0.0f && pl == pl ? 0.0f : pl * by;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l = fmaf(l, old, sum);
+      m = top;
+#pragma unroll
+      for (int i = 0; i < Per; i++) v[i] *= old;
+      const uint32_t n = min(32u, (c1 - c) / step + 1);
+#pragma unroll 4
+      for (uint32_t p = 0; p < n; p++) {
+        const uint32_t part = c + p * step;
+        const float w = __shfl_sync(0xffffffffu, by, p);
+        const float *from = a.part_o + ((uint64_t)(2 * part + (part == c0 ? 1 : 0)) *
+                                            a.rows_at_once + here) * HD + lane;
+#pragma unroll
+        for (int i = 0; i < Per; i++) {
+          const float x = from[i * 32];
+          v[i] = w == 0.0f ? v[i] : fmaf(x, w, v[i]);
+        }
+      }
+    }
+    if (!alone) {
+      __syncthreads();                             // the last row's states are read
+#pragma unroll
+      for (int i = 0; i < Per; i++) red[warp][i * 32 + lane] = v[i];
+      if (lane == 0) red[warp][HD] = m, red[warp][HD + 1] = l;
+      __syncthreads();
+      float c[kTreeWarps];
+      m = -INFINITY;
+      l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kTreeWarps; w++) m = fmaxf(m, red[w][HD]);
+#pragma unroll
+      for (int w = 0; w < kTreeWarps; w++) {
+        c[w] = red[w][HD] == m ? 1.0f : ex2(red[w][HD] - m);
+        l = fmaf(c[w], red[w][HD + 1], l);
+      }
+#pragma unroll
+      for (int i = 0; i < Per; i++) {
+        v[i] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kTreeWarps; w++) v[i] = fmaf(c[w], red[w][i * 32 + lane], v[i]);
+      }
+    }
+    const uint64_t bn = (uint64_t)b * a.nodes + row / a.group;
+    const uint32_t h = head * a.group + row % a.group;
+    const uint64_t words = a.mask[bn] & (a.nodes < 64 ? (1ull << a.nodes) - 1 : ~0ull);
+    const bool empty = words == 0 || l == 0.0f;
+    const float inv = 1.0f / l;
+    if (alone || warp == 0) {
+#pragma unroll
+      for (int i = 0; i < Per; i++)
+        store1((T *)a.o + bn * a.o_stride + (uint64_t)h * HD + i * 32 + lane,
+               empty ? 0.0f : v[i] * inv);
+      if (lane == 0 && a.lse)
+        a.lse[bn * a.heads + h] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < Per; i++) red[warp][i * 32 + lane] = v[i];
-  if (lane == 0) red[warp][HD] = m, red[warp][HD + 1] = l;
-  __syncthreads();
-  float top = -INFINITY, sum = 0.0f, c[kTreeWarps];
-#pragma unroll
-  for (int w = 0; w < kTreeWarps; w++) top = fmaxf(top, red[w][HD]);
-#pragma unroll
-  for (int w = 0; w < kTreeWarps; w++) {
-    c[w] = red[w][HD] == top ? 1.0f : ex2(red[w][HD] - top);
-    sum = fmaf(c[w], red[w][HD + 1], sum);
-  }
-  const uint64_t words = a.mask[bn] & (a.nodes < 64 ? (1ull << a.nodes) - 1 : ~0ull);
-  const bool empty = words == 0 || sum == 0.0f;
-  const float inv = 1.0f / sum;
-  for (uint32_t d = threadIdx.x; d < HD; d += kTreeThreads) {
-    float y = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kTreeWarps; w++) y = fmaf(c[w], red[w][d], y);
-    store1((T *)a.o + (uint64_t)bn * a.o_stride + (uint64_t)h * HD + d, empty ? 0.0f : y * inv);
-  }
-  if (threadIdx.x == 0 && a.lse)
-    a.lse[(uint64_t)bn * a.heads + h] =
-        empty ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 template <typename T, int HD, int BITS, int NR, int WR>
@@ -704,7 +747,7 @@ cudaError_t tree_attn_start(TreeArgs &a, bool bf16, cudaStream_t st) {
 
 template <int HD>
 cudaError_t tree_join_start(TreeArgs &a, bool bf16, cudaStream_t st) {
-  const dim3 grid(a.batch * a.nodes * a.heads), block(kTreeThreads);
+  const dim3 grid(a.ctas, (a.rows_at_once + 3) / 4), block(kTreeThreads);
   count_launches(1);
   return bf16 ? launch_pdl(tree_join_kernel<__nv_bfloat16, HD>, grid, block, 0, st, a)
               : launch_pdl(tree_join_kernel<float, HD>, grid, block, 0, st, a);
