@@ -11,18 +11,23 @@ import ctypes
 from . import _lib as L
 
 
-_ready = False
+_ready = None
+_device = 0
+_raw_stream = None
 
 
 def _lib():
     """The library, with its context on the current torch device."""
-    global _ready
-    lib = L.load()
-    if not _ready:
+    global _ready, _device, _raw_stream
+    if _ready is None:
         import torch
+        lib = L.load()
         L.check(lib.nl_init(torch.cuda.current_device()))
-        _ready = True
-    return lib
+        _device = lib.nl_device()
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _ready = lib
+    return _ready
 
 
 def _p(t):
@@ -35,8 +40,9 @@ def _stream(stream=None):
     than the rest of a call)."""
     if stream is not None:
         return stream.cuda_stream
-    import torch
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    if _raw_stream is None:
+        _lib()
+    return _raw_stream(_device)
 
 
 def _check_tensor(t, dtype_name):
@@ -98,26 +104,21 @@ def decode_attn_rope(QKV, CK, CV, POS, C, batch, heads, kv_heads, head_dim, max_
 
 
 # ---- speculative serving: Q/K norm + RoPE, quantised KV cache, tree attention ----
+# These are called once a layer a token: their checks are written for the time
+# they take.
 
-_ROWS = {"torch.float32": 0, "torch.bfloat16": 1}     # NL_F32, NL_BF16
-_PAIRS = {"half": 0, "adjacent": 1}
-
-
-def _rows(t, name, dtype=None):
-    """The row stride of a 2-D CUDA tensor of rows (f32 or bf16)."""
-    stride = t.stride()
-    if not t.is_cuda or len(stride) != 2 or (stride[1] != 1 and t.shape[1] > 1) or \
-            (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{name}: expected CUDA rows (2-D, unit inner stride"
-                         + (f", {dtype})" if dtype is not None else ")"))
-    return stride[0]
+_PAIRS = {"half": 0, "adjacent": 1}      # NL_PAIRS_HALF, NL_PAIRS_ADJACENT
+_types = None
 
 
-def _row_type(t):
-    code = _ROWS.get(str(t.dtype))
-    if code is None:
-        raise ValueError(f"expected f32 or bf16 rows, not {t.dtype}")
-    return code
+def _torch_types():
+    """(f32, bf16, int32, int64, uint8, {row type: NL_F32 / NL_BF16})."""
+    global _types
+    if _types is None:
+        import torch
+        _types = (torch.float32, torch.bfloat16, torch.int32, torch.int64, torch.uint8,
+                  {torch.float32: 0, torch.bfloat16: 1})
+    return _types
 
 
 def _need(cond, msg):
@@ -125,12 +126,41 @@ def _need(cond, msg):
         raise ValueError(msg)
 
 
+def _flat(dtype, *tensors):
+    """Whether all are contiguous CUDA tensors of DTYPE."""
+    for t in tensors:
+        if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
+            raise ValueError(f"expected a contiguous CUDA {dtype} tensor, not {t.dtype} "
+                             f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def _rows(dtype, *tensors):
+    """Whether all are 2-D CUDA rows of DTYPE with unit inner stride; the
+    tensors' row strides."""
+    strides = []
+    for t in tensors:
+        stride = t.stride()
+        if t.dtype is not dtype or not t.is_cuda or len(stride) != 2 or \
+                (stride[1] != 1 and t.shape[1] > 1):
+            raise ValueError(f"expected CUDA rows of {dtype} (2-D, unit inner stride), not "
+                             f"{t.dtype} {tuple(t.shape)} with strides {stride} on {t.device}")
+        strides.append(stride[0])
+    return strides
+
+
+def _row_type(t):
+    code = _torch_types()[5].get(t.dtype)
+    if code is None:
+        raise ValueError(f"expected f32 or bf16 rows, not {t.dtype}")
+    return code
+
+
 def _workspace(nbytes, workspace, device, stream):
     """WORKSPACE as given, or one of the caching allocator that belongs to the
     call's stream, so that calls on different streams never share one."""
-    import torch
     if workspace is not None:
         return workspace, workspace.numel() * workspace.element_size()
+    import torch
     if stream is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
     with torch.cuda.stream(stream):
@@ -138,20 +168,19 @@ def _workspace(nbytes, workspace, device, stream):
 
 
 def _qk_shapes(QKV, GQ, GK, CO, SI, POS, Q, K, pairs):
-    for t in (GQ, GK, CO, SI):
-        _check_tensor(t, "torch.float32")
-    _check_tensor(POS, "torch.int32")
-    hd, n = GQ.numel(), QKV.shape[0]
-    _need(hd > 0 and GK.numel() == hd, f"gains of {hd} and {GK.numel()} values")
-    _need(CO.dim() == 2 and CO.shape == SI.shape, "CO and SI: two tables of one 2-D shape")
-    _need(POS.numel() == n and Q.shape[0] == n and K.shape[0] == n,
-          f"{n} rows of QKV, {POS.numel()} positions, {Q.shape[0]} and {K.shape[0]} rows")
-    _need(Q.shape[1] % hd == 0 and K.shape[1] % hd == 0 and
-          Q.shape[1] + K.shape[1] <= QKV.shape[1],
-          f"rows of {QKV.shape[1]} values do not hold heads of {hd}: {Q.shape[1]} + {K.shape[1]}")
-    _need(pairs in _PAIRS, f"pairs {pairs!r}: 'half' or 'adjacent'")
-    return (n, Q.shape[1] // hd, K.shape[1] // hd, hd, 2 * CO.shape[1], CO.shape[0],
-            _PAIRS[pairs])
+    types = _torch_types()
+    _flat(types[0], GQ, GK, CO, SI)
+    _flat(types[2], POS)
+    (n, width), (nq, wq), (nk, wk) = QKV.shape, Q.shape, K.shape
+    hd, table = GQ.numel(), CO.shape
+    _need(hd > 0 and GK.numel() == hd, "gains of different or no length")
+    _need(len(table) == 2 and table == SI.shape, "CO and SI: two tables of one 2-D shape")
+    if POS.numel() != n or nq != n or nk != n:
+        raise ValueError(f"{n} rows of QKV, {POS.numel()} positions, {nq} and {nk} rows")
+    if wq % hd or wk % hd or wq + wk > width:
+        raise ValueError(f"rows of {width} values do not hold heads of {hd}: {wq} + {wk}")
+    _need(pairs in _PAIRS, "pairs: 'half' or 'adjacent'")
+    return n, wq // hd, wk // hd, hd, 2 * table[1], table[0], _PAIRS[pairs]
 
 
 def qk_norm_rope(QKV, GQ, GK, CO, SI, POS, Q, K, eps=1e-5, pairs="half", stream=None):
@@ -160,40 +189,45 @@ def qk_norm_rope(QKV, GQ, GK, CO, SI, POS, Q, K, eps=1e-5, pairs="half", stream=
     the rotation of its first 2 * CO.shape[1] values at row POS[i] (int32) of
     the tables CO, SI.  Rows whose position is outside the tables are zeros.
     f32 or bf16; rows may be strided, and Q and K views of QKV itself."""
+    kind = _row_type(QKV)
+    xs, qs, ks = _rows(QKV.dtype, QKV, Q, K)
     dims = _qk_shapes(QKV, GQ, GK, CO, SI, POS, Q, K, pairs)
-    xs = _rows(QKV, "QKV")
-    qs, ks = _rows(Q, "Q", QKV.dtype), _rows(K, "K", QKV.dtype)
-    L.check(_lib().nl_qk_norm_rope_dev(
-        _row_type(QKV), QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(),
-        SI.data_ptr(), POS.data_ptr(), Q.data_ptr(), qs, K.data_ptr(), ks, *dims, eps,
-        _stream(stream)))
+    rc = _lib().nl_qk_norm_rope_dev(
+        kind, QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(), SI.data_ptr(),
+        POS.data_ptr(), Q.data_ptr(), qs, K.data_ptr(), ks, *dims, eps, _stream(stream))
+    if rc:
+        L.check(rc)
 
 
 def qk_norm_rope_bwd(QKV, GQ, GK, CO, SI, POS, DQ, DK, DQKV, DGQ, DGK, eps=1e-5, pairs="half",
                      workspace=None, stream=None):
     """The backward pass of qk_norm_rope: the q and k part of DQKV and the
     gains' gradients DGQ, DGK (f32 [hd]) from the gradients DQ, DK."""
+    kind = _row_type(QKV)
+    xs, qs, ks, dxs = _rows(QKV.dtype, QKV, DQ, DK, DQKV)
     dims = _qk_shapes(QKV, GQ, GK, CO, SI, POS, DQ, DK, pairs)
-    _check_tensor(DGQ, "torch.float32"); _check_tensor(DGK, "torch.float32")
-    _need(DGQ.numel() == dims[3] and DGK.numel() == dims[3], "DGQ and DGK: one value per gain")
-    _need(DQKV.shape[0] == dims[0] and DQKV.shape[1] >= DQ.shape[1] + DK.shape[1],
-          f"DQKV of {tuple(DQKV.shape)} for {dims[0]} rows")
-    xs, dxs = _rows(QKV, "QKV"), _rows(DQKV, "DQKV", QKV.dtype)
-    qs, ks = _rows(DQ, "DQ", QKV.dtype), _rows(DK, "DK", QKV.dtype)
+    _flat(_torch_types()[0], DGQ, DGK)
+    hd = dims[3]
+    _need(DGQ.numel() == hd and DGK.numel() == hd, "DGQ and DGK: one value per gain")
+    n, width = DQKV.shape
+    if n != dims[0] or width < DQ.shape[1] + DK.shape[1]:
+        raise ValueError(f"DQKV of {n} x {width} for {dims[0]} rows")
     lib = _lib()
-    ws, nbytes = _workspace(lib.nl_qk_norm_rope_bwd_workspace_bytes(dims[3]), workspace,
-                            QKV.device, stream)
-    L.check(lib.nl_qk_norm_rope_bwd_dev(
-        _row_type(QKV), QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(),
-        SI.data_ptr(), POS.data_ptr(), DQ.data_ptr(), qs, DK.data_ptr(), ks, DQKV.data_ptr(), dxs,
-        DGQ.data_ptr(), DGK.data_ptr(), *dims, eps, ws.data_ptr(), nbytes, _stream(stream)))
+    ws, nbytes = _workspace(lib.nl_qk_norm_rope_bwd_workspace_bytes(hd), workspace, QKV.device,
+                            stream)
+    rc = lib.nl_qk_norm_rope_bwd_dev(
+        kind, QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(), SI.data_ptr(),
+        POS.data_ptr(), DQ.data_ptr(), qs, DK.data_ptr(), ks, DQKV.data_ptr(), dxs,
+        DGQ.data_ptr(), DGK.data_ptr(), *dims, eps, ws.data_ptr(), nbytes, _stream(stream))
+    if rc:
+        L.check(rc)
 
 
 def kv_cache(num_blocks, block_size, kv_heads, head_dim, bits, device="cuda"):
     """The four arrays of a quantised paged cache (8 or 4 bits a value), zeroed:
     KC, KP, VC, VP, the codes uint8 and the parameter words int32."""
     import torch
-    _need(bits in (4, 8), f"bits {bits}: 8 or 4")
+    _need(bits in (4, 8), "bits: 8 or 4")
     shape = (num_blocks, kv_heads, block_size)
     KC, VC = (torch.zeros(*shape, head_dim * bits // 8, dtype=torch.uint8, device=device)
               for _ in range(2))
@@ -201,54 +235,66 @@ def kv_cache(num_blocks, block_size, kv_heads, head_dim, bits, device="cuda"):
     return KC, KP, VC, VP
 
 
-def _pool(KC, KP, VC, VP, head_dim=None):
-    """(bits, kv_heads, head_dim, block_size, num_blocks) of a cache."""
+def _pool(KC, KP, VC, VP, head_dim):
+    """(bits, (kv_heads, head_dim, block_size, num_blocks)) of a cache."""
+    types = _torch_types()
+    _flat(types[4], KC, VC)
+    _flat(types[2], KP, VP)
     shape = KC.shape
-    for c, w in ((KC, KP), (VC, VP)):
-        _check_tensor(c, "torch.uint8"); _check_tensor(w, "torch.int32")
-        _need(len(shape) == 4 and c.shape == shape and w.shape == shape[:3],
-              f"cache codes of {tuple(c.shape)} and words of {tuple(w.shape)}")
-    bits = 8 * shape[3] // head_dim if head_dim else 0
-    _need(bits in (4, 8) and bits * head_dim == 8 * shape[3],
-          f"rows of {shape[3]} bytes for heads of {head_dim}")
-    return bits, shape[1], head_dim, shape[2], shape[0]
+    if len(shape) != 4 or VC.shape != shape or KP.shape != shape[:3] or VP.shape != shape[:3]:
+        raise ValueError(f"cache codes of {tuple(shape)} and {tuple(VC.shape)}, words of "
+                         f"{tuple(KP.shape)} and {tuple(VP.shape)}")
+    blocks, kvh, size, row = shape
+    if row == head_dim:
+        bits = 8
+    elif 2 * row == head_dim:
+        bits = 4
+    else:
+        raise ValueError(f"rows of {row} bytes for heads of {head_dim}")
+    return bits, (kvh, head_dim, size, blocks)
 
 
-def _kv_call(name, SLOT, KC, KP, VC, VP, K, V):
-    _need(KC.dim() == 4, f"{name}: cache codes have 4 dimensions")
-    width, kvh = K.shape[1], KC.shape[1]
-    _need(kvh > 0 and width % kvh == 0 and V.shape == K.shape,
-          f"{name}: rows of {width} values and {tuple(V.shape)} for {kvh} key heads")
-    _check_tensor(SLOT, "torch.int32")
-    _need(SLOT.numel() == K.shape[0], f"{name}: {SLOT.numel()} slots for {K.shape[0]} rows")
-    return _pool(KC, KP, VC, VP, width // kvh)
+def _kv_shapes(SLOT, KC, KP, VC, VP, K, V):
+    _flat(_torch_types()[2], SLOT)
+    _need(KC.dim() == 4, "cache codes have 4 dimensions")
+    (n, width), kvh = K.shape, KC.shape[1]
+    if V.shape != K.shape or SLOT.numel() != n or kvh == 0 or width % kvh:
+        raise ValueError(f"rows of {n} x {width} and {tuple(V.shape)}, {SLOT.numel()} slots, "
+                         f"{kvh} key heads")
+    return n, _pool(KC, KP, VC, VP, width // kvh)
 
 
 def kv_append(K, V, SLOT, KC, KP, VC, VP, stream=None):
     """Quantise the rows K and V ([n, kv_heads * hd], f32 or bf16, may be
     strided) into the cache's token slots SLOT (int32 [n]; outside: skipped)."""
-    bits, *dims = _kv_call("kv_append", SLOT, KC, KP, VC, VP, K, V)
-    ks, vs = _rows(K, "K"), _rows(V, "V", K.dtype)
-    L.check(_lib().nl_kv_append_dev(
-        bits, _row_type(K), K.data_ptr(), ks, V.data_ptr(), vs, SLOT.data_ptr(), KC.data_ptr(),
-        KP.data_ptr(), VC.data_ptr(), VP.data_ptr(), K.shape[0], *dims, _stream(stream)))
+    kind = _row_type(K)
+    ks, vs = _rows(K.dtype, K, V)
+    n, (bits, dims) = _kv_shapes(SLOT, KC, KP, VC, VP, K, V)
+    rc = _lib().nl_kv_append_dev(
+        bits, kind, K.data_ptr(), ks, V.data_ptr(), vs, SLOT.data_ptr(), KC.data_ptr(),
+        KP.data_ptr(), VC.data_ptr(), VP.data_ptr(), n, *dims, _stream(stream))
+    if rc:
+        L.check(rc)
 
 
 def kv_read(SLOT, KC, KP, VC, VP, K, V, stream=None):
     """The values of the slots SLOT into the rows K and V (outside: zeros)."""
-    bits, *dims = _kv_call("kv_read", SLOT, KC, KP, VC, VP, K, V)
-    ks, vs = _rows(K, "K"), _rows(V, "V", K.dtype)
-    L.check(_lib().nl_kv_read_dev(
-        bits, _row_type(K), SLOT.data_ptr(), KC.data_ptr(), KP.data_ptr(), VC.data_ptr(),
-        VP.data_ptr(), K.data_ptr(), ks, V.data_ptr(), vs, K.shape[0], *dims, _stream(stream)))
+    kind = _row_type(K)
+    ks, vs = _rows(K.dtype, K, V)
+    n, (bits, dims) = _kv_shapes(SLOT, KC, KP, VC, VP, K, V)
+    rc = _lib().nl_kv_read_dev(
+        bits, kind, SLOT.data_ptr(), KC.data_ptr(), KP.data_ptr(), VC.data_ptr(), VP.data_ptr(),
+        K.data_ptr(), ks, V.data_ptr(), vs, n, *dims, _stream(stream))
+    if rc:
+        L.check(rc)
 
 
 def kv_move(SRC, DST, KC, KP, VC, VP, head_dim, stream=None):
     """Move tokens between slots without requantising them: SRC, DST int32
     [batch, count]; per sequence every source is read before any write."""
-    _check_tensor(SRC, "torch.int32"); _check_tensor(DST, "torch.int32")
+    _flat(_torch_types()[2], SRC, DST)
     _need(SRC.dim() == 2 and SRC.shape == DST.shape, "SRC and DST: [batch, count] each")
-    bits, *dims = _pool(KC, KP, VC, VP, head_dim)
+    bits, dims = _pool(KC, KP, VC, VP, head_dim)
     L.check(_lib().nl_kv_move_dev(
         bits, SRC.data_ptr(), DST.data_ptr(), KC.data_ptr(), KP.data_ptr(), VC.data_ptr(),
         VP.data_ptr(), SRC.shape[0], SRC.shape[1], *dims, _stream(stream)))
@@ -263,29 +309,37 @@ def tree_attn(Q, KC, KP, VC, VP, TABLE, LEN, MASK, O, head_dim, scale=None, lse=
     attends to node j (token LEN + j), 0 for an unused node.  SCALE is
     1/sqrt(head_dim) unless given; LSE (f32 [batch * nodes, heads]) receives
     the log of the softmax sums."""
-    _check_tensor(TABLE, "torch.int32"); _check_tensor(LEN, "torch.int32")
-    _check_tensor(MASK, "torch.int64"); _check_tensor(lse, "torch.float32")
-    _need(MASK.dim() == 2 and TABLE.dim() == 2, "MASK and TABLE have 2 dimensions")
-    batch, nodes = MASK.shape
-    bits, kvh, hd, block_size, num_blocks = _pool(KC, KP, VC, VP, head_dim)
-    qs, os_ = _rows(Q, "Q"), _rows(O, "O", Q.dtype)
-    rows, width = Q.shape
-    _need(LEN.numel() == batch and TABLE.shape[0] == batch and rows == batch * nodes and
-          O.shape == Q.shape,
-          f"tree_attn: {rows} rows, {batch} sequences of {nodes} nodes, {LEN.numel()} lengths, "
-          f"a table of {tuple(TABLE.shape)}, outputs of {tuple(O.shape)}")
-    heads = width // hd
-    _need(width == heads * hd and (lse is None or lse.shape == (rows, heads)),
-          f"tree_attn: rows of {width} values, heads of {hd}")
+    types = _torch_types()
+    kind = _row_type(Q)
+    qs, os_ = _rows(Q.dtype, Q, O)
+    _flat(types[2], TABLE, LEN)
+    _flat(types[3], MASK)
+    bits, dims = _pool(KC, KP, VC, VP, head_dim)
+    table, mask, shape = TABLE.shape, MASK.shape, Q.shape
+    _need(len(mask) == 2 and len(table) == 2, "MASK and TABLE have 2 dimensions")
+    batch, nodes = mask
+    rows, width = shape
+    heads = width // head_dim
+    if LEN.numel() != batch or table[0] != batch or rows != batch * nodes or O.shape != shape or \
+            width != heads * head_dim:
+        raise ValueError(f"tree_attn: {rows} rows of {width}, heads of {head_dim}, {batch} "
+                         f"sequences of {nodes} nodes, {LEN.numel()} lengths, a table of "
+                         f"{tuple(table)}, outputs of {tuple(O.shape)}")
+    out_lse = None
+    if lse is not None:
+        _flat(types[0], lse)
+        _need(lse.shape == (rows, heads), "lse: a value per row and head")
+        out_lse = lse.data_ptr()
     lib = _lib()
-    ws, nbytes = _workspace(lib.nl_tree_attn_workspace_bytes(nodes, heads, kvh, hd), workspace,
-                            Q.device, stream)
-    L.check(lib.nl_tree_attn_dev(
-        bits, _row_type(Q), Q.data_ptr(), qs, KC.data_ptr(), KP.data_ptr(), VC.data_ptr(),
-        VP.data_ptr(), TABLE.data_ptr(), LEN.data_ptr(), MASK.data_ptr(), O.data_ptr(), os_,
-        lse.data_ptr() if lse is not None else None, batch, nodes, heads, kvh, hd, block_size,
-        num_blocks, TABLE.shape[1], scale if scale is not None else hd ** -0.5, ws.data_ptr(),
-        nbytes, _stream(stream)))
+    ws, nbytes = _workspace(lib.nl_tree_attn_workspace_bytes(nodes, heads, dims[0], head_dim),
+                            workspace, Q.device, stream)
+    rc = lib.nl_tree_attn_dev(
+        bits, kind, Q.data_ptr(), qs, KC.data_ptr(), KP.data_ptr(), VC.data_ptr(), VP.data_ptr(),
+        TABLE.data_ptr(), LEN.data_ptr(), MASK.data_ptr(), O.data_ptr(), os_, out_lse, batch,
+        nodes, heads, *dims, table[1], scale if scale is not None else head_dim ** -0.5,
+        ws.data_ptr(), nbytes, _stream(stream))
+    if rc:
+        L.check(rc)
 
 
 def launch_count() -> int:
