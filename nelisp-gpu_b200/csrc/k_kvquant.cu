@@ -13,12 +13,18 @@
 //
 // Bound by memory.  As in k_qknorm.cu a group of lanes holds a head vector,
 // two 16-byte chunks a lane half a vector apart, so each request of a group is
-// one contiguous run; U vectors are requested before the first is used.
+// one contiguous run.  A warp takes the key or the value heads of a token (some
+// of them, while there are few tokens), so the slot is looked up once and a
+// head is a step on both sides; U vectors are requested before the first is
+// used.  Codes and floats are turned into one another by adding 2^23 and its
+// like, two at a time: the conversion instructions run at a sixteenth of the
+// rate and bound the first form of these kernels.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "f32x2.cuh"
 #include "kv_quant.cuh"
 
 namespace nl {
@@ -51,7 +57,7 @@ struct KvRows {
   void *out[2];                  // read
   uint64_t stride[2];
   const int32_t *slot;
-  uint32_t vectors;              // 2 * n * kv_heads: a token's key heads, then its value heads
+  uint32_t n, per_job, jobs_per_part;   // tokens; heads a warp takes, its share of a token's
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -65,50 +71,9 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
-// x is at most 2^21 in magnitude and BIAS an integer: the low bits of the
-// result are those of the integer BIAS + rint(x) (ties to even: 1.5 * 2^23 is
-// even, and so is every BIAS used).
-template <int BIAS>
-__device__ __forceinline__ uint32_t round_bits(float x) {
-  return __float_as_uint(__fadd_rn(x, 12582912.0f + (float)BIAS));
-}
 __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-
-// N values (a 16-byte chunk) and back, as floats.
-template <typename T> struct Values;
-template <> struct Values<float> {
-  static constexpr int N = 4;
-  static __device__ __forceinline__ void get(const uint4 &w, float *v) {
-    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y);
-    v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
-  }
-  static __device__ __forceinline__ uint4 put(const float *v) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                      __float_as_uint(v[3]));
-  }
-};
-template <> struct Values<__nv_bfloat16> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ void get(const uint4 &w, float *v) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      v[2 * i] = __uint_as_float(u[i] << 16);
-      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ uint4 put(const float *v) {
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      u[i] = *reinterpret_cast<const uint32_t *>(&p);
-    }
-    return make_uint4(u[0], u[1], u[2], u[3]);
-  }
-};
 
 // The unsigned integer that holds the codes of a chunk of N values.
 template <int BYTES> struct Word;
@@ -117,25 +82,56 @@ template <> struct Word<4> { using type = uint32_t; };
 template <> struct Word<8> { using type = uint2; };
 
 // Codes of N values as 32-bit words (one word, its low half for four 4-bit
-// codes).
+// codes).  Adding 1.5 * 2^23 (and 128) rounds to an integer, ties to even, in
+// the low bits of the sum.
 template <int BITS, int N>
-__device__ __forceinline__ void encode(const float *v, float lo, float inv, uint32_t *w) {
+__device__ __forceinline__ void encode(const Pair *v, float lo, float inv, uint32_t *w) {
+  const float magic = 12582912.0f + (BITS == 8 ? 128.0f : 0.0f);
+  uint32_t c[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    // one at a time: the packed product and sum were contracted, and the code
+    // is that of the rounded product
+    const float2 f = unpair(v[i / 2]);
+    float x = i & 1 ? f.y : f.x;
+    if (BITS == 4) x = __fsub_rn(x, lo);
+    x = __fmul_rn(x, inv);
+    if (BITS == 4) x = fminf(x, 15.0f);
+    c[i] = __float_as_uint(__fadd_rn(x, magic));
+  }
   if (BITS == 8) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4)
-      w[i / 4] = low_bytes(round_bits<128>(__fmul_rn(v[i], inv)),
-                           round_bits<128>(__fmul_rn(v[i + 1], inv)),
-                           round_bits<128>(__fmul_rn(v[i + 2], inv)),
-                           round_bits<128>(__fmul_rn(v[i + 3], inv)));
+    for (int i = 0; i < N; i += 4) w[i / 4] = low_bytes(c[i], c[i + 1], c[i + 2], c[i + 3]);
   } else {
-    uint32_t c[N];
-#pragma unroll
-    for (int i = 0; i < N; i++)
-      c[i] = round_bits<0>(fminf(__fmul_rn(__fsub_rn(v[i], lo), inv), 15.0f)) & 15u;
+    // bytes of the even and the odd codes, the odd ones four bits up
     uint32_t x = 0;
 #pragma unroll
-    for (int i = 0; i < N; i++) x |= c[i] << (4 * i);
+    for (int i = 0; i < N; i += 4) {
+      const uint32_t even = __byte_perm(c[i], c[i + 2], 0x0040) & 0x0f0fu;
+      const uint32_t odd = __byte_perm(c[i + 1], c[i + 3], 0x0040) & 0x0f0fu;
+      x |= (even | odd << 4) << (4 * i);
+    }
     w[0] = x;
+  }
+}
+
+// The values of N codes: 2^23 + code is exact, and so is the difference.
+template <int BITS, int N>
+__device__ __forceinline__ void decode(const uint32_t *w, float s, float lo, Pair *v) {
+  const float back = -(8388608.0f + (BITS == 8 ? 128.0f : 0.0f));
+  const Pair back2 = pair(back, back), s2 = pair(s, s), lo2 = pair(lo, lo);
+#pragma unroll
+  for (int i = 0; i < N / 2; i++) {
+    uint32_t c[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int k = 2 * i + e;
+      c[e] = BITS == 8 ? __byte_perm(w[k / 4], 0x4b000000u, 0x7440 + k % 4)
+                       : (w[0] >> (4 * k) & 15u) | 0x4b000000u;
+    }
+    Pair x = mul2(add2(pair(__uint_as_float(c[0]), __uint_as_float(c[1])), back2), s2);
+    if (BITS == 4) x = add2(x, lo2);   // s c has 12 bits: exact, so rounded once
+    v[i] = x;
   }
 }
 
@@ -143,153 +139,162 @@ __device__ __forceinline__ float bf16_up(float x) {   // of a positive finite x
   return __uint_as_float((__float_as_uint(x) + 0xffffu) & 0xffff0000u);
 }
 
+// A warp's job: some heads of the keys or the values of a token.
+struct Job {
+  uint32_t token, kv, h0, h1;
+  uint32_t row;                  // of head 0 in the pool, or ~0
+};
+__device__ __forceinline__ Job job_of(const KvRows &r, const KvPool &p, uint64_t i) {
+  Job j;
+  const uint32_t per = 2 * r.jobs_per_part;
+  j.token = (uint32_t)(i / per);
+  const uint32_t rest = (uint32_t)(i - (uint64_t)j.token * per);
+  j.kv = rest >= r.jobs_per_part;
+  j.h0 = (j.kv ? rest - r.jobs_per_part : rest) * r.per_job;
+  j.h1 = min(j.h0 + r.per_job, p.kv_heads);
+  const uint32_t slot = (uint32_t)__ldg(r.slot + j.token), block = slot / p.block_size;
+  j.row = block < p.num_blocks ? kv_row(p, block, slot - block * p.block_size, 0) : ~0u;
+  return j;
+}
+
 template <typename T, int HD, int BITS, int U>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPool p) {
-  constexpr int N = Values<T>::N, G = HD / (2 * N), H = 32 / G, CB = N * BITS / 8;
+__global__ void __launch_bounds__(kThreads)
+kv_append_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPool p) {
+  constexpr int N = Chunk<T>::N, G = HD / (2 * N), H = 32 / G, CB = N * BITS / 8;
   using W = typename Word<CB>::type;
   pdl_trigger();
   pdl_wait();
-  const uint32_t lane = threadIdx.x & 31, j = lane % G;
-  const uint64_t step = (uint64_t)gridDim.x * (kThreads / 32) * (H * U);
-  uint64_t base = ((uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (H * U);
-  for (; base < r.vectors; base += step) {
-    uint4 w[U][2];
-    uint32_t at[U];               // row in the pool, or ~0
+  const uint32_t lane = threadIdx.x & 31, j = lane % G, mine = lane / G;
+  const uint64_t jobs = (uint64_t)r.n * 2 * r.jobs_per_part;
+  for (uint64_t i = (uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < jobs;
+       i += (uint64_t)gridDim.x * (kThreads / 32)) {
+    const Job job = job_of(r, p, i);
+    const T *x = (const T *)r.in[job.kv] + (uint64_t)job.token * r.stride[job.kv];
+    uint8_t *code = p.code[job.kv];
+    for (uint32_t h = job.h0; h < job.h1; h += H * U) {
+      uint4 w[U][2];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint64_t i = base + u * H + lane / G;
-      at[u] = ~0u;
-      w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
-      if (i < r.vectors) {
-        const uint32_t token = (uint32_t)i / (2 * p.kv_heads);
-        const uint32_t rest = (uint32_t)i % (2 * p.kv_heads);
-        const uint32_t kv = rest / p.kv_heads, head = rest % p.kv_heads;
-        const uint32_t slot = (uint32_t)__ldg(r.slot + token);
-        const T *x = (const T *)r.in[kv] + (uint64_t)token * r.stride[kv] + (uint64_t)head * HD;
-        w[u][0] = __ldcs(reinterpret_cast<const uint4 *>(x) + j);
-        w[u][1] = __ldcs(reinterpret_cast<const uint4 *>(x) + j + G);
-        const uint32_t block = slot / p.block_size;
-        if (block < p.num_blocks) at[u] = kv_row(p, block, slot % p.block_size, head);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint64_t i = base + u * H + lane / G;
-      const uint32_t kv = (uint32_t)i % (2 * p.kv_heads) / p.kv_heads;
-      float v[2 * N];
-      Values<T>::get(w[u][0], v);
-      Values<T>::get(w[u][1], v + N);
-      float hi = BITS == 8 ? fabsf(v[0]) : v[0], lo = v[0];
-#pragma unroll
-      for (int e = 1; e < 2 * N; e++) {
-        hi = max_nan(hi, BITS == 8 ? fabsf(v[e]) : v[e]);
-        if (BITS == 4) lo = min_nan(lo, v[e]);
+      for (int u = 0; u < U; u++) {
+        const uint32_t hh = h + u * H + mine;
+        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+        if (hh < job.h1) {
+          const uint4 *v = reinterpret_cast<const uint4 *>(x + (uint64_t)hh * HD);
+          w[u][0] = __ldcs(v + j);
+          w[u][1] = __ldcs(v + j + G);
+        }
       }
 #pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) {
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        if (BITS == 4) lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      }
-      float s, inv = 0.0f;
-      uint32_t word;
-      if (BITS == 8) {
-        const bool some = hi >= 127.0f * kKvTiny;
-        s = some ? __fdiv_rn(hi, 127.0f) : 0.0f;
-        if (some) inv = __fdiv_rn(127.0f, hi);
-        if (!(hi < INFINITY)) s = __uint_as_float(0x7fc00000u), inv = 0.0f;
-        word = __float_as_uint(s);
-      } else {
-        lo = __bfloat162float(__float2bfloat16_rd(lo));
-        const float range = __fsub_rn(hi, lo);
-        s = bf16_up(__fdiv_rn(range, 15.0f));
-        const bool some = s >= kKvTiny;
-        if (some) inv = __fdiv_rn(1.0f, s);
-        else s = 0.0f;
-        word = __float_as_uint(s) >> 16 | (__float_as_uint(lo) & 0xffff0000u);
-        if (!(range < INFINITY)) word = 0x7fc0u, inv = 0.0f;
-      }
-      if (at[u] != ~0u) {
-        const bool bad = BITS == 8 ? !(hi < INFINITY) : word == 0x7fc0u;
-        uint32_t c[2][N * BITS / 8 < 4 ? 1 : N * BITS / 32];
+      for (int u = 0; u < U; u++) {
+        const uint32_t hh = h + u * H + mine;
+        Pair v[N];
+        Chunk<T>::get(w[u][0], v);
+        Chunk<T>::get(w[u][1], v + N / 2);
+        const float2 f0 = unpair(v[0]);
+        float hi = BITS == 8 ? max_nan(fabsf(f0.x), fabsf(f0.y)) : max_nan(f0.x, f0.y);
+        float lo = min_nan(f0.x, f0.y);
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-          if (bad) {
+        for (int e = 1; e < N; e++) {
+          const float2 f = unpair(v[e]);
+          hi = BITS == 8 ? max_nan(hi, max_nan(fabsf(f.x), fabsf(f.y)))
+                         : max_nan(hi, max_nan(f.x, f.y));
+          if (BITS == 4) lo = min_nan(lo, min_nan(f.x, f.y));
+        }
 #pragma unroll
-            for (int e = 0; e < N; e++) v[k * N + e] = 0.0f;
+        for (int o = G / 2; o > 0; o >>= 1) {
+          hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+          if (BITS == 4) lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        }
+        float s, inv = 0.0f;
+        uint32_t word;
+        bool bad;
+        if (BITS == 8) {
+          const bool some = hi >= 127.0f * kKvTiny;
+          s = some ? __fdiv_rn(hi, 127.0f) : 0.0f;
+          if (some) inv = __fdiv_rn(127.0f, hi);
+          bad = !(hi < INFINITY);
+          word = bad ? 0x7fc00000u : __float_as_uint(s);
+        } else {
+          lo = __bfloat162float(__float2bfloat16_rd(lo));
+          const float range = __fsub_rn(hi, lo);
+          s = bf16_up(__fdiv_rn(range, 15.0f));
+          const bool some = s >= kKvTiny;
+          if (some) inv = __fdiv_rn(1.0f, s);
+          else s = 0.0f;
+          bad = !(range < INFINITY);
+          word = bad ? 0x7fc0u
+                     : __float_as_uint(s) >> 16 | (__float_as_uint(lo) & 0xffff0000u);
+        }
+        if (bad) {                 // the scale says so: the codes are those of zero
+#pragma unroll
+          for (int e = 0; e < N; e++) v[e] = 0;
+          lo = inv = 0.0f;
+        }
+        if (hh < job.h1 && job.row != ~0u) {
+          const uint32_t at = job.row + hh * p.block_size;
+          uint8_t *to = code + (uint64_t)at * (HD * BITS / 8) + j * CB;
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            uint32_t c[2];
+            encode<BITS, N>(v + k * (N / 2), lo, inv, c);
+            W t;
+            if constexpr (CB == 8) t = make_uint2(c[0], c[1]);
+            else t = (W)c[0];
+            *reinterpret_cast<W *>(to + k * G * CB) = t;
           }
-          encode<BITS, N>(v + k * N, bad ? 0.0f : lo, inv, c[k]);
+          if (j == 0) p.param[job.kv][at] = word;
         }
-        uint8_t *row = p.code[kv] + (uint64_t)at[u] * (HD * BITS / 8);
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-          W t;
-          if constexpr (CB == 8) t = make_uint2(c[k][0], c[k][1]);
-          else t = (W)c[k][0];
-          *reinterpret_cast<W *>(row + (j + k * G) * CB) = t;
-        }
-        if (j == 0) p.param[kv][at[u]] = word;
       }
     }
   }
 }
 
 template <typename T, int HD, int BITS, int U>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPool p) {
-  constexpr int N = Values<T>::N, G = HD / (2 * N), H = 32 / G, CB = N * BITS / 8;
+__global__ void __launch_bounds__(kThreads)
+kv_read_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPool p) {
+  constexpr int N = Chunk<T>::N, G = HD / (2 * N), H = 32 / G, CB = N * BITS / 8;
   using W = typename Word<CB>::type;
   pdl_trigger();
   pdl_wait();
-  const uint32_t lane = threadIdx.x & 31, j = lane % G;
-  const uint64_t step = (uint64_t)gridDim.x * (kThreads / 32) * (H * U);
-  uint64_t base = ((uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (H * U);
-  for (; base < r.vectors; base += step) {
-    W w[U][2];
-    uint32_t word[U];
+  const uint32_t lane = threadIdx.x & 31, j = lane % G, mine = lane / G;
+  const uint64_t jobs = (uint64_t)r.n * 2 * r.jobs_per_part;
+  for (uint64_t i = (uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < jobs;
+       i += (uint64_t)gridDim.x * (kThreads / 32)) {
+    const Job job = job_of(r, p, i);
+    T *y = (T *)r.out[job.kv] + (uint64_t)job.token * r.stride[job.kv];
+    const uint8_t *code = p.code[job.kv];
+    const uint32_t *param = p.param[job.kv];
+    for (uint32_t h = job.h0; h < job.h1; h += H * U) {
+      W w[U][2];
+      uint32_t word[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint64_t i = base + u * H + lane / G;
-      word[u] = 0;
-      w[u][0] = w[u][1] = W{};
-      if (i < r.vectors) {
-        const uint32_t token = (uint32_t)i / (2 * p.kv_heads);
-        const uint32_t rest = (uint32_t)i % (2 * p.kv_heads);
-        const uint32_t kv = rest / p.kv_heads, head = rest % p.kv_heads;
-        const uint32_t slot = (uint32_t)__ldg(r.slot + token), block = slot / p.block_size;
-        if (block < p.num_blocks) {
-          const uint32_t at = kv_row(p, block, slot % p.block_size, head);
-          const uint8_t *row = p.code[kv] + (uint64_t)at * (HD * BITS / 8);
-          word[u] = p.param[kv][at];
-          w[u][0] = *reinterpret_cast<const W *>(row + j * CB);
-          w[u][1] = *reinterpret_cast<const W *>(row + (j + G) * CB);
+      for (int u = 0; u < U; u++) {
+        const uint32_t hh = h + u * H + mine;
+        word[u] = 0;
+        w[u][0] = w[u][1] = W{};
+        if (hh < job.h1 && job.row != ~0u) {
+          const uint32_t at = job.row + hh * p.block_size;
+          const uint8_t *from = code + (uint64_t)at * (HD * BITS / 8) + j * CB;
+          word[u] = param[at];
+          w[u][0] = *reinterpret_cast<const W *>(from);
+          w[u][1] = *reinterpret_cast<const W *>(from + G * CB);
         }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint64_t i = base + u * H + lane / G;
-      if (i >= r.vectors) continue;
-      const uint32_t token = (uint32_t)i / (2 * p.kv_heads);
-      const uint32_t rest = (uint32_t)i % (2 * p.kv_heads);
-      const uint32_t kv = rest / p.kv_heads, head = rest % p.kv_heads;
-      const float s = __uint_as_float(BITS == 8 ? word[u] : word[u] << 16);
-      const float lo = BITS == 8 ? 0.0f : __uint_as_float(word[u] & 0xffff0000u);
-      uint4 *y = reinterpret_cast<uint4 *>((T *)r.out[kv] + (uint64_t)token * r.stride[kv] +
-                                           (uint64_t)head * HD);
+      for (int u = 0; u < U; u++) {
+        const uint32_t hh = h + u * H + mine;
+        if (hh >= job.h1) continue;
+        const float s = __uint_as_float(BITS == 8 ? word[u] : word[u] << 16);
+        const float lo = BITS == 8 ? 0.0f : __uint_as_float(word[u] & 0xffff0000u);
+        uint4 *to = reinterpret_cast<uint4 *>(y + (uint64_t)hh * HD) + j;
 #pragma unroll
-      for (int k = 0; k < 2; k++) {
-        uint32_t c[2];
-        if constexpr (CB == 8) c[0] = w[u][k].x, c[1] = w[u][k].y;
-        else c[0] = w[u][k];
-        float v[N];
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-          if (BITS == 8) {
-            v[e] = s * (float)((int)(c[e / 4] >> (8 * (e % 4)) & 255u) - 128);
-          } else {   // s c has 12 bits: exact, so one rounding either way
-            v[e] = __fadd_rn(__fmul_rn(s, (float)(c[0] >> (4 * e) & 15u)), lo);
-          }
+        for (int k = 0; k < 2; k++) {
+          uint32_t c[2];
+          if constexpr (CB == 8) c[0] = w[u][k].x, c[1] = w[u][k].y;
+          else c[0] = w[u][k], c[1] = 0;
+          Pair v[N / 2];
+          decode<BITS, N>(c, s, lo, v);
+          __stcs(to + k * G, Chunk<T>::put(v));
         }
-        y[j + k * G] = Values<T>::put(v);
       }
     }
   }
@@ -328,20 +333,27 @@ kv_move_kernel(const __grid_constant__ KvPool p, const int32_t *src, const int32
   }
 }
 
-// Both directions take U vectors a group at a time: 4 for rows of 16 bits or
-// 32 bits alike, so a warp has 4 KB requested.
-constexpr int kU = 4;
-
+// U vectors a group at a time (append + read of 4095 tokens of 20 heads of 128,
+// f32, 8 bits: 41.0 us with 2, 37.9 with 4; 16384 of 8 heads, bf16, 4 bits: 37.6
+// with 2, 50.9 with 4); at most 8 blocks an SM, and while there are fewer jobs
+// than warps a warp takes fewer heads.
 template <typename T, int HD, int BITS>
-cudaError_t start(bool append, const KvRows &r, const KvPool &p, cudaStream_t st) {
-  constexpr uint64_t per_block = (kThreads / 32) * (32 / (HD / (2 * Values<T>::N))) * kU;
-  const uint64_t want = ceil_div64(r.vectors, per_block);
-  const dim3 grid((unsigned)(want < 148 * 8 ? want : 148 * 8));
-  return append ? launch_pdl(kv_append_kernel<T, HD, BITS, kU>, grid, dim3(kThreads), 0, st, r, p)
-                : launch_pdl(kv_read_kernel<T, HD, BITS, kU>, grid, dim3(kThreads), 0, st, r, p);
+cudaError_t start(bool append, KvRows &r, const KvPool &p, cudaStream_t st) {
+  constexpr int U = sizeof(T) == 4 ? 4 : 2;
+  constexpr uint32_t H = 32 / (HD / (2 * Chunk<T>::N)), warps = kThreads / 32;
+  constexpr uint64_t most = 148 * 8;
+  uint32_t per = p.kv_heads;
+  while (per > H && (uint64_t)r.n * 2 * ((p.kv_heads + per - 1) / per) < most * warps)
+    per = (per + 1) / 2;
+  r.per_job = (per + H - 1) / H * H;
+  r.jobs_per_part = (p.kv_heads + r.per_job - 1) / r.per_job;
+  const uint64_t want = ceil_div64((uint64_t)r.n * 2 * r.jobs_per_part, warps);
+  const dim3 grid((unsigned)(want < most ? want : most));
+  return append ? launch_pdl(kv_append_kernel<T, HD, BITS, U>, grid, dim3(kThreads), 0, st, r, p)
+                : launch_pdl(kv_read_kernel<T, HD, BITS, U>, grid, dim3(kThreads), 0, st, r, p);
 }
 template <typename T>
-cudaError_t start_t(bool append, const KvRows &r, const KvPool &p, cudaStream_t st) {
+cudaError_t start_t(bool append, KvRows &r, const KvPool &p, cudaStream_t st) {
   switch (p.head_dim + p.bits) {
     case 64 + 8: return start<T, 64, 8>(append, r, p, st);
     case 128 + 8: return start<T, 128, 8>(append, r, p, st);
@@ -372,10 +384,7 @@ int rows_call(const char *what, bool append, int fmt, int dtype, KvRows &r, KvPo
                        "multiple of %u and at least kv heads x head size",
                        what, i ? "V" : "K", (unsigned long long)r.stride[i], unit);
   }
-  if (2 * (uint64_t)n * p.kv_heads > UINT32_MAX)
-    return set_error(NL_ERROR, "%s: %u tokens x %u kv heads: at most 2^31 - 1 head vectors", what,
-                     n, p.kv_heads);
-  r.vectors = 2 * n * p.kv_heads;
+  r.n = n;
   cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = dtype == NL_BF16 ? start_t<__nv_bfloat16>(append, r, p, st)
                                          : start_t<float>(append, r, p, st);
@@ -393,7 +402,7 @@ extern "C" int nl_kv_append_dev(int fmt, int dtype, const void *K, uint64_t k_st
                                 uint32_t *KP, void *VC, uint32_t *VP, uint32_t n,
                                 uint32_t kv_heads, uint32_t head_dim, uint32_t block_size,
                                 uint32_t num_blocks, void *stream) {
-  KvRows r = {{K, V}, {nullptr, nullptr}, {k_stride, v_stride}, SLOT, 0};
+  KvRows r = {{K, V}, {nullptr, nullptr}, {k_stride, v_stride}, SLOT, 0, 0, 0};
   KvPool p = {{(uint8_t *)KC, (uint8_t *)VC}, {KP, VP}, num_blocks, block_size, kv_heads,
               head_dim, 0};
   return rows_call("kv-append", true, fmt, dtype, r, p, n, stream);
@@ -404,7 +413,7 @@ extern "C" int nl_kv_read_dev(int fmt, int dtype, const int32_t *SLOT, const voi
                               uint64_t k_stride, void *V, uint64_t v_stride, uint32_t n,
                               uint32_t kv_heads, uint32_t head_dim, uint32_t block_size,
                               uint32_t num_blocks, void *stream) {
-  KvRows r = {{nullptr, nullptr}, {K, V}, {k_stride, v_stride}, SLOT, 0};
+  KvRows r = {{nullptr, nullptr}, {K, V}, {k_stride, v_stride}, SLOT, 0, 0, 0};
   KvPool p = {{(uint8_t *)const_cast<void *>(KC), (uint8_t *)const_cast<void *>(VC)},
               {const_cast<uint32_t *>(KP), const_cast<uint32_t *>(VP)}, num_blocks, block_size,
               kv_heads, head_dim, 0};

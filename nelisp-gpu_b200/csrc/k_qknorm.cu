@@ -13,15 +13,18 @@
 // Bound by memory: every value is read once (x; x and dy) and written once.
 // A group of G lanes holds a head vector, each lane two 16-byte chunks that
 // are partners of the rotation, so a head needs one reduction over the group
-// and no exchange of values.  A warp takes one row and walks its heads with
-// the row's cosines and sines, and the gain, in registers; U vectors are
-// requested before the first is used.  All arithmetic is in 32 bits; the one
-// rounding to the output type is at the store.
+// and no exchange of values.  A warp takes one row and walks its query or its
+// key heads with the row's products of gain, cosine and sine in registers;
+// blocks belong to one of the two parts, so a thread holds one gain (and one
+// set of gain gradients).  U vectors are requested before the first is used.
+// Arithmetic is two floats an instruction, all in 32 bits; the one rounding to
+// the output type is at the store.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "f32x2.cuh"
 #include "nl_internal.h"
 
 namespace nl {
@@ -39,49 +42,16 @@ struct QkArgs {
   uint64_t dy_stride[2];
   void *out[2];                  // q and k; backward: dx of the two parts
   uint64_t out_stride[2];
-  float *partial;                // backward: [blocks][2][head_dim]
-  uint32_t n, heads, kv_heads, head_dim, rot, rope_rows;
-  uint32_t per_job, jobs_per_row;  // heads a warp takes, and jobs a row has
+  float *partial;                // backward: [blocks][head_dim]
+  uint32_t n, heads[2], head_dim, rot, rope_rows;
+  uint32_t per_job[2], jobs_per_row[2], blocks[2];  // heads a warp takes; how a part is divided
   float eps;
 };
 
-template <typename T> struct Chunk;
-template <> struct Chunk<float> {
-  static constexpr int N = 4;
-  static __device__ __forceinline__ void get(const uint4 &w, float *v) {
-    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y);
-    v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
-  }
-  static __device__ __forceinline__ uint4 put(const float *v) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                      __float_as_uint(v[3]));
-  }
-};
-template <> struct Chunk<__nv_bfloat16> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ void get(const uint4 &w, float *v) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      v[2 * i] = __uint_as_float(u[i] << 16);
-      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ uint4 put(const float *v) {
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      u[i] = *reinterpret_cast<const uint32_t *>(&p);
-    }
-    return make_uint4(u[0], u[1], u[2], u[3]);
-  }
-};
-
-// Where this lane of a group stands: its two chunks of a head vector and
-// whether they are rotated.  Pairs of a rotated lane are (v[e], v[N + e]) in
-// the half form and (v[2e], v[2e + 1]) in the adjacent form; either way their
-// angles are lane * N + e.
+// Where this lane of a group stands: its two chunks of a head vector.  Pair e
+// of a rotated lane turns by angle lane * N + e; in the half form its values
+// are the chunks' values e, in the adjacent form values 2e and 2e + 1 of the
+// two chunks in a row.  Lanes past the rotated part turn by no angle.
 struct Place {
   uint32_t c0, c1;
   bool live, turned;
@@ -98,132 +68,95 @@ __device__ __forceinline__ Place place_of(uint32_t j, uint32_t head_dim, uint32_
   return p;
 }
 
-template <int N, bool HALF>
-__device__ __forceinline__ void turn(float *v, const float *c, const float *s) {
+// The first and second values of a lane's N pairs, from its chunks and back.
+template <typename T, bool HALF>
+__device__ __forceinline__ void split(const uint4 &w0, const uint4 &w1, Pair *a, Pair *b) {
+  constexpr int N = Chunk<T>::N;
+  if (HALF) {
+    Chunk<T>::get(w0, a);
+    Chunk<T>::get(w1, b);
+  } else {
+    Pair v[N];
+    Chunk<T>::get(w0, v);
+    Chunk<T>::get(w1, v + N / 2);
 #pragma unroll
-  for (int e = 0; e < N; e++) {
-    float &a = v[HALF ? e : 2 * e], &b = v[HALF ? N + e : 2 * e + 1];
-    const float a0 = a, b0 = b;
-    a = a0 * c[e] - b0 * s[e];
-    b = a0 * s[e] + b0 * c[e];
+    for (int i = 0; i < N / 2; i++) {
+      const float2 x = unpair(v[2 * i]), y = unpair(v[2 * i + 1]);
+      a[i] = pair(x.x, y.x);
+      b[i] = pair(x.y, y.y);
+    }
+  }
+}
+template <typename T, bool HALF>
+__device__ __forceinline__ void merge(const Pair *a, const Pair *b, uint4 &w0, uint4 &w1) {
+  constexpr int N = Chunk<T>::N;
+  if (HALF) {
+    w0 = Chunk<T>::put(a);
+    w1 = Chunk<T>::put(b);
+  } else {
+    Pair v[N];
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) {
+      const float2 x = unpair(a[i]), y = unpair(b[i]);
+      v[2 * i] = pair(x.x, y.x);
+      v[2 * i + 1] = pair(x.y, y.y);
+    }
+    w0 = Chunk<T>::put(v);
+    w1 = Chunk<T>::put(v + N / 2);
   }
 }
 
 template <int G>
-__device__ __forceinline__ float group_sum(float v) {
+__device__ __forceinline__ float group_sum(Pair p) {
+  const float2 f = unpair(p);
+  float v = f.x + f.y;
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// One warp, one row, the heads [h0, h1) of one part (queries or keys), a
-// group of G lanes per head.
-template <typename T, int G, bool HALF, bool BWD, int U>
-__device__ __forceinline__ void walk(const QkArgs &a, int part, uint32_t row, uint32_t h0,
-                                     uint32_t h1, const Place &p, bool real, const float *c,
-                                     const float *s, float *dg) {
-  constexpr int N = Chunk<T>::N, H = 32 / G;
-  if (h0 >= h1) return;
-  const uint32_t lane = threadIdx.x & 31, mine = lane / G;
-  const T *x = (const T *)a.x + (uint64_t)row * a.x_stride +
-               (part ? (uint64_t)a.heads * a.head_dim : 0);
-  const T *dy = BWD ? (const T *)a.dy[part] + (uint64_t)row * a.dy_stride[part] : nullptr;
-  T *out = (T *)a.out[part] + (uint64_t)row * a.out_stride[part];
-  float g[2 * N];
-#pragma unroll
-  for (int e = 0; e < 2 * N; e++) g[e] = 0.0f;
-  if (p.live) {
-#pragma unroll
-    for (int e = 0; e < N; e++) {
-      g[e] = __ldg(a.g[part] + p.c0 * N + e);
-      g[N + e] = __ldg(a.g[part] + p.c1 * N + e);
-    }
-  }
-  const float inv_d = 1.0f / (float)a.head_dim;
-  for (uint32_t h = h0; h < h1; h += H * U) {
-    uint4 w[U][2], d[BWD ? U : 1][2];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint32_t hh = h + u * H + mine;
-      const bool on = p.live && hh < h1 && real;
-      const uint64_t at = (uint64_t)hh * a.head_dim;
-      w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
-      if (BWD) d[u][0] = d[u][1] = make_uint4(0, 0, 0, 0);
-      if (on) {
-        w[u][0] = *reinterpret_cast<const uint4 *>(x + at + p.c0 * N);
-        w[u][1] = *reinterpret_cast<const uint4 *>(x + at + p.c1 * N);
-        if (BWD) {
-          d[u][0] = *reinterpret_cast<const uint4 *>(dy + at + p.c0 * N);
-          d[u][1] = *reinterpret_cast<const uint4 *>(dy + at + p.c1 * N);
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint32_t hh = h + u * H + mine;
-      float v[2 * N];
-      Chunk<T>::get(w[u][0], v);
-      Chunk<T>::get(w[u][1], v + N);
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 2 * N; e++) ss = fmaf(v[e], v[e], ss);
-      const float r = rsqrtf(fmaf(group_sum<G>(ss), inv_d, a.eps));
-      if (!BWD) {
-#pragma unroll
-        for (int e = 0; e < 2 * N; e++) v[e] = v[e] * r * g[e];
-        if (p.turned) turn<N, HALF>(v, c, s);
-      } else {
-        float q[2 * N];
-        Chunk<T>::get(d[u][0], q);
-        Chunk<T>::get(d[u][1], q + N);
-        if (p.turned) turn<N, HALF>(q, c, s);      // s is negated by the caller
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 2 * N; e++) {
-          v[e] *= r;
-          dg[e] = fmaf(q[e], v[e], dg[e]);
-          q[e] *= g[e];
-          dot = fmaf(q[e], v[e], dot);
-        }
-        dot = group_sum<G>(dot) * inv_d;
-#pragma unroll
-        for (int e = 0; e < 2 * N; e++) v[e] = r * fmaf(-v[e], dot, q[e]);
-      }
-      if (p.live && hh < h1) {
-        const uint64_t at = (uint64_t)hh * a.head_dim;
-        if (!real) {
-#pragma unroll
-          for (int e = 0; e < 2 * N; e++) v[e] = 0.0f;
-        }
-        *reinterpret_cast<uint4 *>(out + at + p.c0 * N) = Chunk<T>::put(v);
-        *reinterpret_cast<uint4 *>(out + at + p.c1 * N) = Chunk<T>::put(v + N);
-      }
-    }
-  }
-}
-
-template <typename T, int G, bool HALF, bool BWD, int U>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
-  constexpr int N = Chunk<T>::N;
+template <typename T, int G, bool HALF, bool BWD, int U, int PER_SM>
+__global__ void __launch_bounds__(kThreads, PER_SM)
+qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
+  constexpr int N = Chunk<T>::N, P = N / 2, H = 32 / G;
   pdl_trigger();
   pdl_wait();
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = lane / G;
+  const int part = blockIdx.x >= a.blocks[0];
+  const uint32_t block = blockIdx.x - (part ? a.blocks[0] : 0), heads = a.heads[part];
+  const uint32_t per_row = a.jobs_per_row[part];
   const Place p = place_of<T, HALF>(lane % G, a.head_dim, a.rot);
-  float dg[2][2 * N];
-  if (BWD) {
+  const uint32_t at0 = p.c0 * N, at1 = p.c1 * N;
+  Pair ga[P], gb[P];
+  {
+    float v[2 * N];
 #pragma unroll
-    for (int e = 0; e < 2 * N; e++) dg[0][e] = dg[1][e] = 0.0f;
+    for (int e = 0; e < N; e++) {
+      v[e] = p.live ? __ldg(a.g[part] + (HALF ? at0 + e : (e < P ? at0 : at1 - N) + 2 * e)) : 0.0f;
+      v[N + e] =
+          p.live ? __ldg(a.g[part] + (HALF ? at1 + e : (e < P ? at0 : at1 - N) + 2 * e + 1)) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+      ga[i] = pair(v[2 * i], v[2 * i + 1]);
+      gb[i] = pair(v[N + 2 * i], v[N + 2 * i + 1]);
+    }
   }
-  const uint64_t jobs = (uint64_t)a.n * a.jobs_per_row;
-  for (uint64_t job = (uint64_t)blockIdx.x * kWarps + warp; job < jobs;
-       job += (uint64_t)gridDim.x * kWarps) {
-    const uint32_t row = (uint32_t)(job / a.jobs_per_row);
-    const uint32_t h0 = (uint32_t)(job % a.jobs_per_row) * a.per_job;
-    const uint32_t h1 = min(h0 + a.per_job, a.heads + a.kv_heads);
-    const int32_t pos = __ldg(a.pos + row);
-    const bool real = (uint32_t)pos < a.rope_rows;
-    float c[N], s[N];
-    if (p.turned && real) {
+  Pair da[P], db[P];             // backward: the gain's gradient so far
+#pragma unroll
+  for (int i = 0; i < P; i++) da[i] = db[i] = 0;
+  const float inv_d = 1.0f / (float)a.head_dim;
+  const uint64_t jobs = (uint64_t)a.n * per_row;
+  // the position and the angles of a job's row, asked for a job ahead
+  const uint64_t step = (uint64_t)a.blocks[part] * kWarps;
+  auto position = [&](uint64_t job) {
+    return job < jobs ? __ldg(a.pos + (per_row == 1 ? job : job / per_row)) : -1;
+  };
+  float c[N], s[N];
+  auto angles = [&](int32_t pos) {
+#pragma unroll
+    for (int e = 0; e < N; e++) c[e] = 1.0f, s[e] = 0.0f;
+    if (p.turned && (uint32_t)pos < a.rope_rows) {
       const uint64_t at = (uint64_t)pos * (a.rot / 2) + (lane % G) * N;
 #pragma unroll
       for (int e = 0; e < N; e += 4) {
@@ -232,42 +165,135 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
         c[e] = cc.x; c[e + 1] = cc.y; c[e + 2] = cc.z; c[e + 3] = cc.w;
         s[e] = sc.x; s[e + 1] = sc.y; s[e + 2] = sc.z; s[e + 3] = sc.w;
       }
-      if (BWD) {
-#pragma unroll
-        for (int e = 0; e < N; e++) s[e] = -s[e];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; e++) c[e] = s[e] = 0.0f;
     }
-    walk<T, G, HALF, BWD, U>(a, 0, row, min(h0, a.heads), min(h1, a.heads), p, real, c, s, dg[0]);
-    walk<T, G, HALF, BWD, U>(a, 1, row, max(h0, a.heads) - a.heads, max(h1, a.heads) - a.heads, p,
-                             real, c, s, dg[1]);
+  };
+  const uint64_t first = (uint64_t)block * kWarps + warp;
+  int32_t pos = position(first), pos_next = position(first + step);
+  angles(pos);
+  for (uint64_t job = first; job < jobs; job += step) {
+    const uint32_t row = per_row == 1 ? (uint32_t)job : (uint32_t)(job / per_row);
+    const uint32_t h0 = per_row == 1 ? 0 : (uint32_t)(job % per_row) * a.per_job[part];
+    const uint32_t h1 = min(h0 + a.per_job[part], heads);
+    const bool real = (uint32_t)pos < a.rope_rows;
+    const T *x = (const T *)a.x + (uint64_t)row * a.x_stride +
+                 (part ? (uint64_t)a.heads[0] * a.head_dim : 0);
+    const T *dy = BWD ? (const T *)a.dy[part] + (uint64_t)row * a.dy_stride[part] : nullptr;
+    T *out = (T *)a.out[part] + (uint64_t)row * a.out_stride[part];
+    // Forward: ca = ga c, sa = ga s, cb = gb c, sb = -gb s, for
+    // y_a = r (a ca + b sb), y_b = r (a sa + b cb).  Backward: ca = c, sa = s,
+    // sb = -s, for u_a = dy_a c + dy_b s, u_b = dy_b c - dy_a s.
+    Pair ca[P], sa[P], cb[BWD ? 1 : P], sb[P];
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+      const Pair c2 = pair(c[2 * i], c[2 * i + 1]), s2 = pair(s[2 * i], s[2 * i + 1]);
+      const Pair m2 = pair(-s[2 * i], -s[2 * i + 1]);
+      ca[i] = BWD ? c2 : mul2(ga[i], c2);
+      sa[i] = BWD ? s2 : mul2(ga[i], s2);
+      sb[i] = BWD ? m2 : mul2(gb[i], m2);
+      if (!BWD) cb[i % (BWD ? 1 : P)] = mul2(gb[i], c2);
+    }
+    pos = pos_next;
+    pos_next = position(job + 2 * step);
+    angles(pos);
+    for (uint32_t h = h0; h < h1; h += H * U) {
+      uint4 w[U][2], d[BWD ? U : 1][2];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const uint32_t hh = h + u * H + mine;
+        const T *v = x + (uint64_t)hh * a.head_dim;
+        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+        if (BWD) d[u % (BWD ? U : 1)][0] = d[u % (BWD ? U : 1)][1] = make_uint4(0, 0, 0, 0);
+        if (p.live && hh < h1) {
+          w[u][0] = __ldcs(reinterpret_cast<const uint4 *>(v + at0));
+          w[u][1] = __ldcs(reinterpret_cast<const uint4 *>(v + at1));
+          if (BWD) {
+            const T *g = dy + (uint64_t)hh * a.head_dim;
+            d[u % (BWD ? U : 1)][0] = *reinterpret_cast<const uint4 *>(g + at0);
+            d[u % (BWD ? U : 1)][1] = *reinterpret_cast<const uint4 *>(g + at1);
+          }
+        }
+      }
+      if (!real) {                 // a row of padding: nothing it holds counts
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+          if (BWD) d[u % (BWD ? U : 1)][0] = d[u % (BWD ? U : 1)][1] = make_uint4(0, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const uint32_t hh = h + u * H + mine;
+        Pair va[P], vb[P], ss = 0;
+        split<T, HALF>(w[u][0], w[u][1], va, vb);
+#pragma unroll
+        for (int i = 0; i < P; i++) ss = fma2(vb[i], vb[i], fma2(va[i], va[i], ss));
+        // 0 where there is nothing: with no eps a vector of zeros would make NaN
+        const float sum = group_sum<G>(ss);
+        const float r = real && hh < h1 ? rsqrtf(fmaf(sum, inv_d, a.eps)) : 0.0f;
+        const Pair r2 = pair(r, r);
+        if (!BWD) {
+#pragma unroll
+          for (int i = 0; i < P; i++) {
+            const Pair x0 = mul2(va[i], r2), x1 = mul2(vb[i], r2);
+            va[i] = fma2(x0, ca[i], mul2(x1, sb[i]));
+            vb[i] = fma2(x0, sa[i], mul2(x1, cb[i % (BWD ? 1 : P)]));
+          }
+        } else {
+          // t = u x: dg += r t, and dx = r g u - x r^3 mean(g t)
+          Pair ua[P], ub[P], dot = 0;
+          split<T, HALF>(d[u % (BWD ? U : 1)][0], d[u % (BWD ? U : 1)][1], ua, ub);
+#pragma unroll
+          for (int i = 0; i < P; i++) {
+            const Pair y0 = ua[i], y1 = ub[i];
+            ua[i] = fma2(y0, ca[i], mul2(y1, sa[i]));
+            ub[i] = fma2(y1, ca[i], mul2(y0, sb[i]));
+            const Pair t0 = mul2(ua[i], va[i]), t1 = mul2(ub[i], vb[i]);
+            da[i] = fma2(t0, r2, da[i]);
+            db[i] = fma2(t1, r2, db[i]);
+            dot = fma2(t1, gb[i], fma2(t0, ga[i], dot));
+          }
+          const float k = -(r * r) * r * (group_sum<G>(dot) * inv_d);
+          const Pair k2 = pair(k, k);
+#pragma unroll
+          for (int i = 0; i < P; i++) {
+            va[i] = fma2(va[i], k2, mul2(mul2(ua[i], ga[i]), r2));
+            vb[i] = fma2(vb[i], k2, mul2(mul2(ub[i], gb[i]), r2));
+          }
+        }
+        if (p.live && hh < h1) {
+          uint4 y0, y1;
+          merge<T, HALF>(va, vb, y0, y1);
+          T *to = out + (uint64_t)hh * a.head_dim;
+          *reinterpret_cast<uint4 *>(to + at0) = y0;
+          *reinterpret_cast<uint4 *>(to + at1) = y1;
+        }
+      }
+    }
   }
   if (BWD) {
-    // this block's share of the gain gradients, summed in a fixed order
+    // this block's share of the gain's gradient, summed in a fixed order
     __shared__ float red[kWarps][2 * N * G];
 #pragma unroll
-    for (int part = 0; part < 2; part++) {
+    for (int i = 0; i < 2 * P; i++) {
+      const float2 f = unpair(i < P ? da[i % P] : db[i % P]);
+      float v[2] = {f.x, f.y};
 #pragma unroll
-      for (int e = 0; e < 2 * N; e++) {
-        float v = dg[part][e];
+      for (int e = 0; e < 2; e++) {
 #pragma unroll
-        for (int o = G; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane < G) red[warp][lane * 2 * N + e] = v;
+        for (int o = G; o < 32; o <<= 1) v[e] += __shfl_xor_sync(0xffffffffu, v[e], o);
+        if (lane < G) red[warp][lane * 2 * N + 2 * i + e] = v[e];
       }
-      __syncthreads();
-      for (uint32_t i = threadIdx.x; i < 2 * N * G; i += kThreads) {
-        const Place q = place_of<T, HALF>(i / (2 * N), a.head_dim, a.rot);
-        float v = 0.0f;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < 2 * N * G; i += kThreads) {
+      const Place q = place_of<T, HALF>(i / (2 * N), a.head_dim, a.rot);
+      float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) v += red[w][i];
-        const uint32_t e = i % (2 * N);
-        if (q.live)
-          a.partial[((uint64_t)blockIdx.x * 2 + part) * a.head_dim +
-                    (e < N ? q.c0 * N + e : q.c1 * N + e - N)] = v;
-      }
-      __syncthreads();
+      for (int w = 0; w < kWarps; w++) v += red[w][i];
+      // slot e < N is the first value of pair e, N + e the second
+      const uint32_t e = i % (2 * N), k = e % N, second = e / N;
+      const uint32_t at = HALF ? (second ? q.c1 : q.c0) * N + k : q.c0 * N + 2 * k + second;
+      if (q.live) a.partial[(uint64_t)blockIdx.x * a.head_dim + at] = v;
     }
   }
 }
@@ -275,44 +301,50 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
 // dG[part][i] = the sum of the blocks' shares, in a fixed order: a block takes
 // eight columns, 32 threads a column.
 __global__ void __launch_bounds__(256)
-qk_gain_sum_kernel(const float *partial, uint32_t blocks, uint32_t head_dim, float *dgq,
-                   float *dgk) {
+qk_gain_sum_kernel(const float *partial, uint32_t blocks_q, uint32_t blocks_k, uint32_t head_dim,
+                   float *dgq, float *dgk) {
   pdl_trigger();
   pdl_wait();
   __shared__ float red[32][9];
-  const uint32_t col = threadIdx.x & 7, k = threadIdx.x >> 3, at = blockIdx.x * 8 + col;
+  const uint32_t col = threadIdx.x & 7, k = threadIdx.x >> 3, part = blockIdx.y;
+  const uint32_t at = blockIdx.x * 8 + col, blocks = part ? blocks_k : blocks_q;
+  if (part) partial += (uint64_t)blocks_q * head_dim;
   float v = 0.0f;
-  for (uint32_t b = k; b < blocks; b += 32) v += partial[(uint64_t)b * 2 * head_dim + at];
+#pragma unroll 4
+  for (uint32_t b = k; b < blocks; b += 32) v += partial[(uint64_t)b * head_dim + at];
   red[k][col] = v;
   __syncthreads();
   if (k == 0) {
     float t = 0.0f;
 #pragma unroll
     for (int i = 0; i < 32; i++) t += red[i][col];
-    if (at < head_dim) dgq[at] = t;
-    else dgk[at - head_dim] = t;
+    (part ? dgk : dgq)[at] = t;
   }
 }
 
-template <typename T, int G, bool HALF, bool BWD, int U>
-cudaError_t start(QkArgs &a, uint32_t blocks, cudaStream_t st) {
-  return launch_pdl(qk_norm_rope_kernel<T, G, HALF, BWD, U>, dim3(blocks), dim3(kThreads), 0, st,
-                    a);
+template <typename T, int G, bool HALF, bool BWD>
+cudaError_t start(QkArgs &a, cudaStream_t st) {
+  // Vectors a group takes at a time, and blocks an SM.  8192 rows of 40 heads of
+  // 128, bf16: 37.2 us with 2 and 2; 40.9 with 4 and 2, 42.7 with 2 and 3 (which
+  // spills).  The same loads and stores with no arithmetic between: 33.5.
+  // Backward, 8191 rows of 40 heads of 64, bf16: 36.2 with 1 and 2, 46.3 with 2
+  // and 2 (spills).  A float32 lane holds half as many values.
+  constexpr int U = (BWD ? 1 : 2) * (sizeof(T) == 4 ? 2 : 1), PER_SM = 2;
+  return launch_pdl(qk_norm_rope_kernel<T, G, HALF, BWD, U, PER_SM>,
+                    dim3(a.blocks[0] + a.blocks[1]), dim3(kThreads), 0, st, a);
 }
 template <typename T, bool BWD>
-cudaError_t start_t(QkArgs &a, bool half, uint32_t group, uint32_t blocks, cudaStream_t st) {
-  constexpr int U = BWD ? 2 : 4;
+cudaError_t start_t(QkArgs &a, bool half, uint32_t group, cudaStream_t st) {
   switch (group * 2 + (half ? 1 : 0)) {
-    case 8: return start<T, 4, false, BWD, U>(a, blocks, st);
-    case 9: return start<T, 4, true, BWD, U>(a, blocks, st);
-    case 16: return start<T, 8, false, BWD, U>(a, blocks, st);
-    case 17: return start<T, 8, true, BWD, U>(a, blocks, st);
-    case 32: return start<T, 16, false, BWD, U>(a, blocks, st);
-    case 33: return start<T, 16, true, BWD, U>(a, blocks, st);
+    case 8: return start<T, 4, false, BWD>(a, st);
+    case 9: return start<T, 4, true, BWD>(a, st);
+    case 16: return start<T, 8, false, BWD>(a, st);
+    case 17: return start<T, 8, true, BWD>(a, st);
+    case 32: return start<T, 16, false, BWD>(a, st);
+    case 33: return start<T, 16, true, BWD>(a, st);
   }
   if constexpr (sizeof(T) == 4) {   // 256 values of 16 bits take 16 lanes
-    return half ? start<T, 32, true, BWD, U>(a, blocks, st)
-                : start<T, 32, false, BWD, U>(a, blocks, st);
+    return half ? start<T, 32, true, BWD>(a, st) : start<T, 32, false, BWD>(a, st);
   }
   return cudaErrorInvalidValue;
 }
@@ -325,21 +357,30 @@ uint32_t group_of(int dtype, uint32_t head_dim) {
   return g;
 }
 
-constexpr uint32_t kMaxBlocks = 148 * 4;
+constexpr uint32_t kMaxBlocks = 148 * 2;
 
-// How a launch divides n rows of HEADS heads: a warp takes whole rows once
-// there are enough of them to fill the GPU's warps, and otherwise as few heads
-// as a warp holds at a time.
-uint32_t divide(QkArgs &a, uint32_t at_once) {
-  const uint32_t all = a.heads + a.kv_heads;
-  a.per_job = all;
-  while (a.per_job > at_once &&
-         (uint64_t)a.n * ((all + a.per_job - 1) / a.per_job) < (uint64_t)kMaxBlocks * kWarps)
-    a.per_job = (a.per_job + 1) / 2;
-  a.per_job = (a.per_job + at_once - 1) / at_once * at_once;
-  a.jobs_per_row = (all + a.per_job - 1) / a.per_job;
-  const uint64_t blocks = ceil_div64((uint64_t)a.n * a.jobs_per_row, kWarps);
-  return (uint32_t)(blocks < kMaxBlocks ? blocks : kMaxBlocks);
+// What a row costs a warp besides its heads, in heads.
+constexpr uint32_t kRowCost = 4;
+
+// How a launch divides n rows of the two parts' heads: the blocks (at most
+// kMaxBlocks) in proportion to the heads; a warp takes whole rows once there
+// are enough of them to fill the blocks' warps, and otherwise as few heads as a
+// warp holds at a time.
+void divide(QkArgs &a, uint32_t at_once) {
+  const uint32_t all = a.heads[0] + a.heads[1];
+  for (int p = 0; p < 2; p++) {
+    uint64_t most = (uint64_t)kMaxBlocks * (a.heads[p] + kRowCost) / (all + 2 * kRowCost);
+    if (most < 1) most = 1;
+    if (p == 1 && most + a.blocks[0] > kMaxBlocks) most = kMaxBlocks - a.blocks[0];
+    uint32_t per = a.heads[p];
+    while (per > at_once && (uint64_t)a.n * ((a.heads[p] + per - 1) / per) < most * kWarps)
+      per = (per + 1) / 2;
+    per = (per + at_once - 1) / at_once * at_once;
+    a.per_job[p] = per;
+    a.jobs_per_row[p] = (a.heads[p] + per - 1) / per;
+    const uint64_t blocks = ceil_div64((uint64_t)a.n * a.jobs_per_row[p], kWarps);
+    a.blocks[p] = (uint32_t)(blocks < most ? blocks : most);
+  }
 }
 
 int check_common(const char *what, int dtype, const QkArgs &a, int pairs) {
@@ -348,8 +389,8 @@ int check_common(const char *what, int dtype, const QkArgs &a, int pairs) {
   if (pairs != NL_PAIRS_HALF && pairs != NL_PAIRS_ADJACENT)
     return set_error(NL_ERROR, "%s: pairs %d", what, pairs);
   const uint32_t unit = dtype == NL_BF16 ? 16 : 8;
-  if (!a.heads || !a.kv_heads || a.heads > 65536 || a.kv_heads > 65536)
-    return set_error(NL_ERROR, "%s: heads %u, kv heads %u", what, a.heads, a.kv_heads);
+  if (!a.heads[0] || !a.heads[1] || a.heads[0] > 65536 || a.heads[1] > 65536)
+    return set_error(NL_ERROR, "%s: heads %u, kv heads %u", what, a.heads[0], a.heads[1]);
   if (!a.head_dim || a.head_dim > 256 || a.head_dim % unit || !a.rot || a.rot > a.head_dim ||
       a.rot % unit)
     return set_error(NL_ERROR,
@@ -392,7 +433,7 @@ extern "C" int nl_qk_norm_rope_dev(int dtype, const void *QKV, uint64_t x_stride
   QkArgs a = {};
   a.x = QKV; a.x_stride = x_stride; a.g[0] = GQ; a.g[1] = GK; a.co = CO; a.si = SI; a.pos = POS;
   a.out[0] = Q; a.out[1] = K; a.out_stride[0] = q_stride; a.out_stride[1] = k_stride;
-  a.n = n; a.heads = heads; a.kv_heads = kv_heads; a.head_dim = head_dim; a.rot = rot_dim;
+  a.n = n; a.heads[0] = heads; a.heads[1] = kv_heads; a.head_dim = head_dim; a.rot = rot_dim;
   a.rope_rows = rope_rows; a.eps = eps;
   if ((rc = check_common(what, dtype, a, pairs))) return rc;
   if (n == 0) return NL_OK;
@@ -402,16 +443,17 @@ extern "C" int nl_qk_norm_rope_dev(int dtype, const void *QKV, uint64_t x_stride
       (rc = check_rows(what, "K", dtype, K, k_stride, kw)) || (rc = check_tables(what, a)))
     return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  const uint32_t group = group_of(dtype, head_dim), blocks = divide(a, 32 / group);
+  const uint32_t group = group_of(dtype, head_dim);
+  divide(a, 32 / group);
   const bool half = pairs == NL_PAIRS_HALF;
-  const cudaError_t e = dtype == NL_BF16 ? start_t<__nv_bfloat16, false>(a, half, group, blocks, st)
-                                         : start_t<float, false>(a, half, group, blocks, st);
+  const cudaError_t e = dtype == NL_BF16 ? start_t<__nv_bfloat16, false>(a, half, group, st)
+                                         : start_t<float, false>(a, half, group, st);
   count_launches(1);
   return cuda_status(e, what);
 }
 
 extern "C" size_t nl_qk_norm_rope_bwd_workspace_bytes(uint32_t head_dim) {
-  return (size_t)kMaxBlocks * 2 * head_dim * sizeof(float);
+  return (size_t)kMaxBlocks * head_dim * sizeof(float);
 }
 
 extern "C" int nl_qk_norm_rope_bwd_dev(int dtype, const void *QKV, uint64_t x_stride,
@@ -430,12 +472,11 @@ extern "C" int nl_qk_norm_rope_bwd_dev(int dtype, const void *QKV, uint64_t x_st
   a.x = QKV; a.x_stride = x_stride; a.g[0] = GQ; a.g[1] = GK; a.co = CO; a.si = SI; a.pos = POS;
   a.dy[0] = DQ; a.dy[1] = DK; a.dy_stride[0] = dq_stride; a.dy_stride[1] = dk_stride;
   a.out_stride[0] = a.out_stride[1] = dx_stride;
-  a.n = n; a.heads = heads; a.kv_heads = kv_heads; a.head_dim = head_dim; a.rot = rot_dim;
+  a.n = n; a.heads[0] = heads; a.heads[1] = kv_heads; a.head_dim = head_dim; a.rot = rot_dim;
   a.rope_rows = rope_rows; a.eps = eps;
   if ((rc = check_common(what, dtype, a, pairs))) return rc;
   if (!DGQ || !DGK) return set_error(NL_ERROR, "%s: a null gain gradient", what);
   cudaStream_t st = (cudaStream_t)stream;
-  uint32_t blocks = 0;
   if (n) {
     const uint64_t qw = (uint64_t)heads * head_dim, kw = (uint64_t)kv_heads * head_dim;
     if ((rc = check_rows(what, "QKV", dtype, QKV, x_stride, qw + kw)) ||
@@ -454,16 +495,16 @@ extern "C" int nl_qk_norm_rope_bwd_dev(int dtype, const void *QKV, uint64_t x_st
     a.out[0] = DQKV;
     a.out[1] = (char *)DQKV + qw * (dtype == NL_BF16 ? 2 : 4);
     const uint32_t group = group_of(dtype, head_dim);
-    blocks = divide(a, 32 / group);
+    divide(a, 32 / group);
     const bool half = pairs == NL_PAIRS_HALF;
-    const cudaError_t e = dtype == NL_BF16
-                              ? start_t<__nv_bfloat16, true>(a, half, group, blocks, st)
-                              : start_t<float, true>(a, half, group, blocks, st);
+    const cudaError_t e = dtype == NL_BF16 ? start_t<__nv_bfloat16, true>(a, half, group, st)
+                                           : start_t<float, true>(a, half, group, st);
     count_launches(1);
     if (e != cudaSuccess) return cuda_status(e, what);
   }
-  const cudaError_t e = launch_pdl(qk_gain_sum_kernel, dim3(2 * head_dim / 8), dim3(256), 0, st,
-                                   (const float *)workspace, blocks, head_dim, DGQ, DGK);
+  const cudaError_t e = launch_pdl(qk_gain_sum_kernel, dim3(head_dim / 8, 2), dim3(256), 0, st,
+                                   (const float *)workspace, a.blocks[0], a.blocks[1], head_dim,
+                                   DGQ, DGK);
   count_launches(1);
   return cuda_status(e, what);
 }

@@ -38,6 +38,7 @@
 #include <cuda.h>
 
 #define NL_TREE_KERNELS
+#include "f32x2.cuh"
 #include "tree_work.cuh"
 
 namespace nl {
@@ -222,34 +223,6 @@ __device__ __forceinline__ void expand(uint32_t w, uint32_t *to) {
     to[2] = codes4_low(x);
     to[3] = codes4_high(x);
   }
-}
-
-// Two floats at a time.
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair(float x, float y) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(Pair v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
 }
 
 // The largest, or the sum, over a warp's lanes of each of 16 values: lanes i and
