@@ -431,22 +431,35 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
         while (w.next(a)) {
           const uint32_t keys = keys_of(a, w.b);
+          // the parameter words of this thread's key, and whether there is one:
+          // the block is looked up two tiles ahead, the words one
+          auto page_of = [&](uint32_t token) {
+            return a.block_shift < 32 ? token >> a.block_shift : token / a.pool.block_size;
+          };
+          auto block_of = [&](uint32_t tile) {
+            const uint32_t token = tile * kTileKeys + key;
+            if (tile >= w.t1 || token >= keys) return kNone;
+            return (uint32_t)__ldg(a.table + (uint64_t)w.b * a.max_blocks + page_of(token));
+          };
+          auto words_of = [&](uint32_t tile, uint32_t block) {
+            uint4 word = make_uint4(0, 0, 0, 0);
+            if (block < a.pool.num_blocks) {
+              const uint32_t token = tile * kTileKeys + key;
+              const uint32_t row =
+                  kv_row(a.pool, block, token - page_of(token) * a.pool.block_size, w.head);
+              word.x = __ldg(a.pool.param[0] + row);
+              word.y = __ldg(a.pool.param[1] + row);
+              word.z = 1;
+            }
+            return word;
+          };
+          uint4 next = words_of(w.t0, block_of(w.t0));
+          uint32_t block = block_of(w.t0 + 1);
           for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
             const uint32_t st = it % L::Stages, h = it & 1;
-            // the parameter words of this thread's key, and whether there is one
-            uint4 word = make_uint4(0, 0, 0, 0);
-            const uint32_t token = tile * kTileKeys + key;
-            if (token < keys) {
-              const uint32_t page =
-                  a.block_shift < 32 ? token >> a.block_shift : token / a.pool.block_size;
-              const uint32_t block = (uint32_t)__ldg(a.table + (uint64_t)w.b * a.max_blocks + page);
-              if (block < a.pool.num_blocks) {
-                const uint32_t row = kv_row(a.pool, block, token - page * a.pool.block_size, w.head);
-                word.x = __ldg(a.pool.param[0] + row);
-                word.y = __ldg(a.pool.param[1] + row);
-                word.z = 1;
-              }
-            }
+            const uint4 word = next;
+            next = words_of(tile + 1, block);
+            block = block_of(tile + 2);
             const uint8_t *kc = sm + st * (2 * L::Codes);
             bar_wait(full + 8 * st, it / L::Stages & 1, alive, err);
             bar_wait(qkdone + 8 * h, (it >> 1 & 1) ^ 1, alive, err);
@@ -864,7 +877,7 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
   }
   a.ctas = 148;
   a.tile = kTileKeys;
-  a.item_cost = 12;
+  a.item_cost = 7;
   int *err = wait_flag_device();
   if (!err) return cudaErrorMemoryAllocation;
   count_launches(1);
