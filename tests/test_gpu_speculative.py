@@ -607,6 +607,138 @@ def test_tree_attn_scales_far_apart(dev, torch, bits, name):
     check_tree(dev, torch, q, kv, table, lens, mask, bits, 2, 128, scale=0.25)
 
 
+# More than 16 rows a key head in bfloat16 take the tcgen05 form where the pages
+# are whole 16-key runs: 32 rows at a time up to 32, else 64.
+WIDE = [(8, 8, 2), (33, 2, 1), (64, 4, 1), (17, 3, 1)]      # nodes, heads, kv_heads
+
+
+@pytest.mark.parametrize("M,H,kvh", WIDE)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("bs,lens", [(16, [0, 300, 1, 126]), (48, [129, 0]), (256, [700]),
+                                     (5, [40, 130])])
+def test_wide_tree_attn(dev, torch, M, H, kvh, d, bits, bs, lens):
+    rng = np.random.default_rng(M + d + bits + bs)
+    masks = [chain(M) if b % 2 else tree(rng, M) for b in range(len(lens))]
+    masks[-1][M // 2:] = [0] * (M - M // 2)             # a sequence with unused nodes
+    masks[0][1] = 0
+    args = attn_inputs(torch, rng, len(lens), M, H, kvh, d, bits, bs, lens, masks, "bf16")
+    got, lse = check_tree(dev, torch, *args, bits, H, d)
+    assert not got[0, 1].any() and (lse[0, 1] == -np.inf).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("M,H", [(5, 4), (9, 8)])
+def test_wide_tree_attn_over_many_parts(dev, torch, bits, M, H):
+    rng = np.random.default_rng(30)
+    args = attn_inputs(torch, rng, 1, M, H, 1, 128, bits, 64, [40001], [tree(rng, M)], "bf16")
+    check_tree(dev, torch, *args, bits, H, 128)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("bad", [-1, 1 << 20])
+def test_wide_tree_attn_blocks_outside_the_pool(dev, torch, bits, bad):
+    rng = np.random.default_rng(31)
+    M = 20
+    q, kv, table, lens, mask = attn_inputs(torch, rng, 2, M, 2, 1, 64, bits, 16, [300, 40],
+                                           [chain(M)] * 2, "bf16")
+    table[0, [2, 9, 10]] = bad
+    table[1, :] = bad
+    got, lse = check_tree(dev, torch, q, kv, table, lens, mask, bits, 2, 64)
+    assert not got[1].any() and (lse[1] == -np.inf).all()
+    check_tree(dev, torch, q, kv, table[:, :3].copy(), lens, mask, bits, 2, 64)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("which", [1, 3])
+@pytest.mark.parametrize("M,H", [(20, 1), (20, 2)])
+def test_wide_tree_attn_nan_reaches_only_rows_that_see_it(dev, torch, bits, which, M, H):
+    rng = np.random.default_rng(32)
+    L = 140
+    m = [1 | 1 << i for i in range(M)]                  # all see node 0, else themselves
+    q, kv, table, lens, mask = attn_inputs(torch, rng, 1, M, H, 1, 128, bits, 16, [L], [m], "bf16")
+    t = L + 3
+    kv[which][table[0, t // 16], 0, t % 16] = 0x7fc00000 if bits == 8 else 0x7fc0
+    got, _ = check_tree(dev, torch, q, kv, table, lens, mask, bits, H, 128)
+    others = [i for i in range(M) if i != 3]
+    assert np.isnan(got[0, 3]).all() and np.isfinite(got[0, others]).all()
+    kv[which][table[0, 1], 0, 2] = 0x7fc00000 if bits == 8 else 0x7fc0    # a prefix key: all see it
+    got, _ = check_tree(dev, torch, q, kv, table, lens, mask, bits, H, 128)
+    assert np.isnan(got).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_wide_tree_attn_scales_far_apart(dev, torch, bits):
+    """Scores that keep rising from key to key, value scales from 2^-100 to
+    2^60, query rows from tiny to large: every way to move a reference."""
+    rng = np.random.default_rng(33)
+    M = 24
+    q, kv, table, lens, mask = attn_inputs(torch, rng, 1, M, 1, 1, 128, bits, 32, [900],
+                                           [chain(M)], "bf16")
+    flat = np.ones(kv[3].shape, np.float32)
+    for j, blk in enumerate(table[0]):
+        flat[blk] = 2.0 ** (-100 + 160 * j / (len(table[0]) - 1))
+    x = rng.standard_normal(kv[2].shape[:3] + (128,)).astype(np.float32) * flat[..., None]
+    code, word = quantise(x, bits)
+    kv[2], kv[3] = pack(code, bits), word
+    y = values(unpack(kv[0], bits), kv[1], bits)
+    for j, blk in enumerate(table[0]):                  # keys along one direction, longer and longer
+        y[blk] = y[blk] * 0.1 + np.float32(0.1 * j)
+    code, word = quantise(y, bits)
+    kv[0], kv[1] = pack(code, bits), word
+    rows = torch.logspace(-30, 1, M, device="cuda")
+    q.copy_((q.float().abs() * rows[:, None]).to(q.dtype))
+    check_tree(dev, torch, q, kv, table, lens, mask, bits, 1, 128, scale=0.25)
+
+
+def test_wide_tree_attn_rows_of_nan_and_infinity(dev, torch):
+    rng = np.random.default_rng(34)
+    M = 20
+    q, kv, table, lens, mask = attn_inputs(torch, rng, 1, M, 1, 1, 128, 8, 16, [200], [chain(M)],
+                                           "bf16")
+    q[1, 16 + 3] = float("nan")
+    q[2, 16 + 100] = float("inf")
+    cache, (tt, tl, tm) = device(torch, kv, table, lens, mask)
+    o = torch.empty(M, 128, device="cuda", dtype=q.dtype)
+    dev.tree_attn(q[:, 16:16 + 128], *cache, tt, tl, tm, o, 128)
+    assert o[1].isnan().all() and o[2].isnan().any()
+    assert o[0].isfinite().all() and o[3:].isfinite().all()
+    from nelisp_cuda import _lib as L
+    assert L.load().nl_wait_status() == L.NL_OK
+
+
+def test_wide_tree_attn_streams_and_graph(dev, torch):
+    rng = np.random.default_rng(35)
+    q, kv, table, lens, mask = attn_inputs(torch, rng, 3, 16, 8, 2, 128, 8, 16, [3000, 17, 900],
+                                           [chain(16)] * 3, "bf16")
+    cache, (tt, tl, tm) = device(torch, kv, table, lens, mask)
+    Q = q[:, :1024]
+    want = torch.empty(48, 1024, device="cuda", dtype=q.dtype)
+    dev.tree_attn(Q, *cache, tt, tl, tm, want, 128)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(want) for _ in range(8)]
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        dev.tree_attn(Q, *cache, tt, tl, tm, o, 128, stream=streams[i % 2])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    g, o = torch.cuda.CUDAGraph(), torch.zeros_like(want)
+    with torch.cuda.graph(g):
+        for _ in range(4):
+            dev.tree_attn(Q, *cache, tt, tl, tm, o, 128)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, want)
+    # the workspace that the query asks for is enough, to the byte
+    from nelisp_cuda import _lib as L
+    n = L.load().nl_tree_attn_workspace_bytes(16, 8, 2, 128)
+    ws = torch.full((n + 4096,), 7, dtype=torch.uint8, device="cuda")
+    o.zero_()
+    dev.tree_attn(Q, *cache, tt, tl, tm, o, 128, workspace=ws[:n])
+    assert torch.equal(o, want) and (ws[n:] == 7).all()
+
+
 def test_tree_attn_rows_of_nan_and_infinity(dev, torch):
     rng = np.random.default_rng(15)
     q, kv, table, lens, mask = attn_inputs(torch, rng, 1, 3, 2, 1, 128, 8, 16, [50], [chain(3)],
