@@ -250,11 +250,10 @@ struct Walk {
   uint32_t b, items;
   uint32_t head, row0, t0, t1, tiles;
   __device__ __forceinline__ bool begin(const TreeArgs &a) {
-    const uint64_t total = all_cost(a);
-    const uint32_t workers = total < a.ctas ? (uint32_t)total : a.ctas;
-    if (blockIdx.x >= workers) return false;
-    at = share(total, workers, blockIdx.x);
-    end = share(total, workers, blockIdx.x + 1);
+    const List list = list_of(a);
+    if (blockIdx.x >= list.workers) return false;
+    at = share(list.total, list.workers, blockIdx.x);
+    end = share(list.total, list.workers, blockIdx.x + 1);
     items = a.pool.kv_heads * a.row_tiles;
     locate(a, at, &b, &before);
     return true;
@@ -337,8 +336,8 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();                 // after the wait: the join reads the lengths before its own
 
   bool alive = true;
   Walk w;

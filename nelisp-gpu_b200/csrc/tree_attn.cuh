@@ -127,12 +127,13 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   uint8_t *ring = qf + P::Q;
   float *join = reinterpret_cast<float *>(qf);
 
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();                 // after the wait: the join reads the lengths before its own
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t wr = warp % WR, wk = warp / WR;
-  const uint64_t total = all_cost(a);
-  const uint32_t workers = total < a.ctas ? (uint32_t)total : a.ctas;
+  const List list = list_of(a);
+  const uint64_t total = list.total;
+  const uint32_t workers = list.workers;
   if (blockIdx.x >= workers) return;
   uint64_t at = share(total, workers, blockIdx.x);
   const uint64_t end = share(total, workers, blockIdx.x + 1);
@@ -602,12 +603,19 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kTreeThreads)
 tree_join_kernel(const __grid_constant__ TreeArgs a) {
   pdl_trigger();
-  pdl_wait();
   __shared__ float red[kTreeWarps][HD + 2];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint64_t total = all_cost(a);
-  const uint32_t workers = total < a.ctas ? (uint32_t)total : a.ctas, cut = blockIdx.x + 1;
-  if (cut >= workers) return;
+  // Whatever wrote the lengths is done: the attention kernel lets this one start
+  // once it has waited for that itself.
+  const List list = list_of(a);
+  const uint64_t total = list.total;
+  const uint32_t workers = list.workers, cut = blockIdx.x + 1;
+  // (Every block waits, also where it has nothing to join: once this grid is
+  // done, whatever follows it takes the attention kernel to be done.)
+  if (cut >= workers) {
+    pdl_wait();
+    return;
+  }
   const uint64_t at = share(total, workers, cut);
   uint32_t b;
   uint64_t before;
@@ -615,10 +623,12 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
   const uint32_t tiles = tiles_of(a, b), cost = tiles + a.item_cost;
   const uint32_t off = (uint32_t)((at - before) % cost), item = (uint32_t)((at - before) / cost);
   const uint64_t s0 = at - off + a.item_cost;     // the item's first tile
-  if (off <= a.item_cost || share(total, workers, cut - 1) > s0) return;
+  const bool cuts = off > a.item_cost && share(total, workers, cut - 1) <= s0;
   const uint32_t c0 = cut - 1, c1 = owner(total, workers, s0 + tiles - 1);
   const uint32_t head = item / a.row_tiles, row0 = item % a.row_tiles * a.rows_at_once;
   constexpr int Per = HD / 32;
+  pdl_wait();
+  if (!cuts) return;
   const bool alone = c1 - c0 < 32;                // a warp per row
   for (uint32_t r = alone ? warp : 0; r < 4; r += alone ? 4 : 1) {
     const uint32_t here = blockIdx.y * 4 + r, row = row0 + here;

@@ -69,12 +69,36 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// The length of the list: an item counts its tiles and its own cost.
-__device__ __forceinline__ uint64_t all_cost(const TreeArgs &a) {
+// The list's length -- an item counts its tiles and its own cost -- and the CTAs
+// it is divided among.  Where all sequences are equally long, a number of CTAs
+// that the items divide evenly gives every CTA a part of one item only (8 x 32
+// items of 33 tiles on 256 of 296 CTAs instead of one and a part of another
+// each); it is taken if it leaves no more than 15% of the CTAs without work.
+struct List {
+  uint64_t total;
+  uint32_t workers;
+};
+__device__ __forceinline__ List list_of(const TreeArgs &a) {
   const uint32_t lane = threadIdx.x & 31;
-  uint64_t v = 0;
-  for (uint32_t b = lane; b < a.batch; b += 32) v += tiles_of(a, b) + a.item_cost;
-  return warp_sum(v) * (a.pool.kv_heads * a.row_tiles);
+  uint64_t sum = 0;
+  uint32_t least = ~0u, most = 0;
+  for (uint32_t b = lane; b < a.batch; b += 32) {
+    const uint32_t t = tiles_of(a, b);
+    sum += t + a.item_cost;
+    least = min(least, t);
+    most = max(most, t);
+  }
+  List l;
+  const uint32_t items = a.pool.kv_heads * a.row_tiles;
+  l.total = warp_sum(sum) * items;
+  l.workers = l.total < a.ctas ? (uint32_t)l.total : a.ctas;
+  const uint64_t all = (uint64_t)items * a.batch;
+  if (__reduce_min_sync(0xffffffffu, least) == __reduce_max_sync(0xffffffffu, most) &&
+      all <= l.workers) {
+    const uint32_t even = l.workers / (uint32_t)all * (uint32_t)all;
+    if (even * 20 >= l.workers * 17) l.workers = even;
+  }
+  return l;
 }
 // The sequence that place AT of the list falls into, and the places before it.
 __device__ __forceinline__ void locate(const TreeArgs &a, uint64_t at, uint32_t *b_out,
