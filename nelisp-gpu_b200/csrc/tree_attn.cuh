@@ -89,9 +89,11 @@ template <int HD, int BITS> struct Geo {
   }
 };
 
-template <typename T, int HD, int BITS, int NR, int WR> struct Plan {
+template <typename T, int HD, int BITS, int NR, int WR, bool PACK> struct Plan {
   using G = Geo<HD, BITS>;
-  static constexpr int Terms = sizeof(T) == 4 ? 2 : 1;
+  // PACK: at most four rows, whose two terms are columns r and r + 4 of one
+  // tile instead of two products.
+  static constexpr int Terms = sizeof(T) == 4 && !PACK ? 2 : 1;
   static constexpr int WK = kTreeWarps / WR;                // warps with keys of their own
   static constexpr int Rows = 8 * NR * WR, Tile = kTreeKeys * WK;
   static constexpr int Q = Terms * Rows * HD * 2;           // query fragments
@@ -112,12 +114,14 @@ template <> __device__ __forceinline__ float load1<__nv_bfloat16>(const __nv_bfl
 __device__ __forceinline__ void store1(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <typename T, int HD, int BITS, int NR, int WR>
+template <typename T, int HD, int BITS, int NR, int WR, bool PACK>
 __global__ void __launch_bounds__(kTreeThreads)
 tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   using G = Geo<HD, BITS>;
-  using P = Plan<T, HD, BITS, NR, WR>;
+  using P = Plan<T, HD, BITS, NR, WR, PACK>;
   constexpr int Terms = P::Terms, WK = P::WK, Stages = P::Stages;
+  constexpr bool Flush = sizeof(T) == 4;         // each 16 keys summed apart
+  constexpr uint32_t Live = PACK ? 4 : P::Rows;  // rows of an item
   extern __shared__ __align__(16) uint8_t smem[];
   float *row_f = reinterpret_cast<float *>(smem);                    // factor of a row's scores
   float *row_sum = row_f + P::Rows;                                  // sum of its query
@@ -164,7 +168,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
     at += c1 - c0;
     if (c1 <= a.item_cost) continue;             // its share ends before the first tile
     const uint32_t t0 = c0 > a.item_cost ? c0 - a.item_cost : 0, t1 = c1 - a.item_cost;
-    const uint32_t head = item / a.row_tiles, row0 = item % a.row_tiles * P::Rows;
+    const uint32_t head = item / a.row_tiles, row0 = item % a.row_tiles * Live;
     const uint32_t prefix = prefix_of(a, b), keys = keys_of(a, b);
 
     // ---- keys on their way ----
@@ -209,9 +213,11 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
     }
 
     // ---- the query rows, as operand fragments: 8 threads a row ----
-    for (uint32_t r = threadIdx.x / 8; r < P::Rows; r += kTreeThreads / 8) {
+    // (threads past the rows go through with the first: the shuffles are whole)
+    for (uint32_t i0 = threadIdx.x / 8; i0 < P::Rows || i0 < kTreeThreads / 8;
+         i0 += kTreeThreads / 8) {
       constexpr int Per = HD / 8;
-      const uint32_t part = threadIdx.x % 8, row = row0 + r;
+      const uint32_t r = i0 < Live ? i0 : 0, part = threadIdx.x % 8, row = row0 + r;
       const bool live = row < a.rows;
       const uint32_t node = live ? row / a.group : 0;
       const T *q = (const T *)a.q + ((uint64_t)b * a.nodes + node) * a.q_stride +
@@ -237,18 +243,24 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
         G::spot(part * Per + i, &step, &quad, &p, &half);
         const uint32_t byte = fragment(r, step, quad) + p * 4 + half * 2;
         const __half hi = __float2half_rn(v[i]);
+        const __half low = __float2half_rn(v[i] - __half2float(hi));
         *reinterpret_cast<__half *>(qf + byte) = hi;
-        if (Terms == 2)
-          *reinterpret_cast<__half *>(qf + P::Rows * HD * 2 + byte) =
-              __float2half_rn(v[i] - __half2float(hi));
+        if (Terms == 2) *reinterpret_cast<__half *>(qf + P::Rows * HD * 2 + byte) = low;
+        if (PACK)
+          *reinterpret_cast<__half *>(qf + fragment(r + 4, step, quad) + p * 4 + half * 2) = low;
       }
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (part == 0) {
-        // never zero: a factor of zero would make NaN of a masked score
-        row_f[r] = fmaxf(a.scale * __uint_as_float((uint32_t)(127 - up) << 23), 1.17549435e-38f);
-        row_sum[r] = sum;
-        row_mask[r] = live ? a.mask[(uint64_t)b * a.nodes + node] & used : 0;
+        const uint64_t mask = live ? a.mask[(uint64_t)b * a.nodes + node] & used : 0;
+#pragma unroll
+        for (uint32_t c = r; c < P::Rows; c += PACK ? 4 : P::Rows) {
+          // never zero: a factor of zero would make NaN of a masked score
+          row_f[c] = fmaxf(a.scale * __uint_as_float((uint32_t)(127 - up) << 23),
+                           1.17549435e-38f);
+          row_sum[c] = sum;
+          row_mask[c] = mask;
+        }
       }
     }
     __syncthreads();
@@ -346,6 +358,13 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
             }
           }
         }
+      }
+
+      if (PACK) {                  // the other term's column is two lanes on
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[k][0][i] += __shfl_xor_sync(0xffffffffu, s[k][0][i], 2);
       }
 
       // scales, offsets and masks: s becomes the score over the row's factor
@@ -458,7 +477,11 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
               if (BITS == 4 && seen) base[n][r] = fmaf(e[r], mid[u], base[n][r]);
               e[r] = seen ? e[r] * sc[u] : 0.0f;
             }
-            const __half2 hi = __floats2half2_rn(e[0], e[1]);
+            __half2 hi = __floats2half2_rn(e[0], e[1]);
+            if (PACK) {
+              const __half2 low = __floats2half2_rn(e[0] - __low2float(hi), e[1] - __high2float(hi));
+              if (t & 2) hi = low;
+            }
             p[0][n][u] = transpose8(h2(hi));
             if (Terms == 2)
               p[Terms - 1][n][u] = transpose8(
@@ -497,7 +520,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
                                            codes8(cd, 0x4140), codes8(cd, 0x4342));
 #pragma unroll
                 for (int n = 0; n < NR; n++)
-                  weigh<Terms, NR>(o[2 * (VL * h + j) + u][n], c, p, n);
+                  weigh<Terms, NR, Flush>(o[2 * (VL * h + j) + u][n], c, p, n);
               }
             } else {
 #pragma unroll
@@ -510,7 +533,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
                                            codes4_high(cd));
 #pragma unroll
                 for (int n = 0; n < NR; n++)
-                  weigh<Terms, NR>(o[4 * (VL * h + j) + u][n], c, p, n);
+                  weigh<Terms, NR, Flush>(o[4 * (VL * h + j) + u][n], c, p, n);
               }
             }
           }
@@ -541,15 +564,15 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
 #pragma unroll
         for (int r = 0; r < 2; r++) {
           float *to = join + (wk * P::Rows + r0 + 8 * n + r) * P::Pitch;
+          const float add = PACK && (t & 2) ? 0.0f : base[n][r];
 #pragma unroll
           for (int i = 0; i < G::MT; i++)
             *reinterpret_cast<float2 *>(to + G::column(g, 2 * i)) =
-                make_float2(fmaf(o[i][n][r], back, base[n][r]),
-                            fmaf(o[i][n][2 + r], back, base[n][r]));
+                make_float2(fmaf(o[i][n][r], back, add), fmaf(o[i][n][2 + r], back, add));
         }
     }
     __syncthreads();
-    for (uint32_t r = threadIdx.x / 8; r < P::Rows; r += kTreeThreads / 8) {
+    for (uint32_t r = threadIdx.x / 8; r < Live; r += kTreeThreads / 8) {
       constexpr int Per = HD / 8;
       const uint32_t part = threadIdx.x % 8, row = row0 + r;
       float top = -INFINITY, sum = 0.0f, c[WK];
@@ -575,7 +598,10 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < WK; w++)
-          v = c[w] == 0.0f ? v : fmaf(c[w], join[(w * P::Rows + r) * P::Pitch + d], v);
+          if (c[w] != 0.0f) {
+            const float *x = join + (w * P::Rows + r) * P::Pitch + d;
+            v = fmaf(c[w], PACK ? x[0] + x[4 * P::Pitch] : x[0], v);
+          }
         if (part_of) {
           a.part_o[((uint64_t)slot * P::Rows + r) * HD + d] = v;
         } else if (row < a.rows) {
@@ -713,16 +739,16 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
   }
 }
 
-template <typename T, int HD, int BITS, int NR, int WR>
+template <typename T, int HD, int BITS, int NR, int WR, bool PACK = false>
 cudaError_t start(TreeArgs &a, cudaStream_t st) {
-  using P = Plan<T, HD, BITS, NR, WR>;
+  using P = Plan<T, HD, BITS, NR, WR, PACK>;
   static int per_sm = 0;
   if (!per_sm) {
-    cudaError_t e = cudaFuncSetAttribute(tree_attn_kernel<T, HD, BITS, NR, WR>,
+    cudaError_t e = cudaFuncSetAttribute(tree_attn_kernel<T, HD, BITS, NR, WR, PACK>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, P::Bytes);
     if (e != cudaSuccess) return e;
     int n = 0;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, tree_attn_kernel<T, HD, BITS, NR, WR>,
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, tree_attn_kernel<T, HD, BITS, NR, WR, PACK>,
                                                       kTreeThreads, P::Bytes);
     if (e != cudaSuccess) return e;
     per_sm = n < 1 ? 1 : n > 4 ? 4 : n;
@@ -730,7 +756,7 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
   a.ctas = 148u * per_sm;
   a.tile = P::Tile;
   a.item_cost = 4 * WR;          // about 512 keys
-  cudaError_t e = launch_pdl(tree_attn_kernel<T, HD, BITS, NR, WR>, dim3(a.ctas),
+  cudaError_t e = launch_pdl(tree_attn_kernel<T, HD, BITS, NR, WR, PACK>, dim3(a.ctas),
                              dim3(kTreeThreads), (size_t)P::Bytes, st, a);
   count_launches(1);
   return e;
@@ -738,6 +764,9 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
 template <typename T, int HD, int BITS>
 cudaError_t start_rows(TreeArgs &a, cudaStream_t st) {
   constexpr int Most = HD == 256 ? 2 : 4;        // row tiles a warp has registers for
+  if constexpr (sizeof(T) == 4) {
+    if (a.rows <= 4) return start<T, HD, BITS, 1, 1, true>(a, st);
+  }
   if (a.rows_at_once == 8) return start<T, HD, BITS, 1, 1>(a, st);
   if (a.rows_at_once == 16) return start<T, HD, BITS, 2, 1>(a, st);
   if (a.rows_at_once == 32) return start<T, HD, BITS, Most, 4 / Most>(a, st);

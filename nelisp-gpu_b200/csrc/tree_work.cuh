@@ -182,10 +182,10 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 // o += codes x weights.  The tensor core cuts, not rounds, what it adds to an
 // accumulator, and over a long context that drifts; where the output is
 // float32 each 16 keys are summed apart and added in float32.
-template <int Terms, int NR>
+template <int Terms, int NR, bool Flush>
 __device__ __forceinline__ void weigh(float (&o)[4], const uint4 &c,
                                       const uint32_t (&p)[Terms][NR][2], int n) {
-  if (Terms == 1) {
+  if (!Flush) {
     mma16(o, c, p[0][n][0], p[0][n][1]);
   } else {
     float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
