@@ -54,7 +54,8 @@ template <int HD, int BITS, int N> struct Plan {
   static constexpr int Soft = 128 * Groups;                   // threads of the score warps
   static constexpr int Threads = Soft + 3 * 128;
   static constexpr int Regs = 65536 / Threads / 8 * 8;        // a thread, at launch
-  static constexpr int RegsSoft = (Regs * (Groups + 3) - 56 - 56 - 40) / Groups / 8 * 8;
+  static constexpr int RegsCtl = N == 32 ? 64 : 40;           // with 7 groups there are no more
+  static constexpr int RegsSoft = (Regs * (Groups + 3) - 56 - 56 - RegsCtl) / Groups / 8 * 8;
   static constexpr int RB = HD * BITS / 8;
   static constexpr int Chunks = RB / 16;
   static constexpr int Codes = kTileKeys * RB;               // one side's codes of a tile
@@ -315,15 +316,13 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
       bar_init(empty + 8 * i, 8);
     }
     for (int i = 0; i < 2; i++) {
+      bar_init(kready + 8 * i, 4);
       bar_init(qkdone + 8 * i, 1);
       bar_init(sfree + 8 * i, 4 * L::Groups);
       bar_init(vready + 8 * i, 4);
       bar_init(pready + 8 * i, 4 * L::Groups);
       bar_init(pvdone + 8 * i, 1);
     }
-    // four: a score warp may come to wait for a tile's keys when those two
-    // tiles on are ready too, and a phase must not be taken for the next
-    for (int i = 0; i < 4; i++) bar_init(kready + 8 * i, 4);
     bar_init(qready, 4 * L::Groups);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -344,7 +343,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
   if (w.begin(a)) {
     uint32_t it = 0;                         // tiles so far, over all items
     if (role == 3) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(L::RegsCtl));
       if (warp % 4 == 0) {
         // ---- TMA of the codes: a run of BOX keys of a page at a time, one lane each ----
         const uint32_t runs = kTileKeys / box;
@@ -385,7 +384,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           item++;
           for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
             const uint32_t st = it & 1, ph = it >> 1 & 1;
-            bar_wait(kready + 8 * (it & 3), it >> 2 & 1, alive, err);
+            bar_wait(kready + 8 * st, ph, alive, err);
             bar_wait(sfree + 8 * st, ph ^ 1, alive, err);
             fence_after();
             const uint64_t q = smem_desc(s0 + L::Q, 16);
@@ -484,7 +483,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             fence_before();
             __syncwarp();
             if (lane == 0) {
-              bar_arrive(kready + 8 * (it & 3));
+              bar_arrive(kready + 8 * h);
               bar_arrive(empty + 8 * st);
             }
           }
@@ -608,7 +607,9 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
 
         for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
           const uint32_t st = it & 1, ph = it >> 1 & 1;
-          bar_wait(kready + 8 * (it & 3), it >> 2 & 1, alive, err);
+          // (the key warps' words came before the barrier that the product waited for)
+          bar_wait(qkdone + 8 * st, ph, alive, err);
+          fence_after();
           const uint4 word = words[(it & 3) * kTileKeys + mykey];
           const uint32_t kw = word.x, vw = word.y;
           const bool have = word.z != 0;
@@ -654,8 +655,6 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
               }
             }
           };
-          bar_wait(qkdone + 8 * st, ph, alive, err);
-          fence_after();
           const uint32_t ts = tmem + (quad << 16) + L::TS + st * N + n0;
           uint32_t s[H];
           for (bool again = false;; again = true) {
