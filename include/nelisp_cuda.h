@@ -334,6 +334,9 @@ int nl_ternary_gemv_static_dev(const float *X, const uint32_t *WP,
 #define NL_PAIRS_HALF 0
 #define NL_PAIRS_ADJACENT 1
 
+/* The entry points below take their arguments in one structure (a field left
+ * zero is a null pointer or an absent option) and a cudaStream_t. */
+
 /* RMS norm of every query and key head and the position rotation, in one
  * pass.  QKV holds N rows, X_STRIDE elements apart, that begin with
  * [heads*head_dim q | kv_heads*head_dim k] (what follows, the values, is not
@@ -347,14 +350,20 @@ int nl_ternary_gemv_static_dev(const float *X, const uint32_t *WP,
  * and K may be the rows of QKV themselves.  Sums are f32 whatever DTYPE.
  * Rows are 16-byte aligned; head_dim (at most 256) and rot_dim are multiples
  * of 8 (f32) or 16 (bf16).  Does not synchronise. */
-int nl_qk_norm_rope_dev(int dtype, const void *QKV, uint64_t x_stride,
-                        const float *GQ, const float *GK, const float *CO,
-                        const float *SI, const int32_t *POS, void *Q,
-                        uint64_t q_stride, void *K, uint64_t k_stride,
-                        uint32_t n, uint32_t heads, uint32_t kv_heads,
-                        uint32_t head_dim, uint32_t rot_dim,
-                        uint32_t rope_rows, int pairs, float eps,
-                        void *stream);
+typedef struct {
+  int dtype, pairs;              /* NL_F32 / NL_BF16; NL_PAIRS_* */
+  const void *qkv;
+  uint64_t x_stride;
+  const float *gq, *gk, *co, *si;
+  const int32_t *pos;
+  void *q;
+  uint64_t q_stride;
+  void *k;
+  uint64_t k_stride;
+  uint32_t n, heads, kv_heads, head_dim, rot_dim, rope_rows;
+  float eps;
+} nl_qk_norm_rope_args;
+int nl_qk_norm_rope_dev(const nl_qk_norm_rope_args *args, void *stream);
 
 /* Its backward pass: from the saved QKV rows and the gradients DQ and DK of
  * the two outputs, the gradient of the q and k part of the rows (DQKV rows,
@@ -364,20 +373,29 @@ int nl_qk_norm_rope_dev(int dtype, const void *QKV, uint64_t x_stride,
  * nl_qk_norm_rope_bwd_workspace_bytes(head_dim) bytes, 16-byte aligned, or is
  * NULL for the library's own (calls that overlap in time must then not
  * share it).  Does not synchronise. */
+typedef struct {
+  int dtype, pairs;
+  const void *qkv;
+  uint64_t x_stride;
+  const float *gq, *gk, *co, *si;
+  const int32_t *pos;
+  const void *dq;
+  uint64_t dq_stride;
+  const void *dk;
+  uint64_t dk_stride;
+  void *dqkv;
+  uint64_t dx_stride;
+  float *dgq, *dgk;
+  uint32_t n, heads, kv_heads, head_dim, rot_dim, rope_rows;
+  float eps;
+  void *workspace;
+  size_t ws_bytes;
+} nl_qk_norm_rope_bwd_args;
 size_t nl_qk_norm_rope_bwd_workspace_bytes(uint32_t head_dim);
-int nl_qk_norm_rope_bwd_dev(int dtype, const void *QKV, uint64_t x_stride,
-                            const float *GQ, const float *GK, const float *CO,
-                            const float *SI, const int32_t *POS,
-                            const void *DQ, uint64_t dq_stride, const void *DK,
-                            uint64_t dk_stride, void *DQKV, uint64_t dx_stride,
-                            float *DGQ, float *DGK, uint32_t n, uint32_t heads,
-                            uint32_t kv_heads, uint32_t head_dim,
-                            uint32_t rot_dim, uint32_t rope_rows, int pairs,
-                            float eps, void *workspace, size_t ws_bytes,
-                            void *stream);
+int nl_qk_norm_rope_bwd_dev(const nl_qk_norm_rope_bwd_args *args, void *stream);
 
-/* Formats of the quantised paged KV cache.  A cache is four device arrays,
- * for the keys and for the values
+/* A quantised paged KV cache: four device arrays, for the keys and for the
+ * values
  *   codes  bytes [num_blocks][kv_heads][block_size][head_dim * bits / 8]
  *   params words [num_blocks][kv_heads][block_size]
  * (codes 16-byte aligned), and token slot s is offset s % block_size of block
@@ -394,25 +412,34 @@ int nl_qk_norm_rope_bwd_dev(int dtype, const void *QKV, uint64_t x_stride,
  * block_size fits uint32. */
 #define NL_KV_I4 4
 #define NL_KV_I8 8
+typedef struct {
+  int fmt;                       /* NL_KV_I8 or NL_KV_I4 */
+  uint32_t kv_heads, head_dim, block_size, num_blocks;
+  void *kc;
+  uint32_t *kp;
+  void *vc;
+  uint32_t *vp;
+} nl_kv_cache;
 
-/* Quantise N tokens' keys and values (rows of kv_heads*head_dim elements,
- * 16-byte aligned, K_STRIDE and V_STRIDE apart) into slots SLOT[i].  A slot
- * outside the pool is skipped; of tokens with the same slot one is kept, its
- * key and value heads not necessarily of the same token.  Does not
- * synchronise. */
-int nl_kv_append_dev(int fmt, int dtype, const void *K, uint64_t k_stride,
-                     const void *V, uint64_t v_stride, const int32_t *SLOT,
-                     void *KC, uint32_t *KP, void *VC, uint32_t *VP,
-                     uint32_t n, uint32_t kv_heads, uint32_t head_dim,
-                     uint32_t block_size, uint32_t num_blocks, void *stream);
-
-/* Read the slots back as values: rows of K and V.  A slot outside the pool
- * reads as zeros.  Does not synchronise. */
-int nl_kv_read_dev(int fmt, int dtype, const int32_t *SLOT, const void *KC,
-                   const uint32_t *KP, const void *VC, const uint32_t *VP,
-                   void *K, uint64_t k_stride, void *V, uint64_t v_stride,
-                   uint32_t n, uint32_t kv_heads, uint32_t head_dim,
-                   uint32_t block_size, uint32_t num_blocks, void *stream);
+/* nl_kv_append_dev quantises N tokens' keys and values (rows of
+ * kv_heads*head_dim elements of DTYPE, 16-byte aligned, K_STRIDE and V_STRIDE
+ * apart) into slots SLOT[i].  A slot outside the pool is skipped; of tokens
+ * with the same slot one is kept, its key and value heads not necessarily of
+ * the same token.  nl_kv_read_dev reads the slots back as values into the
+ * rows of K and V; a slot outside the pool reads as zeros.  Neither
+ * synchronises. */
+typedef struct {
+  nl_kv_cache cache;
+  int dtype;
+  uint32_t n;
+  const int32_t *slot;
+  void *k;                       /* read by the append, written by the read */
+  uint64_t k_stride;
+  void *v;
+  uint64_t v_stride;
+} nl_kv_rows_args;
+int nl_kv_append_dev(const nl_kv_rows_args *args, void *stream);
+int nl_kv_read_dev(const nl_kv_rows_args *args, void *stream);
 
 /* Move tokens inside the pool without requantising them, e.g. the accepted
  * path of a draft tree to the end of its prefix: for each of BATCH sequences
@@ -420,10 +447,12 @@ int nl_kv_read_dev(int fmt, int dtype, const int32_t *SLOT, const void *KC,
  * a sequence are read before any of its destinations is written; a pair with
  * a slot outside the pool is skipped; different sequences must not share
  * slots.  Does not synchronise. */
-int nl_kv_move_dev(int fmt, const int32_t *SRC, const int32_t *DST, void *KC,
-                   uint32_t *KP, void *VC, uint32_t *VP, uint32_t batch,
-                   uint32_t count, uint32_t kv_heads, uint32_t head_dim,
-                   uint32_t block_size, uint32_t num_blocks, void *stream);
+typedef struct {
+  nl_kv_cache cache;
+  const int32_t *src, *dst;
+  uint32_t batch, count;
+} nl_kv_move_args;
+int nl_kv_move_dev(const nl_kv_move_args *args, void *stream);
 
 /* Attention of a tree of NODES (at most 64) drafted tokens per sequence over
  * the quantised cache; NODES 1 is an ordinary decode step.  Sequence b has
@@ -442,18 +471,27 @@ int nl_kv_move_dev(int fmt, const int32_t *SRC, const int32_t *DST, void *KC,
  * are exact in the codes and sums f32.  WORKSPACE holds at least
  * nl_tree_attn_workspace_bytes(nodes, heads, kv_heads, head_dim) bytes,
  * 16-byte aligned, or is NULL for the library's own (calls that overlap in
- * time must then not share it).  Does not synchronise. */
+ * time must then not share it).  Does not synchronise; with bf16 and more
+ * than 16 rows (nodes x heads/kv_heads) it may wait on mbarriers (see
+ * nl_wait_status). */
+typedef struct {
+  nl_kv_cache cache;             /* its arrays are only read */
+  int dtype;
+  uint32_t batch, nodes, heads, max_blocks;
+  float scale;
+  const void *q;
+  uint64_t q_stride;
+  const int32_t *table, *len;
+  const uint64_t *mask;
+  void *o;
+  uint64_t o_stride;
+  float *lse;
+  void *workspace;
+  size_t ws_bytes;
+} nl_tree_attn_args;
 size_t nl_tree_attn_workspace_bytes(uint32_t nodes, uint32_t heads,
                                     uint32_t kv_heads, uint32_t head_dim);
-int nl_tree_attn_dev(int fmt, int dtype, const void *Q, uint64_t q_stride,
-                     const void *KC, const uint32_t *KP, const void *VC,
-                     const uint32_t *VP, const int32_t *TABLE,
-                     const int32_t *LEN, const uint64_t *MASK, void *O,
-                     uint64_t o_stride, float *LSE, uint32_t batch,
-                     uint32_t nodes, uint32_t heads, uint32_t kv_heads,
-                     uint32_t head_dim, uint32_t block_size,
-                     uint32_t num_blocks, uint32_t max_blocks, float scale,
-                     void *workspace, size_t ws_bytes, void *stream);
+int nl_tree_attn_dev(const nl_tree_attn_args *args, void *stream);
 
 /* ---- the ternary decoder (tensor-parallel) --------------------------- */
 

@@ -303,7 +303,8 @@ kv_read_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPool 
 // Rows moved inside the pool, one block per (sequence, head): every source is
 // in shared memory before the first destination is written.
 __global__ void __launch_bounds__(kThreads)
-kv_move_kernel(const __grid_constant__ KvPool p, const int32_t *src, const int32_t *dst, uint32_t count) {
+kv_move_kernel(const __grid_constant__ KvPool p, const int32_t *src, const int32_t *dst,
+               uint32_t count) {
   extern __shared__ uint4 held[];
   pdl_trigger();
   pdl_wait();
@@ -364,14 +365,18 @@ cudaError_t start_t(bool append, KvRows &r, const KvPool &p, cudaStream_t st) {
   }
 }
 
-int rows_call(const char *what, bool append, int fmt, int dtype, KvRows &r, KvPool &p, uint32_t n,
-              void *stream) {
+int rows_call(const char *what, bool append, const nl_kv_rows_args *args, void *stream) {
   int rc = api_ready();
   if (rc) return rc;
+  if (!args) return set_error(NL_ERROR, "%s: null arguments", what);
+  const int dtype = args->dtype, fmt = args->cache.fmt;
+  const uint32_t n = args->n;
+  KvPool p = kv_pool_of(args->cache);
+  KvRows r = {{args->k, args->v}, {args->k, args->v}, {args->k_stride, args->v_stride},
+              args->slot, 0, 0, 0};
   if (dtype != NL_F32 && dtype != NL_BF16)
     return set_error(NL_ERROR, "%s: type %d is neither NL_F32 nor NL_BF16", what, dtype);
   if ((rc = kv_check_pool(what, fmt, p))) return rc;
-  p.bits = (uint32_t)fmt;
   if (n == 0) return NL_OK;
   if (!r.slot) return set_error(NL_ERROR, "%s: null slots", what);
   const uint32_t unit = dtype == NL_BF16 ? 8 : 4;
@@ -397,47 +402,29 @@ int rows_call(const char *what, bool append, int fmt, int dtype, KvRows &r, KvPo
 
 using namespace nl;
 
-extern "C" int nl_kv_append_dev(int fmt, int dtype, const void *K, uint64_t k_stride,
-                                const void *V, uint64_t v_stride, const int32_t *SLOT, void *KC,
-                                uint32_t *KP, void *VC, uint32_t *VP, uint32_t n,
-                                uint32_t kv_heads, uint32_t head_dim, uint32_t block_size,
-                                uint32_t num_blocks, void *stream) {
-  KvRows r = {{K, V}, {nullptr, nullptr}, {k_stride, v_stride}, SLOT, 0, 0, 0};
-  KvPool p = {{(uint8_t *)KC, (uint8_t *)VC}, {KP, VP}, num_blocks, block_size, kv_heads,
-              head_dim, 0};
-  return rows_call("kv-append", true, fmt, dtype, r, p, n, stream);
+extern "C" int nl_kv_append_dev(const nl_kv_rows_args *args, void *stream) {
+  return rows_call("kv-append", true, args, stream);
 }
 
-extern "C" int nl_kv_read_dev(int fmt, int dtype, const int32_t *SLOT, const void *KC,
-                              const uint32_t *KP, const void *VC, const uint32_t *VP, void *K,
-                              uint64_t k_stride, void *V, uint64_t v_stride, uint32_t n,
-                              uint32_t kv_heads, uint32_t head_dim, uint32_t block_size,
-                              uint32_t num_blocks, void *stream) {
-  KvRows r = {{nullptr, nullptr}, {K, V}, {k_stride, v_stride}, SLOT, 0, 0, 0};
-  KvPool p = {{(uint8_t *)const_cast<void *>(KC), (uint8_t *)const_cast<void *>(VC)},
-              {const_cast<uint32_t *>(KP), const_cast<uint32_t *>(VP)}, num_blocks, block_size,
-              kv_heads, head_dim, 0};
-  return rows_call("kv-read", false, fmt, dtype, r, p, n, stream);
+extern "C" int nl_kv_read_dev(const nl_kv_rows_args *args, void *stream) {
+  return rows_call("kv-read", false, args, stream);
 }
 
-extern "C" int nl_kv_move_dev(int fmt, const int32_t *SRC, const int32_t *DST, void *KC,
-                              uint32_t *KP, void *VC, uint32_t *VP, uint32_t batch,
-                              uint32_t count, uint32_t kv_heads, uint32_t head_dim,
-                              uint32_t block_size, uint32_t num_blocks, void *stream) {
+extern "C" int nl_kv_move_dev(const nl_kv_move_args *args, void *stream) {
   int rc = api_ready();
   if (rc) return rc;
-  KvPool p = {{(uint8_t *)KC, (uint8_t *)VC}, {KP, VP}, num_blocks, block_size, kv_heads,
-              head_dim, 0};
-  if ((rc = kv_check_pool("kv-move", fmt, p))) return rc;
-  p.bits = (uint32_t)fmt;
+  if (!args) return set_error(NL_ERROR, "kv-move: null arguments");
+  const KvPool p = kv_pool_of(args->cache);
+  if ((rc = kv_check_pool("kv-move", args->cache.fmt, p))) return rc;
+  const uint32_t batch = args->batch, count = args->count;
   if (batch == 0 || count == 0) return NL_OK;
-  if (!SRC || !DST) return set_error(NL_ERROR, "kv-move: null slots");
-  if (count > 64 || batch > 65535 || kv_heads > 65535)
-    return set_error(NL_ERROR, "kv-move: count %u (at most 64), batch %u, kv heads %u", count,
-                     batch, kv_heads);
-  const size_t smem = (size_t)count * (head_dim * p.bits / 128 + 1) * 16;   // at most 17 KB
-  const cudaError_t e = launch_pdl(kv_move_kernel, dim3(kv_heads, batch, 2), dim3(kThreads), smem,
-                                   (cudaStream_t)stream, p, SRC, DST, count);
+  if (!args->src || !args->dst) return set_error(NL_ERROR, "kv-move: null slots");
+  if (count > 64 || batch > 65535)
+    return set_error(NL_ERROR, "kv-move: count %u (at most 64), batch %u (at most 65535)", count,
+                     batch);
+  const size_t smem = (size_t)count * (p.head_dim * p.bits / 128 + 1) * 16;   // at most 17 KB
+  const cudaError_t e = launch_pdl(kv_move_kernel, dim3(p.kv_heads, batch, 2), dim3(kThreads), smem,
+                                   (cudaStream_t)stream, p, args->src, args->dst, count);
   count_launches(1);
   return cuda_status(e, "kv-move");
 }

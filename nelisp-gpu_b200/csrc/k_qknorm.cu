@@ -421,29 +421,34 @@ int check_tables(const char *what, const QkArgs &a) {
 
 using namespace nl;
 
-extern "C" int nl_qk_norm_rope_dev(int dtype, const void *QKV, uint64_t x_stride, const float *GQ,
-                                   const float *GK, const float *CO, const float *SI,
-                                   const int32_t *POS, void *Q, uint64_t q_stride, void *K,
-                                   uint64_t k_stride, uint32_t n, uint32_t heads,
-                                   uint32_t kv_heads, uint32_t head_dim, uint32_t rot_dim,
-                                   uint32_t rope_rows, int pairs, float eps, void *stream) {
+// The fields that the two directions share.
+template <typename A> static QkArgs common_of(const A &x) {
+  QkArgs a = {};
+  a.x = x.qkv; a.x_stride = x.x_stride;
+  a.g[0] = x.gq; a.g[1] = x.gk; a.co = x.co; a.si = x.si; a.pos = x.pos;
+  a.n = x.n; a.heads[0] = x.heads; a.heads[1] = x.kv_heads; a.head_dim = x.head_dim;
+  a.rot = x.rot_dim; a.rope_rows = x.rope_rows; a.eps = x.eps;
+  return a;
+}
+
+extern "C" int nl_qk_norm_rope_dev(const nl_qk_norm_rope_args *args, void *stream) {
   int rc = api_ready();
   if (rc) return rc;
   const char *what = "qk-norm-rope";
-  QkArgs a = {};
-  a.x = QKV; a.x_stride = x_stride; a.g[0] = GQ; a.g[1] = GK; a.co = CO; a.si = SI; a.pos = POS;
-  a.out[0] = Q; a.out[1] = K; a.out_stride[0] = q_stride; a.out_stride[1] = k_stride;
-  a.n = n; a.heads[0] = heads; a.heads[1] = kv_heads; a.head_dim = head_dim; a.rot = rot_dim;
-  a.rope_rows = rope_rows; a.eps = eps;
+  if (!args) return set_error(NL_ERROR, "%s: null arguments", what);
+  const nl_qk_norm_rope_args &x = *args;
+  const int dtype = x.dtype, pairs = x.pairs;
+  QkArgs a = common_of(x);
+  a.out[0] = x.q; a.out[1] = x.k; a.out_stride[0] = x.q_stride; a.out_stride[1] = x.k_stride;
   if ((rc = check_common(what, dtype, a, pairs))) return rc;
-  if (n == 0) return NL_OK;
-  const uint64_t qw = (uint64_t)heads * head_dim, kw = (uint64_t)kv_heads * head_dim;
-  if ((rc = check_rows(what, "QKV", dtype, QKV, x_stride, qw + kw)) ||
-      (rc = check_rows(what, "Q", dtype, Q, q_stride, qw)) ||
-      (rc = check_rows(what, "K", dtype, K, k_stride, kw)) || (rc = check_tables(what, a)))
+  if (x.n == 0) return NL_OK;
+  const uint64_t qw = (uint64_t)x.heads * x.head_dim, kw = (uint64_t)x.kv_heads * x.head_dim;
+  if ((rc = check_rows(what, "QKV", dtype, x.qkv, x.x_stride, qw + kw)) ||
+      (rc = check_rows(what, "Q", dtype, x.q, x.q_stride, qw)) ||
+      (rc = check_rows(what, "K", dtype, x.k, x.k_stride, kw)) || (rc = check_tables(what, a)))
     return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  const uint32_t group = group_of(dtype, head_dim);
+  const uint32_t group = group_of(dtype, x.head_dim);
   divide(a, 32 / group);
   const bool half = pairs == NL_PAIRS_HALF;
   const cudaError_t e = dtype == NL_BF16 ? start_t<__nv_bfloat16, false>(a, half, group, st)
@@ -456,45 +461,37 @@ extern "C" size_t nl_qk_norm_rope_bwd_workspace_bytes(uint32_t head_dim) {
   return (size_t)kMaxBlocks * head_dim * sizeof(float);
 }
 
-extern "C" int nl_qk_norm_rope_bwd_dev(int dtype, const void *QKV, uint64_t x_stride,
-                                       const float *GQ, const float *GK, const float *CO,
-                                       const float *SI, const int32_t *POS, const void *DQ,
-                                       uint64_t dq_stride, const void *DK, uint64_t dk_stride,
-                                       void *DQKV, uint64_t dx_stride, float *DGQ, float *DGK,
-                                       uint32_t n, uint32_t heads, uint32_t kv_heads,
-                                       uint32_t head_dim, uint32_t rot_dim, uint32_t rope_rows,
-                                       int pairs, float eps, void *workspace, size_t ws_bytes,
-                                       void *stream) {
+extern "C" int nl_qk_norm_rope_bwd_dev(const nl_qk_norm_rope_bwd_args *args, void *stream) {
   int rc = api_ready();
   if (rc) return rc;
   const char *what = "qk-norm-rope-bwd";
-  QkArgs a = {};
-  a.x = QKV; a.x_stride = x_stride; a.g[0] = GQ; a.g[1] = GK; a.co = CO; a.si = SI; a.pos = POS;
-  a.dy[0] = DQ; a.dy[1] = DK; a.dy_stride[0] = dq_stride; a.dy_stride[1] = dk_stride;
-  a.out_stride[0] = a.out_stride[1] = dx_stride;
-  a.n = n; a.heads[0] = heads; a.heads[1] = kv_heads; a.head_dim = head_dim; a.rot = rot_dim;
-  a.rope_rows = rope_rows; a.eps = eps;
+  if (!args) return set_error(NL_ERROR, "%s: null arguments", what);
+  const nl_qk_norm_rope_bwd_args &x = *args;
+  const int dtype = x.dtype, pairs = x.pairs;
+  QkArgs a = common_of(x);
+  a.dy[0] = x.dq; a.dy[1] = x.dk; a.dy_stride[0] = x.dq_stride; a.dy_stride[1] = x.dk_stride;
+  a.out_stride[0] = a.out_stride[1] = x.dx_stride;
   if ((rc = check_common(what, dtype, a, pairs))) return rc;
-  if (!DGQ || !DGK) return set_error(NL_ERROR, "%s: a null gain gradient", what);
+  if (!x.dgq || !x.dgk) return set_error(NL_ERROR, "%s: a null gain gradient", what);
   cudaStream_t st = (cudaStream_t)stream;
-  if (n) {
-    const uint64_t qw = (uint64_t)heads * head_dim, kw = (uint64_t)kv_heads * head_dim;
-    if ((rc = check_rows(what, "QKV", dtype, QKV, x_stride, qw + kw)) ||
-        (rc = check_rows(what, "DQ", dtype, DQ, dq_stride, qw)) ||
-        (rc = check_rows(what, "DK", dtype, DK, dk_stride, kw)) ||
-        (rc = check_rows(what, "DQKV", dtype, DQKV, dx_stride, qw + kw)) ||
+  if (x.n) {
+    const uint64_t qw = (uint64_t)x.heads * x.head_dim, kw = (uint64_t)x.kv_heads * x.head_dim;
+    if ((rc = check_rows(what, "QKV", dtype, x.qkv, x.x_stride, qw + kw)) ||
+        (rc = check_rows(what, "DQ", dtype, x.dq, x.dq_stride, qw)) ||
+        (rc = check_rows(what, "DK", dtype, x.dk, x.dk_stride, kw)) ||
+        (rc = check_rows(what, "DQKV", dtype, x.dqkv, x.dx_stride, qw + kw)) ||
         (rc = check_tables(what, a)))
       return rc;
-    const size_t need = nl_qk_norm_rope_bwd_workspace_bytes(head_dim);
-    if (workspace && ws_bytes < need)
-      return set_error(NL_ERROR, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, need);
-    if (!workspace) workspace = library_workspace(need, st);
+    const size_t need = nl_qk_norm_rope_bwd_workspace_bytes(x.head_dim);
+    if (x.workspace && x.ws_bytes < need)
+      return set_error(NL_ERROR, "%s: workspace of %zu bytes, %zu needed", what, x.ws_bytes, need);
+    void *workspace = x.workspace ? x.workspace : library_workspace(need, st);
     if (!workspace || !aligned16(workspace))
       return set_error(NL_ERROR, "%s: no aligned workspace of %zu bytes", what, need);
     a.partial = (float *)workspace;
-    a.out[0] = DQKV;
-    a.out[1] = (char *)DQKV + qw * (dtype == NL_BF16 ? 2 : 4);
-    const uint32_t group = group_of(dtype, head_dim);
+    a.out[0] = x.dqkv;
+    a.out[1] = (char *)x.dqkv + qw * (dtype == NL_BF16 ? 2 : 4);
+    const uint32_t group = group_of(dtype, x.head_dim);
     divide(a, 32 / group);
     const bool half = pairs == NL_PAIRS_HALF;
     const cudaError_t e = dtype == NL_BF16 ? start_t<__nv_bfloat16, true>(a, half, group, st)
@@ -502,9 +499,9 @@ extern "C" int nl_qk_norm_rope_bwd_dev(int dtype, const void *QKV, uint64_t x_st
     count_launches(1);
     if (e != cudaSuccess) return cuda_status(e, what);
   }
-  const cudaError_t e = launch_pdl(qk_gain_sum_kernel, dim3(head_dim / 8, 2), dim3(256), 0, st,
-                                   (const float *)workspace, a.blocks[0], a.blocks[1], head_dim,
-                                   DGQ, DGK);
+  const cudaError_t e = launch_pdl(qk_gain_sum_kernel, dim3(x.head_dim / 8, 2), dim3(256), 0, st,
+                                   (const float *)a.partial, a.blocks[0], a.blocks[1], x.head_dim,
+                                   x.dgq, x.dgk);
   count_launches(1);
   return cuda_status(e, what);
 }

@@ -26,24 +26,20 @@ extern "C" size_t nl_tree_attn_workspace_bytes(uint32_t nodes, uint32_t heads, u
   return (size_t)2 * kTreeMaxCtas * rows * (head_dim + 2) * sizeof(float);
 }
 
-extern "C" int nl_tree_attn_dev(int fmt, int dtype, const void *Q, uint64_t q_stride,
-                                const void *KC, const uint32_t *KP, const void *VC,
-                                const uint32_t *VP, const int32_t *TABLE, const int32_t *LEN,
-                                const uint64_t *MASK, void *O, uint64_t o_stride, float *LSE,
-                                uint32_t batch, uint32_t nodes, uint32_t heads, uint32_t kv_heads,
-                                uint32_t head_dim, uint32_t block_size, uint32_t num_blocks,
-                                uint32_t max_blocks, float scale, void *workspace,
-                                size_t ws_bytes, void *stream) {
+extern "C" int nl_tree_attn_dev(const nl_tree_attn_args *args, void *stream) {
   int rc = api_ready();
   if (rc) return rc;
   const char *what = "tree-attn";
-  if (dtype != NL_F32 && dtype != NL_BF16)
-    return set_error(NL_ERROR, "%s: type %d is neither NL_F32 nor NL_BF16", what, dtype);
+  if (!args) return set_error(NL_ERROR, "%s: null arguments", what);
+  const nl_tree_attn_args &x = *args;
+  const uint32_t batch = x.batch, nodes = x.nodes, heads = x.heads, kv_heads = x.cache.kv_heads,
+                 head_dim = x.cache.head_dim, block_size = x.cache.block_size;
+  const float scale = x.scale;
+  if (x.dtype != NL_F32 && x.dtype != NL_BF16)
+    return set_error(NL_ERROR, "%s: type %d is neither NL_F32 nor NL_BF16", what, x.dtype);
   TreeArgs a = {};
-  a.pool = {{(uint8_t *)const_cast<void *>(KC), (uint8_t *)const_cast<void *>(VC)},
-            {const_cast<uint32_t *>(KP), const_cast<uint32_t *>(VP)}, num_blocks, block_size,
-            kv_heads, head_dim, (uint32_t)fmt};
-  if ((rc = kv_check_pool(what, fmt, a.pool))) return rc;
+  a.pool = kv_pool_of(x.cache);
+  if ((rc = kv_check_pool(what, x.cache.fmt, a.pool))) return rc;
   if (!heads || heads % kv_heads || heads > 65536)
     return set_error(NL_ERROR, "%s: heads %u, kv heads %u", what, heads, kv_heads);
   if (nodes > 64) return set_error(NL_ERROR, "%s: %u nodes (at most 64)", what, nodes);
@@ -52,37 +48,37 @@ extern "C" int nl_tree_attn_dev(int fmt, int dtype, const void *Q, uint64_t q_st
   if (batch == 0 || nodes == 0) return NL_OK;
   if ((uint64_t)batch * nodes * heads > INT32_MAX)
     return set_error(NL_ERROR, "%s: %u sequences x %u nodes x %u heads", what, batch, nodes, heads);
-  if (!LEN || !MASK || ((uintptr_t)MASK & 7u) || (!TABLE && max_blocks))
+  if (!x.len || !x.mask || ((uintptr_t)x.mask & 7u) || (!x.table && x.max_blocks))
     return set_error(NL_ERROR, "%s: null lengths, masks or table, or unaligned masks", what);
-  const uint32_t unit = dtype == NL_BF16 ? 8 : 4;
+  const uint32_t unit = x.dtype == NL_BF16 ? 8 : 4;
   const uint64_t width = (uint64_t)heads * head_dim;
-  if (!Q || !O || !aligned16(Q) || !aligned16(O) || q_stride % unit || o_stride % unit ||
-      q_stride < width || o_stride < width)
+  if (!x.q || !x.o || !aligned16(x.q) || !aligned16(x.o) || x.q_stride % unit ||
+      x.o_stride % unit || x.q_stride < width || x.o_stride < width)
     return set_error(NL_ERROR,
                      "%s: Q and O rows must be 16-byte aligned, with strides (%llu, %llu) that are "
                      "multiples of %u and at least heads x head size",
-                     what, (unsigned long long)q_stride, (unsigned long long)o_stride, unit);
+                     what, (unsigned long long)x.q_stride, (unsigned long long)x.o_stride, unit);
   cudaStream_t st = (cudaStream_t)stream;
   const size_t need = nl_tree_attn_workspace_bytes(nodes, heads, kv_heads, head_dim);
-  if (workspace && ws_bytes < need)
-    return set_error(NL_ERROR, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, need);
-  if (!workspace) workspace = library_workspace(need, st);
+  if (x.workspace && x.ws_bytes < need)
+    return set_error(NL_ERROR, "%s: workspace of %zu bytes, %zu needed", what, x.ws_bytes, need);
+  void *workspace = x.workspace ? x.workspace : library_workspace(need, st);
   if (!workspace || !aligned16(workspace))
     return set_error(NL_ERROR, "%s: no aligned workspace of %zu bytes", what, need);
-  a.q = Q; a.o = O; a.lse = LSE; a.table = TABLE; a.len = LEN; a.mask = MASK;
-  a.q_stride = q_stride; a.o_stride = o_stride;
+  a.q = x.q; a.o = x.o; a.lse = x.lse; a.table = x.table; a.len = x.len; a.mask = x.mask;
+  a.q_stride = x.q_stride; a.o_stride = x.o_stride;
   a.batch = batch; a.nodes = nodes; a.heads = heads; a.group = heads / kv_heads;
   a.rows = a.group * nodes;
-  const bool bf16 = dtype == NL_BF16;
+  const bool bf16 = x.dtype == NL_BF16;
   const uint32_t umma_rows = tree_umma_rows(a, bf16);
   a.rows_at_once = umma_rows ? umma_rows : tree_rows_at_once(a.rows, head_dim);
   a.row_tiles = (a.rows + a.rows_at_once - 1) / a.rows_at_once;
   a.block_shift = 32;
   for (uint32_t s = 0; s < 32; s++)
     if (block_size == 1u << s) a.block_shift = s;
-  a.max_blocks = max_blocks;
+  a.max_blocks = x.max_blocks;
   a.scale = scale * 1.4426950408889634f;
-  if (!num_blocks)                 // nothing is read of an empty pool, but its addresses are formed
+  if (!x.cache.num_blocks)         // nothing is read of an empty pool, but its addresses are formed
     for (int i = 0; i < 2; i++)
       a.pool.code[i] = (uint8_t *)workspace, a.pool.param[i] = (uint32_t *)workspace;
   a.part_o = (float *)workspace;

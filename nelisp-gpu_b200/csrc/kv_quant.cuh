@@ -33,6 +33,10 @@ __device__ __forceinline__ uint32_t kv_row(const KvPool &p, uint32_t block, uint
   return (block * p.kv_heads + head) * p.block_size + off;
 }
 
+static inline KvPool kv_pool_of(const nl_kv_cache &c) {
+  return {{(uint8_t *)c.kc, (uint8_t *)c.vc}, {c.kp, c.vp}, c.num_blocks, c.block_size,
+          c.kv_heads, c.head_dim, (uint32_t)c.fmt};
+}
 // NL_OK if the pool's description can be served (k_kvquant.cu).
 int kv_check_pool(const char *what, int fmt, const KvPool &p);
 

@@ -107,7 +107,9 @@ __device__ __forceinline__ void locate(const TreeArgs &a, uint64_t at, uint32_t 
   const uint64_t items = (uint64_t)a.pool.kv_heads * a.row_tiles;
   uint64_t before = 0;
   for (uint32_t base = 0; base < a.batch; base += 32) {
-    uint64_t mine = base + lane < a.batch ? (tiles_of(a, base + lane) + a.item_cost) * items : 0, end = mine;
+    const uint64_t mine =
+        base + lane < a.batch ? (tiles_of(a, base + lane) + a.item_cost) * items : 0;
+    uint64_t end = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t up = __shfl_up_sync(0xffffffffu, end, o);

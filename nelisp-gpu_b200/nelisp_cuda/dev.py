@@ -108,6 +108,11 @@ def decode_attn_rope(QKV, CK, CV, POS, C, batch, heads, kv_heads, head_dim, max_
 # they take.
 
 _PAIRS = {"half": 0, "adjacent": 1}      # NL_PAIRS_HALF, NL_PAIRS_ADJACENT
+_PACK_QK = L.PACKED["nl_qk_norm_rope_dev"].pack
+_PACK_QK_BWD = L.PACKED["nl_qk_norm_rope_bwd_dev"].pack
+_PACK_ROWS = L.PACKED["nl_kv_rows"].pack
+_PACK_MOVE = L.PACKED["nl_kv_move_dev"].pack
+_PACK_TREE = L.PACKED["nl_tree_attn_dev"].pack
 _types = None
 
 
@@ -180,7 +185,7 @@ def _qk_shapes(QKV, GQ, GK, CO, SI, POS, Q, K, pairs):
     if wq % hd or wk % hd or wq + wk > width:
         raise ValueError(f"rows of {width} values do not hold heads of {hd}: {wq} + {wk}")
     _need(pairs in _PAIRS, "pairs: 'half' or 'adjacent'")
-    return n, wq // hd, wk // hd, hd, 2 * table[1], table[0], _PAIRS[pairs]
+    return n, wq // hd, wk // hd, hd, 2 * table[1], table[0]
 
 
 def qk_norm_rope(QKV, GQ, GK, CO, SI, POS, Q, K, eps=1e-5, pairs="half", stream=None):
@@ -192,9 +197,10 @@ def qk_norm_rope(QKV, GQ, GK, CO, SI, POS, Q, K, eps=1e-5, pairs="half", stream=
     kind = _row_type(QKV)
     xs, qs, ks = _rows(QKV.dtype, QKV, Q, K)
     dims = _qk_shapes(QKV, GQ, GK, CO, SI, POS, Q, K, pairs)
-    rc = _lib().nl_qk_norm_rope_dev(
-        kind, QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(), SI.data_ptr(),
-        POS.data_ptr(), Q.data_ptr(), qs, K.data_ptr(), ks, *dims, eps, _stream(stream))
+    rc = _lib().nl_qk_norm_rope_dev(_PACK_QK(
+        kind, _PAIRS[pairs], QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(),
+        SI.data_ptr(), POS.data_ptr(), Q.data_ptr(), qs, K.data_ptr(), ks, *dims, eps),
+        _stream(stream))
     if rc:
         L.check(rc)
 
@@ -215,10 +221,10 @@ def qk_norm_rope_bwd(QKV, GQ, GK, CO, SI, POS, DQ, DK, DQKV, DGQ, DGK, eps=1e-5,
     lib = _lib()
     ws, nbytes = _workspace(lib.nl_qk_norm_rope_bwd_workspace_bytes(hd), workspace, QKV.device,
                             stream)
-    rc = lib.nl_qk_norm_rope_bwd_dev(
-        kind, QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(), SI.data_ptr(),
-        POS.data_ptr(), DQ.data_ptr(), qs, DK.data_ptr(), ks, DQKV.data_ptr(), dxs,
-        DGQ.data_ptr(), DGK.data_ptr(), *dims, eps, ws.data_ptr(), nbytes, _stream(stream))
+    rc = lib.nl_qk_norm_rope_bwd_dev(_PACK_QK_BWD(
+        kind, _PAIRS[pairs], QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(),
+        SI.data_ptr(), POS.data_ptr(), DQ.data_ptr(), qs, DK.data_ptr(), ks, DQKV.data_ptr(), dxs,
+        DGQ.data_ptr(), DGK.data_ptr(), *dims, eps, ws.data_ptr(), nbytes), _stream(stream))
     if rc:
         L.check(rc)
 
@@ -236,7 +242,7 @@ def kv_cache(num_blocks, block_size, kv_heads, head_dim, bits, device="cuda"):
 
 
 def _pool(KC, KP, VC, VP, head_dim):
-    """(bits, (kv_heads, head_dim, block_size, num_blocks)) of a cache."""
+    """A cache as the fields of nl_kv_cache."""
     types = _torch_types()
     _flat(types[4], KC, VC)
     _flat(types[2], KP, VP)
@@ -251,7 +257,8 @@ def _pool(KC, KP, VC, VP, head_dim):
         bits = 4
     else:
         raise ValueError(f"rows of {row} bytes for heads of {head_dim}")
-    return bits, (kvh, head_dim, size, blocks)
+    return (bits, kvh, head_dim, size, blocks, KC.data_ptr(), KP.data_ptr(), VC.data_ptr(),
+            VP.data_ptr())
 
 
 def _kv_shapes(SLOT, KC, KP, VC, VP, K, V):
@@ -269,10 +276,9 @@ def kv_append(K, V, SLOT, KC, KP, VC, VP, stream=None):
     strided) into the cache's token slots SLOT (int32 [n]; outside: skipped)."""
     kind = _row_type(K)
     ks, vs = _rows(K.dtype, K, V)
-    n, (bits, dims) = _kv_shapes(SLOT, KC, KP, VC, VP, K, V)
-    rc = _lib().nl_kv_append_dev(
-        bits, kind, K.data_ptr(), ks, V.data_ptr(), vs, SLOT.data_ptr(), KC.data_ptr(),
-        KP.data_ptr(), VC.data_ptr(), VP.data_ptr(), n, *dims, _stream(stream))
+    n, pool = _kv_shapes(SLOT, KC, KP, VC, VP, K, V)
+    rc = _lib().nl_kv_append_dev(_PACK_ROWS(
+        *pool, kind, n, SLOT.data_ptr(), K.data_ptr(), ks, V.data_ptr(), vs), _stream(stream))
     if rc:
         L.check(rc)
 
@@ -281,10 +287,9 @@ def kv_read(SLOT, KC, KP, VC, VP, K, V, stream=None):
     """The values of the slots SLOT into the rows K and V (outside: zeros)."""
     kind = _row_type(K)
     ks, vs = _rows(K.dtype, K, V)
-    n, (bits, dims) = _kv_shapes(SLOT, KC, KP, VC, VP, K, V)
-    rc = _lib().nl_kv_read_dev(
-        bits, kind, SLOT.data_ptr(), KC.data_ptr(), KP.data_ptr(), VC.data_ptr(), VP.data_ptr(),
-        K.data_ptr(), ks, V.data_ptr(), vs, n, *dims, _stream(stream))
+    n, pool = _kv_shapes(SLOT, KC, KP, VC, VP, K, V)
+    rc = _lib().nl_kv_read_dev(_PACK_ROWS(
+        *pool, kind, n, SLOT.data_ptr(), K.data_ptr(), ks, V.data_ptr(), vs), _stream(stream))
     if rc:
         L.check(rc)
 
@@ -294,10 +299,9 @@ def kv_move(SRC, DST, KC, KP, VC, VP, head_dim, stream=None):
     [batch, count]; per sequence every source is read before any write."""
     _flat(_torch_types()[2], SRC, DST)
     _need(SRC.dim() == 2 and SRC.shape == DST.shape, "SRC and DST: [batch, count] each")
-    bits, dims = _pool(KC, KP, VC, VP, head_dim)
-    L.check(_lib().nl_kv_move_dev(
-        bits, SRC.data_ptr(), DST.data_ptr(), KC.data_ptr(), KP.data_ptr(), VC.data_ptr(),
-        VP.data_ptr(), SRC.shape[0], SRC.shape[1], *dims, _stream(stream)))
+    L.check(_lib().nl_kv_move_dev(_PACK_MOVE(
+        *_pool(KC, KP, VC, VP, head_dim), SRC.data_ptr(), DST.data_ptr(), *SRC.shape),
+        _stream(stream)))
 
 
 def tree_attn(Q, KC, KP, VC, VP, TABLE, LEN, MASK, O, head_dim, scale=None, lse=None,
@@ -314,7 +318,7 @@ def tree_attn(Q, KC, KP, VC, VP, TABLE, LEN, MASK, O, head_dim, scale=None, lse=
     qs, os_ = _rows(Q.dtype, Q, O)
     _flat(types[2], TABLE, LEN)
     _flat(types[3], MASK)
-    bits, dims = _pool(KC, KP, VC, VP, head_dim)
+    pool = _pool(KC, KP, VC, VP, head_dim)
     table, mask, shape = TABLE.shape, MASK.shape, Q.shape
     _need(len(mask) == 2 and len(table) == 2, "MASK and TABLE have 2 dimensions")
     batch, nodes = mask
@@ -325,19 +329,19 @@ def tree_attn(Q, KC, KP, VC, VP, TABLE, LEN, MASK, O, head_dim, scale=None, lse=
         raise ValueError(f"tree_attn: {rows} rows of {width}, heads of {head_dim}, {batch} "
                          f"sequences of {nodes} nodes, {LEN.numel()} lengths, a table of "
                          f"{tuple(table)}, outputs of {tuple(O.shape)}")
-    out_lse = None
+    out_lse = 0
     if lse is not None:
         _flat(types[0], lse)
         _need(lse.shape == (rows, heads), "lse: a value per row and head")
         out_lse = lse.data_ptr()
     lib = _lib()
-    ws, nbytes = _workspace(lib.nl_tree_attn_workspace_bytes(nodes, heads, dims[0], head_dim),
+    ws, nbytes = _workspace(lib.nl_tree_attn_workspace_bytes(nodes, heads, pool[1], head_dim),
                             workspace, Q.device, stream)
-    rc = lib.nl_tree_attn_dev(
-        bits, kind, Q.data_ptr(), qs, KC.data_ptr(), KP.data_ptr(), VC.data_ptr(), VP.data_ptr(),
-        TABLE.data_ptr(), LEN.data_ptr(), MASK.data_ptr(), O.data_ptr(), os_, out_lse, batch,
-        nodes, heads, *dims, table[1], scale if scale is not None else head_dim ** -0.5,
-        ws.data_ptr(), nbytes, _stream(stream))
+    rc = lib.nl_tree_attn_dev(_PACK_TREE(
+        *pool, kind, batch, nodes, heads, table[1],
+        scale if scale is not None else head_dim ** -0.5, Q.data_ptr(), qs, TABLE.data_ptr(),
+        LEN.data_ptr(), MASK.data_ptr(), O.data_ptr(), os_, out_lse, ws.data_ptr(), nbytes),
+        _stream(stream))
     if rc:
         L.check(rc)
 

@@ -17,7 +17,6 @@ Tolerances.  u = 2^-24 is the rounding of float32.
   |error| <= (2^-20 scale max_t sum |q k_t| + 2^-19) max |v|; where the output
   is bfloat16 the weights' float16 rounding adds 2^-11 max |v|.
 """
-import ctypes
 import math
 
 import numpy as np
@@ -885,33 +884,46 @@ def test_library_refusals(dev, torch):
     s = torch.zeros(4, dtype=torch.int32, device="cuda")
     with pytest.raises(L.NlError, match="head size"):
         dev.kv_append(k[:, :32], k[:, :32], s, *dev.kv_cache(2, 16, 1, 32, 8))
-    lib, p = L.load(), ctypes.c_void_p(16)
-    cases = [("nl_kv_append_dev", (5, 0, p, 64, p, 64, p, p, p, p, p, 1, 1, 64, 16, 1, None),
-              "format"),
-             ("nl_kv_append_dev", (8, 2, p, 64, p, 64, p, p, p, p, p, 1, 1, 64, 16, 1, None),
-              "type"),
-             ("nl_kv_append_dev", (8, 0, p, 64, p, 64, p, p, p, p, p, 1, 1, 64, 1 << 16, 1 << 15,
-                                   None), "slots"),
-             ("nl_kv_append_dev", (8, 0, p, 32, p, 64, p, p, p, p, p, 1, 1, 64, 16, 1, None),
-              "stride"),
-             ("nl_kv_read_dev", (8, 0, None, p, p, p, p, p, 64, p, 64, 1, 1, 64, 16, 1, None),
-              "slots"),
-             ("nl_kv_move_dev", (8, p, p, p, p, p, p, 1, 65, 1, 64, 16, 1, None), "count"),
-             ]
+    lib, p = L.load(), 16
 
-    def tree(**kw):
-        a = dict(fmt=8, dtype=0, q=p, qs=64, kc=p, kp=p, vc=p, vp=p, table=p, ln=p, mask=p, o=p,
-                 os=64, lse=None, batch=1, nodes=1, heads=1, kvh=1, hd=64, bs=16, nb=1, mb=1,
-                 scale=0.1, ws=p, wsb=1 << 30, stream=None)
-        a.update(kw)
-        return ("nl_tree_attn_dev", tuple(a.values()))
-    cases += [(*tree(nodes=65), "nodes"), (*tree(heads=3, kvh=2), "heads"),
-              (*tree(hd=96, qs=96, os=96), "head size"), (*tree(scale=0.0), "scale"),
-              (*tree(scale=math.inf), "scale"), (*tree(scale=math.nan), "scale"),
-              (*tree(qs=63), "strides"), (*tree(o=ctypes.c_void_p(8)), "aligned"),
-              (*tree(mask=None), "null"), (*tree(wsb=100), "workspace"),
-              (*tree(fmt=6), "format"), (*tree(kc=ctypes.c_void_p(4)), "unaligned")]
+    def cache(fmt=8, kvh=1, hd=64, bs=16, nb=1, kc=p, kp=p, vc=p, vp=p):
+        return fmt, kvh, hd, bs, nb, kc, kp, vc, vp
+
+    def rows(pool, dtype=0, n=1, slot=p, k=p, ks=64, v=p, vs=64):
+        return L.PACKED["nl_kv_rows"].pack(*pool, dtype, n, slot, k, ks, v, vs)
+
+    def tree(pool, dtype=0, batch=1, nodes=1, heads=1, mb=1, scale=0.1, q=p, qs=64, table=p, ln=p,
+             mask=p, o=p, os=64, lse=0, ws=p, wsb=1 << 30):
+        return L.PACKED["nl_tree_attn_dev"].pack(*pool, dtype, batch, nodes, heads, mb, scale, q,
+                                                 qs, table, ln, mask, o, os, lse, ws, wsb)
+    move = L.PACKED["nl_kv_move_dev"].pack
+    cases = [("nl_kv_append_dev", rows(cache(fmt=5)), "format"),
+             ("nl_kv_append_dev", rows(cache(), dtype=2), "type"),
+             ("nl_kv_append_dev", rows(cache(bs=1 << 16, nb=1 << 15)), "slots"),
+             ("nl_kv_append_dev", rows(cache(kvh=4, bs=1 << 16, nb=1 << 14), ks=256, vs=256),
+              "rows"),
+             ("nl_kv_append_dev", rows(cache(), ks=32), "stride"),
+             ("nl_kv_append_dev", rows(cache(hd=32)), "head size"),
+             ("nl_kv_read_dev", rows(cache(), slot=0), "slots"),
+             ("nl_kv_read_dev", rows(cache(), v=8), "aligned"),
+             ("nl_kv_move_dev", move(*cache(), p, p, 1, 65), "count"),
+             ("nl_kv_move_dev", move(*cache(), 0, p, 1, 1), "null"),
+             ("nl_tree_attn_dev", tree(cache(), nodes=65), "nodes"),
+             ("nl_tree_attn_dev", tree(cache(kvh=2), heads=3), "heads"),
+             ("nl_tree_attn_dev", tree(cache(hd=96), qs=96, os=96), "head size"),
+             ("nl_tree_attn_dev", tree(cache(), scale=0.0), "scale"),
+             ("nl_tree_attn_dev", tree(cache(), scale=math.inf), "scale"),
+             ("nl_tree_attn_dev", tree(cache(), scale=math.nan), "scale"),
+             ("nl_tree_attn_dev", tree(cache(), qs=63), "strides"),
+             ("nl_tree_attn_dev", tree(cache(), o=8), "aligned"),
+             ("nl_tree_attn_dev", tree(cache(), mask=0), "null"),
+             ("nl_tree_attn_dev", tree(cache(), wsb=100), "workspace"),
+             ("nl_tree_attn_dev", tree(cache(fmt=6)), "format"),
+             ("nl_tree_attn_dev", tree(cache(kc=4)), "unaligned")]
+    cases += [(name, None, "null") for name in
+              ("nl_qk_norm_rope_dev", "nl_qk_norm_rope_bwd_dev", "nl_kv_append_dev",
+               "nl_kv_read_dev", "nl_kv_move_dev", "nl_tree_attn_dev")]
     for name, args, word in cases:
-        assert getattr(lib, name)(*args) == L.NL_ERROR, (name, word)
+        assert getattr(lib, name)(args, None) == L.NL_ERROR, (name, word)
         assert word in lib.nl_last_error().decode(), (name, word, lib.nl_last_error())
     assert dev.launch_count() == before

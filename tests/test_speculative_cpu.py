@@ -53,3 +53,29 @@ def test_workspace_queries():
             assert n % 16 == 0 and n >= last
             last = n
     assert lib.nl_tree_attn_workspace_bytes(0, 0, 0, 128) >= 0
+
+
+def test_packed_structures_match_the_header(tmp_path):
+    """The Python packing and the C compiler agree on every structure's size
+    and on where its last field is."""
+    import os
+    import subprocess
+
+    from conftest import ROOT
+    names = {"nl_qk_norm_rope_args": ("nl_qk_norm_rope_dev", "eps"),
+             "nl_qk_norm_rope_bwd_args": ("nl_qk_norm_rope_bwd_dev", "ws_bytes"),
+             "nl_kv_rows_args": ("nl_kv_rows", "v_stride"),
+             "nl_kv_move_args": ("nl_kv_move_dev", "count"),
+             "nl_tree_attn_args": ("nl_tree_attn_dev", "ws_bytes")}
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "nelisp_cuda.h"\n'
+                   "int main(void) {\n" +
+                   "".join(f'printf("%zu %zu\\n", offsetof({n}, {last}) + sizeof((({n} *)0)->{last}), '
+                           f"sizeof({n}));\n" for n, (_, last) in names.items()) + "}\n")
+    exe = tmp_path / "sizes"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), "-o", str(exe), str(src)],
+                   check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split("\n")
+    for line, (packed, _) in zip(out, names.values()):
+        end, size = map(int, line.split())
+        assert L.PACKED[packed].size == end <= size < end + 8, packed
