@@ -885,8 +885,23 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
 
 }  // namespace
 
+// The rows of an item of this form, 0 where the other one serves.  It takes
+// about 3,000 cycles a tile whatever the rows, the other one a time that grows
+// with them and with the head size, so this one is for many (us, 4 sequences of
+// 32,768 keys, 8 key heads, 8 bits / 4 bits):
+//   rows            8        16       20        32         48        64
+//   128 values
+//     this form   92/99    93/99    92/ 99    93/100    114/131   117/133
+//     the other   59/61    68/71   100/106   103/109    176/193   181/197
+//   64 values
+//     this form   87/103   87/103   87/104    89/105    108/127   110/130
+//     the other   42/43    50/52    66/ 72    68/ 75    116/135   120/139
+// More than 16 rows of 128 values, then, or 32 of 64.  (256 values have no room
+// in TMEM and shared memory; a run of a page that is no multiple of 16 keys has
+// no copy of whole boxes; float32 needs its sums out of the tensor core often.)
 uint32_t tree_umma_rows(const TreeArgs &a, bool bf16) {
-  if (!bf16 || a.pool.head_dim > 128 || a.pool.block_size % 16 || a.rows <= 16 ||
+  if (!bf16 || a.pool.head_dim > 128 || a.pool.block_size % 16 ||
+      (uint64_t)a.rows * a.pool.head_dim <= 2048 ||
       (uint64_t)a.pool.num_blocks * a.pool.kv_heads * a.pool.block_size > INT32_MAX ||
       !a.pool.num_blocks || (uint64_t)a.batch * a.nodes * a.heads >= kNone || !encode_fn())
     return 0;
@@ -897,10 +912,10 @@ cudaError_t tree_umma_start(TreeArgs &a, cudaStream_t st) {
   const bool h128 = a.pool.head_dim == 128;
   const bool few = a.rows_at_once == 32;
   if (a.pool.bits == 4) {
-    if (few) return h128 ? start<128, 4, 32>(a, st) : start<64, 4, 32>(a, st);
+    if (few) return start<128, 4, 32>(a, st);          // 64 values have more rows than 32
     return h128 ? start<128, 4, 64>(a, st) : start<64, 4, 64>(a, st);
   }
-  if (few) return h128 ? start<128, 8, 32>(a, st) : start<64, 8, 32>(a, st);
+  if (few) return start<128, 8, 32>(a, st);
   return h128 ? start<128, 8, 64>(a, st) : start<64, 8, 64>(a, st);
 }
 

@@ -606,8 +606,9 @@ def test_tree_attn_scales_far_apart(dev, torch, bits, name):
     check_tree(dev, torch, q, kv, table, lens, mask, bits, 2, 128, scale=0.25)
 
 
-# More than 16 rows a key head in bfloat16 take the tcgen05 form where the pages
-# are whole 16-key runs: 32 rows at a time up to 32, else 64.
+# More than 16 rows a key head of 128 values, or 32 of 64, in bfloat16 take the
+# tcgen05 form where the pages are whole 16-key runs: 32 rows at a time up to
+# 32, else 64.
 WIDE = [(8, 8, 2), (33, 2, 1), (64, 4, 1), (17, 3, 1)]      # nodes, heads, kv_heads
 
 
