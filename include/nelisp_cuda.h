@@ -472,8 +472,8 @@ int nl_kv_move_dev(const nl_kv_move_args *args, void *stream);
  * nl_tree_attn_workspace_bytes(nodes, heads, kv_heads, head_dim) bytes,
  * 16-byte aligned, or is NULL for the library's own (calls that overlap in
  * time must then not share it).  Does not synchronise; with bf16 and more
- * than 16 rows (nodes x heads/kv_heads) it may wait on mbarriers (see
- * nl_wait_status). */
+ * than 16 rows (nodes x heads/kv_heads) it may wait on mbarriers, each wait
+ * bounded (see nl_wait_status). */
 typedef struct {
   nl_kv_cache cache;             /* its arrays are only read */
   int dtype;

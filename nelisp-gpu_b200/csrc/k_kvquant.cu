@@ -18,7 +18,10 @@
 // head is a step on both sides; U vectors are requested before the first is
 // used.  Codes and floats are turned into one another by adding 2^23 and its
 // like, two at a time: the conversion instructions run at a sixteenth of the
-// rate and bound the first form of these kernels.
+// rate and bound the first form of these kernels.  Append and read of 4,095
+// tokens of 20 heads of 128, float32, 8 bits: 35.7 us together, 5.9 TB/s, 0.90 of
+// a copy; of 16,384 tokens of 8 heads, bfloat16, 4 bits: 35.5 us, 4.8 TB/s, where
+// the quantiser's issue is the bound (two reductions, a code a value).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

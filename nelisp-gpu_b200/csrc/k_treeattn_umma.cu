@@ -28,6 +28,16 @@
 //               descriptors are formed in uniform registers: from a single
 //               thread's branch the issue of a tile took longer than its work.
 // The registers of the launch are shared out anew among the roles.
+//
+// What bounds it: a tile takes about 3,150 cycles (131,071 keys, 16 nodes of 4
+// heads, 8 bits: 107 us, 2.6 TB/s, 321 TF/s) with the tensor cores 17% busy, issue 58%, and shared memory -- codes in and out, values
+// out and in again, weights, the rows' factors and references -- about 80%.  No
+// role is the one: each is 2,000 to 2,300 cycles busy a tile at 5 to 8 cycles an
+// instruction, and waits the rest of it for another.  Measured and not taken: two
+// streams of score warps on alternate tiles (32 rows, 4 bits: 68 us, not 62), the
+// vote by a barrier that is waited for after the exponentials (125, not 110), the
+// scores' columns released before the weights (113), deeper batches of loads in
+// the conversions (110 to 115).
 // The stages run on over the end of an item: the next item's codes are on
 // their way and converted while the last one's output is written.
 //
@@ -556,7 +566,8 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           for (int i = 0; i < Per / 8; i++) raw[i] = live ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
           auto value = [&](int i) {
             const uint4 &x = raw[i / 8];
-            const uint32_t u = i % 8 / 2 == 0 ? x.x : i % 8 / 2 == 1 ? x.y : i % 8 / 2 == 2 ? x.z : x.w;
+            const uint32_t w2 = i % 8 / 2;
+            const uint32_t u = w2 == 0 ? x.x : w2 == 1 ? x.y : w2 == 2 ? x.z : x.w;
             return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
           };
 #pragma unroll
@@ -639,7 +650,8 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
                 Pair x = pair(__uint_as_float(s[i + j]), __uint_as_float(s[i + j + 1]));
                 x = mul2(x, sk2);
                 if (BITS == 4) x = fma2(mk2, j ? pair(q.z, q.w) : pair(q.x, q.y), x);
-                x = fma2(x, j ? pair(f.z, f.w) : pair(f.x, f.y), j ? pair(r.z, r.w) : pair(r.x, r.y));
+                x = fma2(x, j ? pair(f.z, f.w) : pair(f.x, f.y),
+                         j ? pair(r.z, r.w) : pair(r.x, r.y));
                 const float2 y = unpair(x);
                 s[i + j] = __float_as_uint(y.x);
                 s[i + j + 1] = __float_as_uint(y.y);
@@ -649,8 +661,9 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
 #pragma unroll
               for (int i = 0; i < H; i++) {
                 const uint64_t m = masks[n + i];
-                const bool seen = have && (key < prefix ? m != 0
-                                                        : key - prefix < 64 && (m >> (key - prefix) & 1));
+                const uint32_t node = key - prefix;
+                const bool seen =
+                    have && (key < prefix ? m != 0 : node < 64 && (m >> node & 1));
                 if (!seen) s[i] = 0xff800000u;             // -inf
               }
             }
@@ -803,7 +816,8 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
 #pragma unroll
             for (int i = 0; i < H; i++) {
               const uint32_t n = n0 + i;
-              const float k = keep[n], v = k == 0.0f ? 0.0f : fmaf(__uint_as_float(o[i]), k, qsum[n]);
+              const float k = keep[n];
+              const float v = k == 0.0f ? 0.0f : fmaf(__uint_as_float(o[i]), k, qsum[n]);
               const uint64_t at = offs[n];
               if (part_of) part[i * HD] = v;
               else if (at != ~0ull) ((__nv_bfloat16 *)a.o)[at + d] = __float2bfloat16_rn(v);
@@ -811,7 +825,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           }
         }
         fence_before();
-        soft_sync<L::Soft>();                         // the rows are read: the next item may write them
+        soft_sync<L::Soft>();              // the rows are read: the next item may write them
       }
     }
   }

@@ -29,6 +29,12 @@
 // kernel joins.  The WR warps of 32 keys share a cp.async ring, and nothing
 // else synchronises the CTA until an item ends.
 //
+// What bounds it: with few rows the loads.  8 sequences of 4,096 keys, 32 heads
+// of 128, float32, 8 bits: 62.6 us for 277 MB, 0.67 of a copy's rate; the same
+// without the products 50, the join 3.  With many rows the issue of products and
+// weights: the table at start_rows; in bfloat16 the tcgen05 form
+// (k_treeattn_umma.cu) takes over there.
+//
 // Key order.  Row r of a 16-key tile is key 4 (r % 8 / 2) + r % 2 + 2 (r / 8):
 // the second product then takes four successive value rows a lane.  The K
 // index of the score product is permuted so a lane's part of a key is whole
@@ -99,7 +105,7 @@ template <typename T, int HD, int BITS, int NR, int WR, bool PACK> struct Plan {
   static constexpr int Q = Terms * Rows * HD * 2;           // query fragments
   static constexpr int Stages = WR > 1 ? 4 : G::RB <= 64 ? 4 : G::RB <= 128 ? 3 : 2;
   static constexpr int Ring = WK * Stages * G::Stage;
-  static constexpr int Pitch = HD + 4;                      // floats of a row when states are joined
+  static constexpr int Pitch = HD + 4;                     // floats of a row when states are joined
   static constexpr int Join = WK * Rows * Pitch * 4;        // over the fragments and the ring
   // row factors, row sums, masks, per-warp (max, sum)
   static constexpr int Small = Rows * 4 + Rows * 4 + Rows * 8 + WK * Rows * 8;
@@ -328,7 +334,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
             for (int e = 0; e < Terms; e++) {
               const uint8_t *from = qf + e * (P::Rows * HD * 2);
               if (NR == 1) {
-                const uint2 x = *reinterpret_cast<const uint2 *>(from + fragment(8 * wr + g, step, t));
+                const uint2 x =
+                    *reinterpret_cast<const uint2 *>(from + fragment(8 * wr + g, step, t));
                 q[e][0][0] = x.x; q[e][0][1] = x.y;
               } else {
 #pragma unroll
@@ -479,7 +486,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
             }
             __half2 hi = __floats2half2_rn(e[0], e[1]);
             if (PACK) {
-              const __half2 low = __floats2half2_rn(e[0] - __low2float(hi), e[1] - __high2float(hi));
+              const __half2 low =
+                  __floats2half2_rn(e[0] - __low2float(hi), e[1] - __high2float(hi));
               if (t & 2) hi = low;
             }
             p[0][n][u] = transpose8(h2(hi));
@@ -501,7 +509,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
             if (VW == 1) {
               w[i][0] = *reinterpret_cast<const uint32_t *>(vc + G::v_at(key, g / 4) + g % 4 * 4);
             } else if (VW == 2) {
-              const uint2 y = *reinterpret_cast<const uint2 *>(vc + G::v_at(key, g / 2) + g % 2 * 8);
+              const uint2 y =
+                  *reinterpret_cast<const uint2 *>(vc + G::v_at(key, g / 2) + g % 2 * 8);
               w[i][0] = y.x; w[i][VL - 1] = y.y;
             } else {
               const uint4 y = *reinterpret_cast<const uint4 *>(vc + G::v_at(key, g + 8 * h));
@@ -748,8 +757,8 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, P::Bytes);
     if (e != cudaSuccess) return e;
     int n = 0;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, tree_attn_kernel<T, HD, BITS, NR, WR, PACK>,
-                                                      kTreeThreads, P::Bytes);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+        &n, tree_attn_kernel<T, HD, BITS, NR, WR, PACK>, kTreeThreads, P::Bytes);
     if (e != cudaSuccess) return e;
     per_sm = n < 1 ? 1 : n > 4 ? 4 : n;
   }
@@ -763,14 +772,28 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
 }
 template <typename T, int HD, int BITS>
 cudaError_t start_rows(TreeArgs &a, cudaStream_t st) {
-  constexpr int Most = HD == 256 ? 2 : 4;        // row tiles a warp has registers for
+  // Row tiles of a warp: as many as it has registers for, since every warp that
+  // shares keys converts their codes again (us, 4 sequences of 32,768 keys, 8 key
+  // heads of 128, 8 bits / 4 bits):
+  //   rows               16         32         64         128
+  //   bf16  4 a warp   68/ 72    104/110    181/197    334/371
+  //         half       87/100    115/128    216/240    418/468
+  //   f32   4 a warp   90/ 90    225/158    312/293    561/562
+  //         half      111/117    155/164    297/321    622/677
+  // (half: 1 of 16 rows, 2 of more).  With both terms of float32 four tiles of 8
+  // bits spill, which only the joint reading of 128 rows makes up for; in 4 bits a
+  // step has one lane part of codes to hold, not two.
+  constexpr int Most = HD == 256 ? 2 : 4;
+  constexpr int Part = sizeof(T) == 4 && HD == 128 && BITS == 8 ? 2 : Most;
+  // Up to four rows of float32: both terms in one 8-row tile (8 sequences of 4,096
+  // keys, 32 heads, 8 bits: 62.6 us; as two tiles 72.8).
   if constexpr (sizeof(T) == 4) {
     if (a.rows <= 4) return start<T, HD, BITS, 1, 1, true>(a, st);
   }
   if (a.rows_at_once == 8) return start<T, HD, BITS, 1, 1>(a, st);
   if (a.rows_at_once == 16) return start<T, HD, BITS, 2, 1>(a, st);
-  if (a.rows_at_once == 32) return start<T, HD, BITS, Most, 4 / Most>(a, st);
-  if (a.rows_at_once == 64) return start<T, HD, BITS, Most, 8 / Most>(a, st);
+  if (a.rows_at_once == 32) return start<T, HD, BITS, Part, 4 / Part>(a, st);
+  if (a.rows_at_once == 64) return start<T, HD, BITS, Part, 8 / Part>(a, st);
   if constexpr (Most == 4) return start<T, HD, BITS, Most, 4>(a, st);
   return cudaErrorInvalidValue;
 }

@@ -70,8 +70,9 @@ def test_packed_structures_match_the_header(tmp_path):
     src = tmp_path / "sizes.c"
     src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "nelisp_cuda.h"\n'
                    "int main(void) {\n" +
-                   "".join(f'printf("%zu %zu\\n", offsetof({n}, {last}) + sizeof((({n} *)0)->{last}), '
-                           f"sizeof({n}));\n" for n, (_, last) in names.items()) + "}\n")
+                   "".join(f'printf("%zu %zu\\n", offsetof({n}, {last}) + '
+                           f"sizeof((({n} *)0)->{last}), sizeof({n}));\n"
+                           for n, (_, last) in names.items()) + "}\n")
     exe = tmp_path / "sizes"
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), "-o", str(exe), str(src)],
                    check=True)
