@@ -13,15 +13,17 @@
 //
 // Bound by memory.  As in k_qknorm.cu a group of lanes holds a head vector,
 // two 16-byte chunks a lane half a vector apart, so each request of a group is
-// one contiguous run.  A warp takes the key or the value heads of a token (some
-// of them, while there are few tokens), so the slot is looked up once and a
-// head is a step on both sides; U vectors are requested before the first is
-// used.  Codes and floats are turned into one another by adding 2^23 and its
-// like, two at a time: the conversion instructions run at a sixteenth of the
-// rate and bound the first form of these kernels.  Append and read of 4,095
-// tokens of 20 heads of 128, float32, 8 bits: 35.7 us together, 5.9 TB/s, 0.90 of
-// a copy; of 16,384 tokens of 8 heads, bfloat16, 4 bits: 35.5 us, 4.8 TB/s, where
-// the quantiser's issue is the bound (two reductions, a code a value).
+// one contiguous run.  A warp takes a token's key and value heads (some of
+// them, while there are few tokens), so the slot is looked up once and a head
+// is a step on both sides; U vectors are requested before the first is used.
+// Their extremes are joined together, each lane ends with one vector's, divides
+// for that one alone, and the group shares the quotients: a division costs as
+// much as two values.  Codes and floats are turned into one another by adding
+// 2^23 and its like, two at a time: the conversion instructions run at a
+// sixteenth of the rate and bound the first form of these kernels.  Append and
+// read of 4,095 tokens of 20 heads of 128, float32, 8 bits: 33.9 us together, 6.2
+// TB/s, 0.95 of a copy; of 16,384 tokens of 8 heads, bfloat16, 4 bits: 29.5 us,
+// 5.8 TB/s, where issue is the bound.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -60,7 +62,7 @@ struct KvRows {
   void *out[2];                  // read
   uint64_t stride[2];
   const int32_t *slot;
-  uint32_t n, per_job, jobs_per_part;   // tokens; heads a warp takes, its share of a token's
+  uint32_t n, per_job, jobs;     // tokens; heads a warp takes, and how many warps a token
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -98,8 +100,7 @@ __device__ __forceinline__ void encode(const Pair *v, float lo, float inv, uint3
     const float2 f = unpair(v[i / 2]);
     float x = i & 1 ? f.y : f.x;
     if (BITS == 4) x = __fsub_rn(x, lo);
-    x = __fmul_rn(x, inv);
-    if (BITS == 4) x = fminf(x, 15.0f);
+    x = __fmul_rn(x, inv);         // (4 bits: it rounds to at most 15, by lo and s)
     c[i] = __float_as_uint(__fadd_rn(x, magic));
   }
   if (BITS == 8) {
@@ -142,22 +143,89 @@ __device__ __forceinline__ float bf16_up(float x) {   // of a positive finite x
   return __uint_as_float((__float_as_uint(x) + 0xffffu) & 0xffff0000u);
 }
 
-// A warp's job: some heads of the keys or the values of a token.
+// A warp's job: some of a token's heads, the values' after the keys'.
 struct Job {
-  uint32_t token, kv, h0, h1;
+  uint32_t token, h0, h1;
   uint32_t row;                  // of head 0 in the pool, or ~0
 };
 __device__ __forceinline__ Job job_of(const KvRows &r, const KvPool &p, uint64_t i) {
   Job j;
-  const uint32_t per = 2 * r.jobs_per_part;
-  j.token = (uint32_t)(i / per);
-  const uint32_t rest = (uint32_t)(i - (uint64_t)j.token * per);
-  j.kv = rest >= r.jobs_per_part;
-  j.h0 = (j.kv ? rest - r.jobs_per_part : rest) * r.per_job;
-  j.h1 = min(j.h0 + r.per_job, p.kv_heads);
+  j.token = r.jobs == 1 ? (uint32_t)i : (uint32_t)(i / r.jobs);
+  j.h0 = (uint32_t)(i - (uint64_t)j.token * r.jobs) * r.per_job;
+  j.h1 = min(j.h0 + r.per_job, 2 * p.kv_heads);
   const uint32_t slot = (uint32_t)__ldg(r.slot + j.token), block = slot / p.block_size;
   j.row = block < p.num_blocks ? kv_row(p, block, slot - block * p.block_size, 0) : ~0u;
   return j;
+}
+// Head HH of a token: keys or values, which of them, and its row in the pool.
+struct Head {
+  uint32_t kv, head, at;
+};
+__device__ __forceinline__ Head head_of(const KvPool &p, const Job &job, uint32_t hh) {
+  Head h;
+  h.kv = hh >= p.kv_heads;
+  h.head = h.kv ? hh - p.kv_heads : hh;
+  h.at = job.row + h.head * p.block_size;
+  return h;
+}
+
+// The largest and the smallest of a lane's part of a vector (8 bits: the largest
+// magnitude, and nothing), NaN if any is.
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T, int BITS>
+__device__ __forceinline__ void extremes(const uint4 (&w)[2], float *hi, float *lo) {
+  const uint32_t v[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+  if constexpr (sizeof(T) == 4) {
+    auto of = [&](int i) {
+      const float f = __uint_as_float(v[i]);
+      return BITS == 8 ? fabsf(f) : f;
+    };
+    float h = of(0), l = of(0);
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+      h = max_nan(h, of(i));
+      if (BITS == 4) l = min_nan(l, of(i));
+    }
+    *hi = h;
+    *lo = l;
+  } else {                         // two at a time; exact
+    auto of = [&](int i) { return BITS == 8 ? v[i] & 0x7fff7fffu : v[i]; };
+    uint32_t h = of(0), l = of(0);
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+      h = max2_nan(h, of(i));
+      if (BITS == 4) l = min2_nan(l, of(i));
+    }
+    *hi = max_nan(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+    *lo = min_nan(__uint_as_float(l << 16), __uint_as_float(l & 0xffff0000u));
+  }
+}
+// Of U values a lane, the join over the lanes of a group of G: lane j of it gets
+// that of value j / (G / U), in log2(G) + U - 1 - log2(U) exchanges.
+template <int G, int U, typename F>
+__device__ __forceinline__ float across(float (&v)[U], uint32_t j, F join) {
+  int o = G / 2;
+#pragma unroll
+  for (int n = U / 2; n > 0; n /= 2, o /= 2) {
+    const bool high = j & o;
+#pragma unroll
+    for (int i = 0; i < n; i++) {
+      const float give = high ? v[i] : v[i + n], have = high ? v[i + n] : v[i];
+      v[i] = join(have, __shfl_xor_sync(0xffffffffu, give, o));
+    }
+  }
+#pragma unroll
+  for (; o > 0; o /= 2) v[0] = join(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+  return v[0];
 }
 
 template <typename T, int HD, int BITS, int U>
@@ -168,12 +236,12 @@ kv_append_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPoo
   pdl_trigger();
   pdl_wait();
   const uint32_t lane = threadIdx.x & 31, j = lane % G, mine = lane / G;
-  const uint64_t jobs = (uint64_t)r.n * 2 * r.jobs_per_part;
+  const uint64_t jobs = (uint64_t)r.n * r.jobs;
   for (uint64_t i = (uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < jobs;
        i += (uint64_t)gridDim.x * (kThreads / 32)) {
     const Job job = job_of(r, p, i);
-    const T *x = (const T *)r.in[job.kv] + (uint64_t)job.token * r.stride[job.kv];
-    uint8_t *code = p.code[job.kv];
+    const T *x[2] = {(const T *)r.in[0] + (uint64_t)job.token * r.stride[0],
+                     (const T *)r.in[1] + (uint64_t)job.token * r.stride[1]};
     for (uint32_t h = job.h0; h < job.h1; h += H * U) {
       uint4 w[U][2];
 #pragma unroll
@@ -181,70 +249,73 @@ kv_append_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPoo
         const uint32_t hh = h + u * H + mine;
         w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
         if (hh < job.h1) {
-          const uint4 *v = reinterpret_cast<const uint4 *>(x + (uint64_t)hh * HD);
+          const Head at = head_of(p, job, hh);
+          const uint4 *v = reinterpret_cast<const uint4 *>((at.kv ? x[1] : x[0]) +
+                                                           (uint64_t)at.head * HD);
           w[u][0] = __ldcs(v + j);
           w[u][1] = __ldcs(v + j + G);
         }
       }
+      // a lane makes the parameters of one of the U vectors, and the group shares
+      // them: the divisions are most of what a vector costs besides its values
+      float hi[U], lo[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) extremes<T, BITS>(w[u], &hi[u], &lo[u]);
+      const float top = across<G, U>(hi, j, max_nan);
+      float s, low = 0.0f, inv = 0.0f;
+      uint32_t word;
+      bool bad;
+      if (BITS == 8) {
+        const bool some = top >= 127.0f * kKvTiny;
+        s = some ? __fdiv_rn(top, 127.0f) : 0.0f;
+        if (some) inv = __fdiv_rn(127.0f, top);
+        bad = !(top < INFINITY);
+        word = bad ? 0x7fc00000u : __float_as_uint(s);
+      } else {
+        low = __bfloat162float(__float2bfloat16_rd(across<G, U>(lo, j, min_nan)));
+        const float range = __fsub_rn(top, low);
+        s = bf16_up(__fdiv_rn(range, 15.0f));
+        const bool some = s >= kKvTiny;
+        if (some) inv = __fdiv_rn(1.0f, s);
+        else s = 0.0f;
+        bad = !(range < INFINITY);
+        word = bad ? 0x7fc0u
+                   : __float_as_uint(s) >> 16 | (__float_as_uint(low) & 0xffff0000u);
+      }
+      if (bad) inv = -1.0f;        // the scale says so: the codes are those of zero
+      if (j % (G / U) == 0) {
+        const uint32_t hh = h + j / (G / U) * H + mine;
+        if (hh < job.h1 && job.row != ~0u) {
+          const Head at = head_of(p, job, hh);
+          (at.kv ? p.param[1] : p.param[0])[at.at] = word;
+        }
+      }
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const uint32_t hh = h + u * H + mine;
+        const uint32_t hh = h + u * H + mine, from = mine * G + u * (G / U);
+        float by = __shfl_sync(0xffffffffu, inv, from);
+        float off = BITS == 4 ? __shfl_sync(0xffffffffu, low, from) : 0.0f;
         Pair v[N];
         Chunk<T>::get(w[u][0], v);
         Chunk<T>::get(w[u][1], v + N / 2);
-        const float2 f0 = unpair(v[0]);
-        float hi = BITS == 8 ? max_nan(fabsf(f0.x), fabsf(f0.y)) : max_nan(f0.x, f0.y);
-        float lo = min_nan(f0.x, f0.y);
-#pragma unroll
-        for (int e = 1; e < N; e++) {
-          const float2 f = unpair(v[e]);
-          hi = BITS == 8 ? max_nan(hi, max_nan(fabsf(f.x), fabsf(f.y)))
-                         : max_nan(hi, max_nan(f.x, f.y));
-          if (BITS == 4) lo = min_nan(lo, min_nan(f.x, f.y));
-        }
-#pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) {
-          hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-          if (BITS == 4) lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        }
-        float s, inv = 0.0f;
-        uint32_t word;
-        bool bad;
-        if (BITS == 8) {
-          const bool some = hi >= 127.0f * kKvTiny;
-          s = some ? __fdiv_rn(hi, 127.0f) : 0.0f;
-          if (some) inv = __fdiv_rn(127.0f, hi);
-          bad = !(hi < INFINITY);
-          word = bad ? 0x7fc00000u : __float_as_uint(s);
-        } else {
-          lo = __bfloat162float(__float2bfloat16_rd(lo));
-          const float range = __fsub_rn(hi, lo);
-          s = bf16_up(__fdiv_rn(range, 15.0f));
-          const bool some = s >= kKvTiny;
-          if (some) inv = __fdiv_rn(1.0f, s);
-          else s = 0.0f;
-          bad = !(range < INFINITY);
-          word = bad ? 0x7fc0u
-                     : __float_as_uint(s) >> 16 | (__float_as_uint(lo) & 0xffff0000u);
-        }
-        if (bad) {                 // the scale says so: the codes are those of zero
+        if (by < 0.0f) {
 #pragma unroll
           for (int e = 0; e < N; e++) v[e] = 0;
-          lo = inv = 0.0f;
+          by = off = 0.0f;
         }
         if (hh < job.h1 && job.row != ~0u) {
-          const uint32_t at = job.row + hh * p.block_size;
-          uint8_t *to = code + (uint64_t)at * (HD * BITS / 8) + j * CB;
+          const Head at = head_of(p, job, hh);
+          uint8_t *to = (at.kv ? p.code[1] : p.code[0]) +
+                        (uint64_t)at.at * (HD * BITS / 8) + j * CB;
 #pragma unroll
           for (int k = 0; k < 2; k++) {
             uint32_t c[2];
-            encode<BITS, N>(v + k * (N / 2), lo, inv, c);
+            encode<BITS, N>(v + k * (N / 2), off, by, c);
             W t;
             if constexpr (CB == 8) t = make_uint2(c[0], c[1]);
             else t = (W)c[0];
             *reinterpret_cast<W *>(to + k * G * CB) = t;
           }
-          if (j == 0) p.param[job.kv][at] = word;
         }
       }
     }
@@ -259,13 +330,12 @@ kv_read_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPool 
   pdl_trigger();
   pdl_wait();
   const uint32_t lane = threadIdx.x & 31, j = lane % G, mine = lane / G;
-  const uint64_t jobs = (uint64_t)r.n * 2 * r.jobs_per_part;
+  const uint64_t jobs = (uint64_t)r.n * r.jobs;
   for (uint64_t i = (uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < jobs;
        i += (uint64_t)gridDim.x * (kThreads / 32)) {
     const Job job = job_of(r, p, i);
-    T *y = (T *)r.out[job.kv] + (uint64_t)job.token * r.stride[job.kv];
-    const uint8_t *code = p.code[job.kv];
-    const uint32_t *param = p.param[job.kv];
+    T *y[2] = {(T *)r.out[0] + (uint64_t)job.token * r.stride[0],
+               (T *)r.out[1] + (uint64_t)job.token * r.stride[1]};
     for (uint32_t h = job.h0; h < job.h1; h += H * U) {
       W w[U][2];
       uint32_t word[U];
@@ -275,9 +345,10 @@ kv_read_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPool 
         word[u] = 0;
         w[u][0] = w[u][1] = W{};
         if (hh < job.h1 && job.row != ~0u) {
-          const uint32_t at = job.row + hh * p.block_size;
-          const uint8_t *from = code + (uint64_t)at * (HD * BITS / 8) + j * CB;
-          word[u] = param[at];
+          const Head at = head_of(p, job, hh);
+          const uint8_t *from = (at.kv ? p.code[1] : p.code[0]) +
+                                (uint64_t)at.at * (HD * BITS / 8) + j * CB;
+          word[u] = (at.kv ? p.param[1] : p.param[0])[at.at];
           w[u][0] = *reinterpret_cast<const W *>(from);
           w[u][1] = *reinterpret_cast<const W *>(from + G * CB);
         }
@@ -288,7 +359,8 @@ kv_read_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPool 
         if (hh >= job.h1) continue;
         const float s = __uint_as_float(BITS == 8 ? word[u] : word[u] << 16);
         const float lo = BITS == 8 ? 0.0f : __uint_as_float(word[u] & 0xffff0000u);
-        uint4 *to = reinterpret_cast<uint4 *>(y + (uint64_t)hh * HD) + j;
+        const Head at = head_of(p, job, hh);
+        uint4 *to = reinterpret_cast<uint4 *>((at.kv ? y[1] : y[0]) + (uint64_t)at.head * HD) + j;
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           uint32_t c[2];
@@ -338,20 +410,26 @@ kv_move_kernel(const __grid_constant__ KvPool p, const int32_t *src, const int32
 }
 
 // U vectors a group at a time (append + read of 4095 tokens of 20 heads of 128,
-// f32, 8 bits: 41.0 us with 2, 37.9 with 4; 16384 of 8 heads, bf16, 4 bits: 37.6
-// with 2, 50.9 with 4); at most 8 blocks an SM, and while there are fewer jobs
-// than warps a warp takes fewer heads.
+// f32, 8 bits: 40.9 us with 2, 37.6 with 4; 16384 of 8 heads, bf16, 4 bits: 34.1
+// with 2, 31.3 with 4).  Up to 16 blocks an SM, and a token's heads divided so
+// that there are as many jobs as warps (f32: 47.5 us with 4 blocks, 37.6 with 8,
+// 35.8 with 16 or 32), whole steps of U vectors each; with too few tokens for
+// that a vector a group, for the shortest call.
 template <typename T, int HD, int BITS>
 cudaError_t start(bool append, KvRows &r, const KvPool &p, cudaStream_t st) {
-  constexpr int U = sizeof(T) == 4 ? 4 : 2;
+  constexpr int U = 4;
   constexpr uint32_t H = 32 / (HD / (2 * Chunk<T>::N)), warps = kThreads / 32;
-  constexpr uint64_t most = 148 * 8;
-  uint32_t per = p.kv_heads;
-  while (per > H && (uint64_t)r.n * 2 * ((p.kv_heads + per - 1) / per) < most * warps)
-    per = (per + 1) / 2;
-  r.per_job = (per + H - 1) / H * H;
-  r.jobs_per_part = (p.kv_heads + r.per_job - 1) / r.per_job;
-  const uint64_t want = ceil_div64((uint64_t)r.n * 2 * r.jobs_per_part, warps);
+  constexpr uint64_t most = 148 * 16;
+  const uint32_t heads = 2 * p.kv_heads, steps = (heads + H * U - 1) / (H * U);
+  if ((uint64_t)r.n * steps >= 148 * warps) {
+    const uint64_t split = ceil_div64(most * warps, r.n);
+    const uint32_t jobs = split < steps ? (uint32_t)split : steps;
+    r.per_job = (steps + jobs - 1) / jobs * (H * U);
+  } else {
+    r.per_job = H;
+  }
+  r.jobs = (heads + r.per_job - 1) / r.per_job;
+  const uint64_t want = ceil_div64((uint64_t)r.n * r.jobs, warps);
   const dim3 grid((unsigned)(want < most ? want : most));
   return append ? launch_pdl(kv_append_kernel<T, HD, BITS, U>, grid, dim3(kThreads), 0, st, r, p)
                 : launch_pdl(kv_read_kernel<T, HD, BITS, U>, grid, dim3(kThreads), 0, st, r, p);
@@ -382,6 +460,8 @@ int rows_call(const char *what, bool append, const nl_kv_rows_args *args, void *
   if ((rc = kv_check_pool(what, fmt, p))) return rc;
   if (n == 0) return NL_OK;
   if (!r.slot) return set_error(NL_ERROR, "%s: null slots", what);
+  if (p.kv_heads > INT32_MAX)      // twice as many are counted in 32 bits
+    return set_error(NL_ERROR, "%s: %u kv heads", what, p.kv_heads);
   const uint32_t unit = dtype == NL_BF16 ? 8 : 4;
   for (int i = 0; i < 2; i++) {
     const void *x = append ? r.in[i] : r.out[i];
