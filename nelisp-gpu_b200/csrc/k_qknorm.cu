@@ -16,12 +16,12 @@
 // and no exchange of values.  A warp takes one row and walks its query or its
 // key heads with the row's products of gain, cosine and sine in registers;
 // blocks belong to one of the two parts, so a thread holds one gain (and one
-// set of gain gradients).  U vectors are requested before the first is used.
-// Arithmetic is two floats an instruction, all in 32 bits; the one rounding to
-// the output type is at the store.  8,192 rows of 40 heads of 128, bfloat16, one
-// row in twenty padding: 35.2 us, 4.9 TB/s, where the same loads and stores with
-// nothing between take 33.5; backward, 8,191 rows of 40 heads of 64: 33.1 us, 3.8
-// TB/s, bound by issue.
+// set of gain gradients).  The next vectors are on their way to shared memory
+// meanwhile, in runs of whole vectors whatever the pairs (forward), or to
+// registers.  Arithmetic is two floats an instruction, all in 32 bits; the one
+// rounding to the output type is at the store.  8,192 rows of 40 heads of 128,
+// bfloat16, one row in twenty padding: 30.7 us, 5.6 TB/s, 0.85 of a copy;
+// backward, 8,191 rows of 40 heads of 64: 33.1 us, 3.8 TB/s.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -118,10 +118,26 @@ __device__ __forceinline__ float group_sum(Pair p) {
   return v;
 }
 
-template <typename T, int G, bool HALF, bool BWD, int U, int PER_SM>
+// 16 bytes to shared memory on their way while others are worked on, or zeros.
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool some) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from),
+               "r"(some ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() {
+  asm volatile("cp.async.commit_group;\n" ::: "memory");
+}
+template <int AHEAD> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(AHEAD) : "memory");
+}
+
+// DEPTH steps of U vectors a group are on their way to shared memory (forward),
+// or the next one to registers (backward, DEPTH 0).
+template <typename T, int G, bool HALF, bool BWD, int U, int DEPTH, int PER_SM>
 __global__ void __launch_bounds__(kThreads, PER_SM)
 qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
-  constexpr int N = Chunk<T>::N, P = N / 2, H = 32 / G;
+  constexpr int N = Chunk<T>::N, P = N / 2, H = 32 / G, CH = BWD ? 4 : 2;
+  extern __shared__ uint4 ring[];
   pdl_trigger();
   pdl_wait();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = lane / G;
@@ -173,6 +189,47 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
   const uint64_t first = (uint64_t)block * kWarps + warp;
   int32_t pos = position(first), pos_next = position(first + step);
   angles(pos);
+  // The vectors to come, over the ends of jobs: a group copies one in two runs,
+  // whatever chunks its lanes then take.
+  uint4 *slots = ring + warp * (DEPTH * U * 64) + mine * (2 * G);
+  const uint32_t j = lane % G, chunks = a.head_dim / N;
+  const uint32_t slots_at = (uint32_t)__cvta_generic_to_shared(slots + j);
+  uint64_t next_job = first;
+  uint32_t next_h = 0, next_end = 0, into = 0, from = 0;
+  const T *next_x = nullptr;
+  auto aim = [&]() {
+    const uint32_t row = per_row == 1 ? (uint32_t)next_job : (uint32_t)(next_job / per_row);
+    next_h = per_row == 1 ? 0 : (uint32_t)(next_job % per_row) * a.per_job[part];
+    next_end = min(next_h + a.per_job[part], heads);
+    next_x = (const T *)a.x + (uint64_t)row * a.x_stride +
+             (uint64_t)((part ? a.heads[0] : 0) + next_h + mine) * a.head_dim + j * N;
+  };
+  auto fetch = [&]() {
+    if (next_job < jobs) {
+      const uint32_t to = slots_at + into * (U * 1024);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const bool some = next_h + mine + u * H < next_end;
+        const bool in0 = some && j < chunks, in1 = some && j + G < chunks;
+        const T *v = next_x + u * H * a.head_dim;
+        copy16(to + u * 1024, in0 ? v : (const T *)a.x, in0);
+        copy16(to + u * 1024 + G * 16, in1 ? v + G * N : (const T *)a.x, in1);
+      }
+      into = into + 1 == DEPTH ? 0 : into + 1;
+      next_h += H * U;
+      next_x += H * U * a.head_dim;
+      if (next_h >= next_end) {
+        next_job += step;
+        if (next_job < jobs) aim();
+      }
+    }
+    copy_commit();
+  };
+  if constexpr (DEPTH > 0) {
+    if (next_job < jobs) aim();
+#pragma unroll
+    for (int i = 0; i < DEPTH; i++) fetch();
+  }
   for (uint64_t job = first; job < jobs; job += step) {
     const uint32_t row = per_row == 1 ? (uint32_t)job : (uint32_t)(job / per_row);
     const uint32_t h0 = per_row == 1 ? 0 : (uint32_t)(job % per_row) * a.per_job[part];
@@ -199,29 +256,36 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
     pos_next = position(job + 2 * step);
     angles(pos);
     for (uint32_t h = h0; h < h1; h += H * U) {
-      uint4 w[U][2], d[BWD ? U : 1][2];
+      uint4 w[U][CH];
+      if constexpr (DEPTH > 0) {
+        copy_wait<DEPTH - 1>();
+        __syncwarp();
+        const uint4 *here = slots + from * (U * 64);
+        from = from + 1 == DEPTH ? 0 : from + 1;
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const uint32_t hh = h + u * H + mine;
-        const T *v = x + (uint64_t)hh * a.head_dim;
-        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
-        if (BWD) d[u % (BWD ? U : 1)][0] = d[u % (BWD ? U : 1)][1] = make_uint4(0, 0, 0, 0);
-        if (p.live && hh < h1) {
-          w[u][0] = __ldcs(reinterpret_cast<const uint4 *>(v + at0));
-          w[u][1] = __ldcs(reinterpret_cast<const uint4 *>(v + at1));
-          if (BWD) {
-            const T *g = dy + (uint64_t)hh * a.head_dim;
-            d[u % (BWD ? U : 1)][0] = *reinterpret_cast<const uint4 *>(g + at0);
-            d[u % (BWD ? U : 1)][1] = *reinterpret_cast<const uint4 *>(g + at1);
+        for (int u = 0; u < U; u++)
+          w[u][0] = p.live ? here[u * 64 + p.c0] : make_uint4(0, 0, 0, 0),
+          w[u][1] = p.live ? here[u * 64 + p.c1] : make_uint4(0, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const uint32_t hh = h + u * H + mine;
+#pragma unroll
+          for (int i = 0; i < CH; i++) w[u][i] = make_uint4(0, 0, 0, 0);
+          if (p.live && hh < h1) {
+            const T *v = x + (uint64_t)hh * a.head_dim, *g = dy + (uint64_t)hh * a.head_dim;
+            w[u][0] = __ldcs(reinterpret_cast<const uint4 *>(v + at0));
+            w[u][1] = __ldcs(reinterpret_cast<const uint4 *>(v + at1));
+            w[u][CH - 2] = *reinterpret_cast<const uint4 *>(g + at0);
+            w[u][CH - 1] = *reinterpret_cast<const uint4 *>(g + at1);
           }
         }
       }
       if (!real) {                 // a row of padding: nothing it holds counts
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
-          if (BWD) d[u % (BWD ? U : 1)][0] = d[u % (BWD ? U : 1)][1] = make_uint4(0, 0, 0, 0);
-        }
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int i = 0; i < CH; i++) w[u][i] = make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
@@ -244,7 +308,7 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
         } else {
           // t = u x: dg += r t, and dx = r g u - x r^3 mean(g t)
           Pair ua[P], ub[P], dot = 0;
-          split<T, HALF>(d[u % (BWD ? U : 1)][0], d[u % (BWD ? U : 1)][1], ua, ub);
+          split<T, HALF>(w[u][CH - 2], w[u][CH - 1], ua, ub);
 #pragma unroll
           for (int i = 0; i < P; i++) {
             const Pair y0 = ua[i], y1 = ub[i];
@@ -270,6 +334,10 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
           *reinterpret_cast<uint4 *>(to + at0) = y0;
           *reinterpret_cast<uint4 *>(to + at1) = y1;
         }
+      }
+      if constexpr (DEPTH > 0) {               // into the slots just read
+        __syncwarp();
+        fetch();
       }
     }
   }
@@ -327,14 +395,25 @@ qk_gain_sum_kernel(const float *partial, uint32_t blocks_q, uint32_t blocks_k, u
 
 template <typename T, int G, bool HALF, bool BWD>
 cudaError_t start(QkArgs &a, cudaStream_t st) {
-  // Vectors a group takes at a time, and blocks an SM.  8192 rows of 40 heads of
-  // 128, bf16: 37.2 us with 2 and 2; 40.9 with 4 and 2, 42.7 with 2 and 3 (which
-  // spills).  The same loads and stores with no arithmetic between: 33.5.
-  // Backward, 8191 rows of 40 heads of 64, bf16: 36.2 with 1 and 2, 46.3 with 2
-  // and 2 (spills).  A float32 lane holds half as many values.
-  constexpr int U = (BWD ? 1 : 2) * (sizeof(T) == 4 ? 2 : 1), PER_SM = 2;
-  return launch_pdl(qk_norm_rope_kernel<T, G, HALF, BWD, U, PER_SM>,
-                    dim3(a.blocks[0] + a.blocks[1]), dim3(kThreads), 0, st, a);
+  // Vectors a group takes at a time, steps on their way, blocks an SM.  Forward,
+  // 8192 rows of 40 heads of 128, bf16: 30.6 us with 1, 3 and 2; 33.1 with 1, 2,
+  // 2; 31.6 with 2, 2, 2.  With loads to registers instead 35.1, and with a lane
+  // copying its own chunks 31.5, but 20.0 and not 14.3 where these are two
+  // neighbours (3000 rows of 20 heads of 256, adjacent pairs).  4096 rows of 40
+  // heads, f32: 30.4 us with 2, 2 and 2; 31.3 with 2, 3, 2.
+  // Backward, 8191 rows of 40 heads of 64, bf16: 36.2 with 1 and 2 blocks, 46.3
+  // with 2 and 2 (spills).  A float32 lane holds half as many values.
+  constexpr int U = (sizeof(T) == 4 ? 2 : 1), DEPTH = BWD ? 0 : sizeof(T) == 4 ? 2 : 3, PER_SM = 2;
+  constexpr auto kernel = qk_norm_rope_kernel<T, G, HALF, BWD, U, DEPTH, PER_SM>;
+  constexpr int bytes = kWarps * DEPTH * U * 1024;
+  static bool configured = false;
+  if (!configured) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    configured = true;
+  }
+  return launch_pdl(kernel, dim3(a.blocks[0] + a.blocks[1]), dim3(kThreads), (size_t)bytes, st, a);
 }
 template <typename T, bool BWD>
 cudaError_t start_t(QkArgs &a, bool half, uint32_t group, cudaStream_t st) {
