@@ -17,11 +17,11 @@
 // key heads with the row's products of gain, cosine and sine in registers;
 // blocks belong to one of the two parts, so a thread holds one gain (and one
 // set of gain gradients).  The next vectors are on their way to shared memory
-// meanwhile, in runs of whole vectors whatever the pairs (forward), or to
-// registers.  Arithmetic is two floats an instruction, all in 32 bits; the one
+// meanwhile, in runs of whole vectors whatever the pairs.  Arithmetic is two floats an instruction, all in 32 bits; the one
 // rounding to the output type is at the store.  8,192 rows of 40 heads of 128,
-// bfloat16, one row in twenty padding: 30.7 us, 5.6 TB/s, 0.85 of a copy;
-// backward, 8,191 rows of 40 heads of 64: 33.1 us, 3.8 TB/s.
+// bfloat16, one row in twenty padding: 30.6 us, 5.6 TB/s, 0.86 of a copy;
+// backward, 8,191 rows of 40 heads of 64: 28.4 us, 4.5 TB/s, bound by the latency
+// of a step that few warps hide.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -131,8 +131,7 @@ template <int AHEAD> __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;\n" ::"n"(AHEAD) : "memory");
 }
 
-// DEPTH steps of U vectors a group are on their way to shared memory (forward),
-// or the next one to registers (backward, DEPTH 0).
+// DEPTH steps of U vectors a group are on their way to shared memory.
 template <typename T, int G, bool HALF, bool BWD, int U, int DEPTH, int PER_SM>
 __global__ void __launch_bounds__(kThreads, PER_SM)
 qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
@@ -191,33 +190,42 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
   angles(pos);
   // The vectors to come, over the ends of jobs: a group copies one in two runs,
   // whatever chunks its lanes then take.
-  uint4 *slots = ring + warp * (DEPTH * U * 64) + mine * (2 * G);
+  uint4 *slots = ring + warp * (DEPTH * U * CH * 32) + mine * (2 * G);
   const uint32_t j = lane % G, chunks = a.head_dim / N;
   const uint32_t slots_at = (uint32_t)__cvta_generic_to_shared(slots + j);
   uint64_t next_job = first;
   uint32_t next_h = 0, next_end = 0, into = 0, from = 0;
-  const T *next_x = nullptr;
+  const T *next_x = nullptr, *next_dy = nullptr;
   auto aim = [&]() {
     const uint32_t row = per_row == 1 ? (uint32_t)next_job : (uint32_t)(next_job / per_row);
     next_h = per_row == 1 ? 0 : (uint32_t)(next_job % per_row) * a.per_job[part];
     next_end = min(next_h + a.per_job[part], heads);
     next_x = (const T *)a.x + (uint64_t)row * a.x_stride +
              (uint64_t)((part ? a.heads[0] : 0) + next_h + mine) * a.head_dim + j * N;
+    if (BWD)
+      next_dy = (const T *)a.dy[part] + (uint64_t)row * a.dy_stride[part] +
+                (uint64_t)(next_h + mine) * a.head_dim + j * N;
   };
   auto fetch = [&]() {
     if (next_job < jobs) {
-      const uint32_t to = slots_at + into * (U * 1024);
+      const uint32_t to = slots_at + into * (U * CH * 512);
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const bool some = next_h + mine + u * H < next_end;
         const bool in0 = some && j < chunks, in1 = some && j + G < chunks;
         const T *v = next_x + u * H * a.head_dim;
-        copy16(to + u * 1024, in0 ? v : (const T *)a.x, in0);
-        copy16(to + u * 1024 + G * 16, in1 ? v + G * N : (const T *)a.x, in1);
+        copy16(to + u * CH * 512, in0 ? v : (const T *)a.x, in0);
+        copy16(to + u * CH * 512 + G * 16, in1 ? v + G * N : (const T *)a.x, in1);
+        if (BWD) {
+          const T *g = next_dy + u * H * a.head_dim;
+          copy16(to + u * CH * 512 + 1024, in0 ? g : (const T *)a.x, in0);
+          copy16(to + u * CH * 512 + 1024 + G * 16, in1 ? g + G * N : (const T *)a.x, in1);
+        }
       }
       into = into + 1 == DEPTH ? 0 : into + 1;
       next_h += H * U;
       next_x += H * U * a.head_dim;
+      if (BWD) next_dy += H * U * a.head_dim;
       if (next_h >= next_end) {
         next_job += step;
         if (next_job < jobs) aim();
@@ -225,19 +233,14 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
     }
     copy_commit();
   };
-  if constexpr (DEPTH > 0) {
-    if (next_job < jobs) aim();
+  if (next_job < jobs) aim();
 #pragma unroll
-    for (int i = 0; i < DEPTH; i++) fetch();
-  }
+  for (int i = 0; i < DEPTH; i++) fetch();
   for (uint64_t job = first; job < jobs; job += step) {
     const uint32_t row = per_row == 1 ? (uint32_t)job : (uint32_t)(job / per_row);
     const uint32_t h0 = per_row == 1 ? 0 : (uint32_t)(job % per_row) * a.per_job[part];
     const uint32_t h1 = min(h0 + a.per_job[part], heads);
     const bool real = (uint32_t)pos < a.rope_rows;
-    const T *x = (const T *)a.x + (uint64_t)row * a.x_stride +
-                 (part ? (uint64_t)a.heads[0] * a.head_dim : 0);
-    const T *dy = BWD ? (const T *)a.dy[part] + (uint64_t)row * a.dy_stride[part] : nullptr;
     T *out = (T *)a.out[part] + (uint64_t)row * a.out_stride[part];
     // Forward: ca = ga c, sa = ga s, cb = gb c, sb = -gb s, for
     // y_a = r (a ca + b sb), y_b = r (a sa + b cb).  Backward: ca = c, sa = s,
@@ -257,30 +260,16 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
     angles(pos);
     for (uint32_t h = h0; h < h1; h += H * U) {
       uint4 w[U][CH];
-      if constexpr (DEPTH > 0) {
-        copy_wait<DEPTH - 1>();
-        __syncwarp();
-        const uint4 *here = slots + from * (U * 64);
-        from = from + 1 == DEPTH ? 0 : from + 1;
+      copy_wait<DEPTH - 1>();
+      __syncwarp();
+      const uint4 *here = slots + from * (U * CH * 32);
+      from = from + 1 == DEPTH ? 0 : from + 1;
 #pragma unroll
-        for (int u = 0; u < U; u++)
-          w[u][0] = p.live ? here[u * 64 + p.c0] : make_uint4(0, 0, 0, 0),
-          w[u][1] = p.live ? here[u * 64 + p.c1] : make_uint4(0, 0, 0, 0);
-      } else {
+      for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          const uint32_t hh = h + u * H + mine;
-#pragma unroll
-          for (int i = 0; i < CH; i++) w[u][i] = make_uint4(0, 0, 0, 0);
-          if (p.live && hh < h1) {
-            const T *v = x + (uint64_t)hh * a.head_dim, *g = dy + (uint64_t)hh * a.head_dim;
-            w[u][0] = __ldcs(reinterpret_cast<const uint4 *>(v + at0));
-            w[u][1] = __ldcs(reinterpret_cast<const uint4 *>(v + at1));
-            w[u][CH - 2] = *reinterpret_cast<const uint4 *>(g + at0);
-            w[u][CH - 1] = *reinterpret_cast<const uint4 *>(g + at1);
-          }
-        }
-      }
+        for (int i = 0; i < CH; i++)
+          w[u][i] = p.live ? here[(u * CH + i / 2 * 2) * 32 + (i % 2 ? p.c1 : p.c0)]
+                           : make_uint4(0, 0, 0, 0);
       if (!real) {                 // a row of padding: nothing it holds counts
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -335,10 +324,8 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
           *reinterpret_cast<uint4 *>(to + at1) = y1;
         }
       }
-      if constexpr (DEPTH > 0) {               // into the slots just read
-        __syncwarp();
-        fetch();
-      }
+      __syncwarp();
+      fetch();                     // into the slots just read
     }
   }
   if (BWD) {
@@ -393,6 +380,8 @@ qk_gain_sum_kernel(const float *partial, uint32_t blocks_q, uint32_t blocks_k, u
   }
 }
 
+template <typename T, bool BWD> constexpr int per_sm = BWD && sizeof(T) == 2 ? 1 : 2;
+
 template <typename T, int G, bool HALF, bool BWD>
 cudaError_t start(QkArgs &a, cudaStream_t st) {
   // Vectors a group takes at a time, steps on their way, blocks an SM.  Forward,
@@ -401,11 +390,15 @@ cudaError_t start(QkArgs &a, cudaStream_t st) {
   // copying its own chunks 31.5, but 20.0 and not 14.3 where these are two
   // neighbours (3000 rows of 20 heads of 256, adjacent pairs).  4096 rows of 40
   // heads, f32: 30.4 us with 2, 2 and 2; 31.3 with 2, 3, 2.
-  // Backward, 8191 rows of 40 heads of 64, bf16: 36.2 with 1 and 2 blocks, 46.3
-  // with 2 and 2 (spills).  A float32 lane holds half as many values.
-  constexpr int U = (sizeof(T) == 4 ? 2 : 1), DEPTH = BWD ? 0 : sizeof(T) == 4 ? 2 : 3, PER_SM = 2;
+  // Backward, 8192 rows of 40 heads, bf16, of 128 / of 64 (adjacent pairs): 45.8 /
+  // 28.4 with 1, 4 and 1 block; 50.9 / 32.3 with 1, 3 and 2 (whose 128 registers
+  // spill), 46.3 / 36.5 with 2, 2 and 1, 62.0 / 33.4 with 1, loads to registers
+  // and 2.  4096 rows of 40 heads of 128, f32: 45.4 with 2, 2 and 2; 45.6 with 2, 4
+  // and 1; 4096 rows of 40 heads of 64: 25.7 and 26.5.
+  constexpr int U = sizeof(T) == 4 ? 2 : 1, DEPTH = sizeof(T) == 4 ? 2 : BWD ? 4 : 3,
+                PER_SM = per_sm<T, BWD>;
   constexpr auto kernel = qk_norm_rope_kernel<T, G, HALF, BWD, U, DEPTH, PER_SM>;
-  constexpr int bytes = kWarps * DEPTH * U * 1024;
+  constexpr int bytes = kWarps * DEPTH * U * (BWD ? 2048 : 1024);
   static bool configured = false;
   if (!configured) {
     const cudaError_t e =
@@ -445,15 +438,15 @@ constexpr uint32_t kMaxBlocks = 148 * 2;
 constexpr uint32_t kRowCost = 4;
 
 // How a launch divides n rows of the two parts' heads: the blocks (at most
-// kMaxBlocks) in proportion to the heads; a warp takes whole rows once there
+// MAX_BLOCKS) in proportion to the heads; a warp takes whole rows once there
 // are enough of them to fill the blocks' warps, and otherwise as few heads as a
 // warp holds at a time.
-void divide(QkArgs &a, uint32_t at_once) {
+void divide(QkArgs &a, uint32_t at_once, uint32_t max_blocks) {
   const uint32_t all = a.heads[0] + a.heads[1];
   for (int p = 0; p < 2; p++) {
-    uint64_t most = (uint64_t)kMaxBlocks * (a.heads[p] + kRowCost) / (all + 2 * kRowCost);
+    uint64_t most = (uint64_t)max_blocks * (a.heads[p] + kRowCost) / (all + 2 * kRowCost);
     if (most < 1) most = 1;
-    if (p == 1 && most + a.blocks[0] > kMaxBlocks) most = kMaxBlocks - a.blocks[0];
+    if (p == 1 && most + a.blocks[0] > max_blocks) most = max_blocks - a.blocks[0];
     uint32_t per = a.heads[p];
     while (per > at_once && (uint64_t)a.n * ((a.heads[p] + per - 1) / per) < most * kWarps)
       per = (per + 1) / 2;
@@ -531,7 +524,7 @@ extern "C" int nl_qk_norm_rope_dev(const nl_qk_norm_rope_args *args, void *strea
     return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const uint32_t group = group_of(dtype, x.head_dim);
-  divide(a, 32 / group);
+  divide(a, 32 / group, kMaxBlocks);
   const bool half = pairs == NL_PAIRS_HALF;
   const cudaError_t e = dtype == NL_BF16 ? start_t<__nv_bfloat16, false>(a, half, group, st)
                                          : start_t<float, false>(a, half, group, st);
@@ -574,7 +567,8 @@ extern "C" int nl_qk_norm_rope_bwd_dev(const nl_qk_norm_rope_bwd_args *args, voi
     a.out[0] = x.dqkv;
     a.out[1] = (char *)x.dqkv + qw * (dtype == NL_BF16 ? 2 : 4);
     const uint32_t group = group_of(dtype, x.head_dim);
-    divide(a, 32 / group);
+    divide(a, 32 / group,
+           148 * (dtype == NL_BF16 ? per_sm<__nv_bfloat16, true> : per_sm<float, true>));
     const bool half = pairs == NL_PAIRS_HALF;
     const cudaError_t e = dtype == NL_BF16 ? start_t<__nv_bfloat16, true>(a, half, group, st)
                                            : start_t<float, true>(a, half, group, st);
