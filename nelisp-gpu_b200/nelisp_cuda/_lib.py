@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(PKG_DIR, "lib", "libnelisp_cuda.so")
@@ -84,7 +83,7 @@ SIGNATURES = {
     "nl_ternary_gemv_static_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp]),
     "nl_decode_attn_rope_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32,
                                      ctypes.c_float, _vp]),
-    # one packed argument structure (PACKED below) and a stream
+    # one argument structure, as bytes, and a stream
     "nl_qk_norm_rope_dev": (_i, [ctypes.c_char_p, _vp]),
     "nl_qk_norm_rope_bwd_workspace_bytes": (_sz, [_u32]),
     "nl_qk_norm_rope_bwd_dev": (_i, [ctypes.c_char_p, _vp]),
@@ -112,18 +111,6 @@ SIGNATURES = {
     "nl_decoder_info": (_i, [_vp, _vp, _vp, _vp]),
     "nl_decoder_shard": (_i, [_vp, _i, _i, _vp]),
     "nl_decoder_destroy": (None, [_vp]),
-}
-
-# The argument structures of the serving entry points, in the header's field
-# order and the C compiler's layout: packing one value list is several times
-# cheaper than converting as many arguments.
-_CACHE = "iIIIIPPPP"           # nl_kv_cache
-PACKED = {
-    "nl_qk_norm_rope_dev": struct.Struct("@iiPQPPPPPPQPQIIIIIIf"),
-    "nl_qk_norm_rope_bwd_dev": struct.Struct("@iiPQPPPPPPQPQPQPPIIIIIIfPN"),
-    "nl_kv_rows": struct.Struct("@" + _CACHE + "iIPPQPQ"),
-    "nl_kv_move_dev": struct.Struct("@" + _CACHE + "PPII"),
-    "nl_tree_attn_dev": struct.Struct("@" + _CACHE + "iIIIIfPQPPPPQPPN"),
 }
 
 _lib = None

@@ -104,88 +104,38 @@ def decode_attn_rope(QKV, CK, CV, POS, C, batch, heads, kv_heads, head_dim, max_
 
 
 # ---- speculative serving: Q/K norm + RoPE, quantised KV cache, tree attention ----
-# These are called once a layer a token: their checks are written for the time
-# they take.
+# Called once a layer a token: the tensors are checked and the arguments filled
+# in C++ (csrc/nl_torch.cpp); a refusal is a ValueError.
 
-_PAIRS = {"half": 0, "adjacent": 1}      # NL_PAIRS_HALF, NL_PAIRS_ADJACENT
-_PACK_QK = L.PACKED["nl_qk_norm_rope_dev"].pack
-_PACK_QK_BWD = L.PACKED["nl_qk_norm_rope_bwd_dev"].pack
-_PACK_ROWS = L.PACKED["nl_kv_rows"].pack
-_PACK_MOVE = L.PACKED["nl_kv_move_dev"].pack
-_PACK_TREE = L.PACKED["nl_tree_attn_dev"].pack
-_types = None
+_ENTRIES = ("nl_qk_norm_rope_dev", "nl_qk_norm_rope_bwd_workspace_bytes",
+            "nl_qk_norm_rope_bwd_dev", "nl_kv_append_dev", "nl_kv_read_dev", "nl_kv_move_dev",
+            "nl_tree_attn_workspace_bytes", "nl_tree_attn_dev")
+_module = None
 
 
-def _torch_types():
-    """(f32, bf16, int32, int64, uint8, {row type: NL_F32 / NL_BF16})."""
-    global _types
-    if _types is None:
-        import torch
-        _types = (torch.float32, torch.bfloat16, torch.int32, torch.int64, torch.uint8,
-                  {torch.float32: 0, torch.bfloat16: 1})
-    return _types
+def _bind():
+    lib = _lib()
+    _module.bind(_device, tuple(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                                for name in _ENTRIES))
 
 
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
+def _load_serving():
+    global _module
+    import torch  # noqa: F401  (its libraries are what the module links to)
+    try:
+        from . import _serving
+    except ImportError as e:
+        raise RuntimeError(f"nelisp_cuda._serving is not built (make -C nelisp-gpu_b200): {e}")
+    _serving.binder(_bind)
+    _module = _serving
+    return _serving
 
 
-def _flat(dtype, *tensors):
-    """Whether all are contiguous CUDA tensors of DTYPE."""
-    for t in tensors:
-        if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
-            raise ValueError(f"expected a contiguous CUDA {dtype} tensor, not {t.dtype} "
-                             f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
-
-
-def _rows(dtype, *tensors):
-    """Whether all are 2-D CUDA rows of DTYPE with unit inner stride; the
-    tensors' row strides."""
-    strides = []
-    for t in tensors:
-        stride = t.stride()
-        if t.dtype is not dtype or not t.is_cuda or len(stride) != 2 or \
-                (stride[1] != 1 and t.shape[1] > 1):
-            raise ValueError(f"expected CUDA rows of {dtype} (2-D, unit inner stride), not "
-                             f"{t.dtype} {tuple(t.shape)} with strides {stride} on {t.device}")
-        strides.append(stride[0])
-    return strides
-
-
-def _row_type(t):
-    code = _torch_types()[5].get(t.dtype)
-    if code is None:
-        raise ValueError(f"expected f32 or bf16 rows, not {t.dtype}")
-    return code
-
-
-def _workspace(nbytes, workspace, device, stream):
-    """WORKSPACE as given, or one of the caching allocator that belongs to the
-    call's stream, so that calls on different streams never share one."""
-    if workspace is not None:
-        return workspace, workspace.numel() * workspace.element_size()
+def _on(stream, function, *args):
+    """FUNCTION with STREAM as the current one."""
     import torch
-    if stream is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
     with torch.cuda.stream(stream):
-        return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
-
-
-def _qk_shapes(QKV, GQ, GK, CO, SI, POS, Q, K, pairs):
-    types = _torch_types()
-    _flat(types[0], GQ, GK, CO, SI)
-    _flat(types[2], POS)
-    (n, width), (nq, wq), (nk, wk) = QKV.shape, Q.shape, K.shape
-    hd, table = GQ.numel(), CO.shape
-    _need(hd > 0 and GK.numel() == hd, "gains of different or no length")
-    _need(len(table) == 2 and table == SI.shape, "CO and SI: two tables of one 2-D shape")
-    if POS.numel() != n or nq != n or nk != n:
-        raise ValueError(f"{n} rows of QKV, {POS.numel()} positions, {nq} and {nk} rows")
-    if wq % hd or wk % hd or wq + wk > width:
-        raise ValueError(f"rows of {width} values do not hold heads of {hd}: {wq} + {wk}")
-    _need(pairs in _PAIRS, "pairs: 'half' or 'adjacent'")
-    return n, wq // hd, wk // hd, hd, 2 * table[1], table[0]
+        return function(*args)
 
 
 def qk_norm_rope(QKV, GQ, GK, CO, SI, POS, Q, K, eps=1e-5, pairs="half", stream=None):
@@ -194,13 +144,9 @@ def qk_norm_rope(QKV, GQ, GK, CO, SI, POS, Q, K, eps=1e-5, pairs="half", stream=
     the rotation of its first 2 * CO.shape[1] values at row POS[i] (int32) of
     the tables CO, SI.  Rows whose position is outside the tables are zeros.
     f32 or bf16; rows may be strided, and Q and K views of QKV itself."""
-    kind = _row_type(QKV)
-    xs, qs, ks = _rows(QKV.dtype, QKV, Q, K)
-    dims = _qk_shapes(QKV, GQ, GK, CO, SI, POS, Q, K, pairs)
-    rc = _lib().nl_qk_norm_rope_dev(_PACK_QK(
-        kind, _PAIRS[pairs], QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(),
-        SI.data_ptr(), POS.data_ptr(), Q.data_ptr(), qs, K.data_ptr(), ks, *dims, eps),
-        _stream(stream))
+    if stream is not None:
+        return _on(stream, qk_norm_rope, QKV, GQ, GK, CO, SI, POS, Q, K, eps, pairs)
+    rc = (_module or _load_serving()).qk_norm_rope(QKV, GQ, GK, CO, SI, POS, Q, K, eps, pairs)
     if rc:
         L.check(rc)
 
@@ -209,22 +155,11 @@ def qk_norm_rope_bwd(QKV, GQ, GK, CO, SI, POS, DQ, DK, DQKV, DGQ, DGK, eps=1e-5,
                      workspace=None, stream=None):
     """The backward pass of qk_norm_rope: the q and k part of DQKV and the
     gains' gradients DGQ, DGK (f32 [hd]) from the gradients DQ, DK."""
-    kind = _row_type(QKV)
-    xs, qs, ks, dxs = _rows(QKV.dtype, QKV, DQ, DK, DQKV)
-    dims = _qk_shapes(QKV, GQ, GK, CO, SI, POS, DQ, DK, pairs)
-    _flat(_torch_types()[0], DGQ, DGK)
-    hd = dims[3]
-    _need(DGQ.numel() == hd and DGK.numel() == hd, "DGQ and DGK: one value per gain")
-    n, width = DQKV.shape
-    if n != dims[0] or width < DQ.shape[1] + DK.shape[1]:
-        raise ValueError(f"DQKV of {n} x {width} for {dims[0]} rows")
-    lib = _lib()
-    ws, nbytes = _workspace(lib.nl_qk_norm_rope_bwd_workspace_bytes(hd), workspace, QKV.device,
-                            stream)
-    rc = lib.nl_qk_norm_rope_bwd_dev(_PACK_QK_BWD(
-        kind, _PAIRS[pairs], QKV.data_ptr(), xs, GQ.data_ptr(), GK.data_ptr(), CO.data_ptr(),
-        SI.data_ptr(), POS.data_ptr(), DQ.data_ptr(), qs, DK.data_ptr(), ks, DQKV.data_ptr(), dxs,
-        DGQ.data_ptr(), DGK.data_ptr(), *dims, eps, ws.data_ptr(), nbytes), _stream(stream))
+    if stream is not None:
+        return _on(stream, qk_norm_rope_bwd, QKV, GQ, GK, CO, SI, POS, DQ, DK, DQKV, DGQ, DGK, eps,
+                   pairs, workspace)
+    rc = (_module or _load_serving()).qk_norm_rope_bwd(QKV, GQ, GK, CO, SI, POS, DQ, DK, DQKV, DGQ,
+                                                       DGK, eps, pairs, workspace)
     if rc:
         L.check(rc)
 
@@ -233,7 +168,8 @@ def kv_cache(num_blocks, block_size, kv_heads, head_dim, bits, device="cuda"):
     """The four arrays of a quantised paged cache (8 or 4 bits a value), zeroed:
     KC, KP, VC, VP, the codes uint8 and the parameter words int32."""
     import torch
-    _need(bits in (4, 8), "bits: 8 or 4")
+    if bits not in (4, 8):
+        raise ValueError("bits: 8 or 4")
     shape = (num_blocks, kv_heads, block_size)
     KC, VC = (torch.zeros(*shape, head_dim * bits // 8, dtype=torch.uint8, device=device)
               for _ in range(2))
@@ -241,55 +177,21 @@ def kv_cache(num_blocks, block_size, kv_heads, head_dim, bits, device="cuda"):
     return KC, KP, VC, VP
 
 
-def _pool(KC, KP, VC, VP, head_dim):
-    """A cache as the fields of nl_kv_cache."""
-    types = _torch_types()
-    _flat(types[4], KC, VC)
-    _flat(types[2], KP, VP)
-    shape = KC.shape
-    if len(shape) != 4 or VC.shape != shape or KP.shape != shape[:3] or VP.shape != shape[:3]:
-        raise ValueError(f"cache codes of {tuple(shape)} and {tuple(VC.shape)}, words of "
-                         f"{tuple(KP.shape)} and {tuple(VP.shape)}")
-    blocks, kvh, size, row = shape
-    if row == head_dim:
-        bits = 8
-    elif 2 * row == head_dim:
-        bits = 4
-    else:
-        raise ValueError(f"rows of {row} bytes for heads of {head_dim}")
-    return (bits, kvh, head_dim, size, blocks, KC.data_ptr(), KP.data_ptr(), VC.data_ptr(),
-            VP.data_ptr())
-
-
-def _kv_shapes(SLOT, KC, KP, VC, VP, K, V):
-    _flat(_torch_types()[2], SLOT)
-    _need(KC.dim() == 4, "cache codes have 4 dimensions")
-    (n, width), kvh = K.shape, KC.shape[1]
-    if V.shape != K.shape or SLOT.numel() != n or kvh == 0 or width % kvh:
-        raise ValueError(f"rows of {n} x {width} and {tuple(V.shape)}, {SLOT.numel()} slots, "
-                         f"{kvh} key heads")
-    return n, _pool(KC, KP, VC, VP, width // kvh)
-
-
 def kv_append(K, V, SLOT, KC, KP, VC, VP, stream=None):
     """Quantise the rows K and V ([n, kv_heads * hd], f32 or bf16, may be
     strided) into the cache's token slots SLOT (int32 [n]; outside: skipped)."""
-    kind = _row_type(K)
-    ks, vs = _rows(K.dtype, K, V)
-    n, pool = _kv_shapes(SLOT, KC, KP, VC, VP, K, V)
-    rc = _lib().nl_kv_append_dev(_PACK_ROWS(
-        *pool, kind, n, SLOT.data_ptr(), K.data_ptr(), ks, V.data_ptr(), vs), _stream(stream))
+    if stream is not None:
+        return _on(stream, kv_append, K, V, SLOT, KC, KP, VC, VP)
+    rc = (_module or _load_serving()).kv_append(K, V, SLOT, KC, KP, VC, VP)
     if rc:
         L.check(rc)
 
 
 def kv_read(SLOT, KC, KP, VC, VP, K, V, stream=None):
     """The values of the slots SLOT into the rows K and V (outside: zeros)."""
-    kind = _row_type(K)
-    ks, vs = _rows(K.dtype, K, V)
-    n, pool = _kv_shapes(SLOT, KC, KP, VC, VP, K, V)
-    rc = _lib().nl_kv_read_dev(_PACK_ROWS(
-        *pool, kind, n, SLOT.data_ptr(), K.data_ptr(), ks, V.data_ptr(), vs), _stream(stream))
+    if stream is not None:
+        return _on(stream, kv_read, SLOT, KC, KP, VC, VP, K, V)
+    rc = (_module or _load_serving()).kv_read(SLOT, KC, KP, VC, VP, K, V)
     if rc:
         L.check(rc)
 
@@ -297,11 +199,11 @@ def kv_read(SLOT, KC, KP, VC, VP, K, V, stream=None):
 def kv_move(SRC, DST, KC, KP, VC, VP, head_dim, stream=None):
     """Move tokens between slots without requantising them: SRC, DST int32
     [batch, count]; per sequence every source is read before any write."""
-    _flat(_torch_types()[2], SRC, DST)
-    _need(SRC.dim() == 2 and SRC.shape == DST.shape, "SRC and DST: [batch, count] each")
-    L.check(_lib().nl_kv_move_dev(_PACK_MOVE(
-        *_pool(KC, KP, VC, VP, head_dim), SRC.data_ptr(), DST.data_ptr(), *SRC.shape),
-        _stream(stream)))
+    if stream is not None:
+        return _on(stream, kv_move, SRC, DST, KC, KP, VC, VP, head_dim)
+    rc = (_module or _load_serving()).kv_move(SRC, DST, KC, KP, VC, VP, head_dim)
+    if rc:
+        L.check(rc)
 
 
 def tree_attn(Q, KC, KP, VC, VP, TABLE, LEN, MASK, O, head_dim, scale=None, lse=None,
@@ -312,36 +214,13 @@ def tree_attn(Q, KC, KP, VC, VP, TABLE, LEN, MASK, O, head_dim, scale=None, lse=
     prefix tokens; MASK int64 [batch, nodes], bit j of node i set where i
     attends to node j (token LEN + j), 0 for an unused node.  SCALE is
     1/sqrt(head_dim) unless given; LSE (f32 [batch * nodes, heads]) receives
-    the log of the softmax sums."""
-    types = _torch_types()
-    kind = _row_type(Q)
-    qs, os_ = _rows(Q.dtype, Q, O)
-    _flat(types[2], TABLE, LEN)
-    _flat(types[3], MASK)
-    pool = _pool(KC, KP, VC, VP, head_dim)
-    table, mask, shape = TABLE.shape, MASK.shape, Q.shape
-    _need(len(mask) == 2 and len(table) == 2, "MASK and TABLE have 2 dimensions")
-    batch, nodes = mask
-    rows, width = shape
-    heads = width // head_dim
-    if LEN.numel() != batch or table[0] != batch or rows != batch * nodes or O.shape != shape or \
-            width != heads * head_dim:
-        raise ValueError(f"tree_attn: {rows} rows of {width}, heads of {head_dim}, {batch} "
-                         f"sequences of {nodes} nodes, {LEN.numel()} lengths, a table of "
-                         f"{tuple(table)}, outputs of {tuple(O.shape)}")
-    out_lse = 0
-    if lse is not None:
-        _flat(types[0], lse)
-        _need(lse.shape == (rows, heads), "lse: a value per row and head")
-        out_lse = lse.data_ptr()
-    lib = _lib()
-    ws, nbytes = _workspace(lib.nl_tree_attn_workspace_bytes(nodes, heads, pool[1], head_dim),
-                            workspace, Q.device, stream)
-    rc = lib.nl_tree_attn_dev(_PACK_TREE(
-        *pool, kind, batch, nodes, heads, table[1],
-        scale if scale is not None else head_dim ** -0.5, Q.data_ptr(), qs, TABLE.data_ptr(),
-        LEN.data_ptr(), MASK.data_ptr(), O.data_ptr(), os_, out_lse, ws.data_ptr(), nbytes),
-        _stream(stream))
+    the log of the softmax sums.  The workspace, unless given, is the caching
+    allocator's on the call's stream."""
+    if stream is not None:
+        return _on(stream, tree_attn, Q, KC, KP, VC, VP, TABLE, LEN, MASK, O, head_dim, scale, lse,
+                   workspace)
+    rc = (_module or _load_serving()).tree_attn(Q, KC, KP, VC, VP, TABLE, LEN, MASK, O, head_dim,
+                                                scale, lse, workspace)
     if rc:
         L.check(rc)
 

@@ -22,6 +22,8 @@ import math
 import numpy as np
 import pytest
 
+from serving_structs import PACKED
+
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
@@ -891,13 +893,13 @@ def test_library_refusals(dev, torch):
         return fmt, kvh, hd, bs, nb, kc, kp, vc, vp
 
     def rows(pool, dtype=0, n=1, slot=p, k=p, ks=64, v=p, vs=64):
-        return L.PACKED["nl_kv_rows"].pack(*pool, dtype, n, slot, k, ks, v, vs)
+        return PACKED["nl_kv_rows"].pack(*pool, dtype, n, slot, k, ks, v, vs)
 
     def tree(pool, dtype=0, batch=1, nodes=1, heads=1, mb=1, scale=0.1, q=p, qs=64, table=p, ln=p,
              mask=p, o=p, os=64, lse=0, ws=p, wsb=1 << 30):
-        return L.PACKED["nl_tree_attn_dev"].pack(*pool, dtype, batch, nodes, heads, mb, scale, q,
+        return PACKED["nl_tree_attn_dev"].pack(*pool, dtype, batch, nodes, heads, mb, scale, q,
                                                  qs, table, ln, mask, o, os, lse, ws, wsb)
-    move = L.PACKED["nl_kv_move_dev"].pack
+    move = PACKED["nl_kv_move_dev"].pack
     cases = [("nl_kv_append_dev", rows(cache(fmt=5)), "format"),
              ("nl_kv_append_dev", rows(cache(), dtype=2), "type"),
              ("nl_kv_append_dev", rows(cache(bs=1 << 16, nb=1 << 15)), "slots"),

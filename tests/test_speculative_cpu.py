@@ -6,6 +6,7 @@ import torch
 
 from nelisp_cuda import _lib as L
 from nelisp_cuda import dev
+from serving_structs import PACKED
 
 
 def test_host_tensors_are_refused():
@@ -79,4 +80,4 @@ def test_packed_structures_match_the_header(tmp_path):
     out = subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split("\n")
     for line, (packed, _) in zip(out, names.values()):
         end, size = map(int, line.split())
-        assert L.PACKED[packed].size == end <= size < end + 8, packed
+        assert PACKED[packed].size == end <= size < end + 8, packed
