@@ -112,10 +112,26 @@ template <typename T, int HD, int BITS, int NR, int WR, bool PACK> struct Plan {
   static constexpr int Bytes = Small + (Q + Ring > Join ? Q + Ring : Join);
 };
 
-template <typename T> __device__ __forceinline__ float load1(const T *p);
-template <> __device__ __forceinline__ float load1<float>(const float *p) { return __ldg(p); }
-template <> __device__ __forceinline__ float load1<__nv_bfloat16>(const __nv_bfloat16 *p) {
-  return __bfloat162float(__ldg(p));
+// N values from a place aligned to all of them, or to 16 bytes.
+template <int N> __device__ __forceinline__ void load_row(const float *p, float *v) {
+  if constexpr (N == 2) {
+    const float2 x = __ldg(reinterpret_cast<const float2 *>(p));
+    v[0] = x.x; v[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = __ldg(reinterpret_cast<const float4 *>(p + i));
+      v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+    }
+  }
+}
+template <int N> __device__ __forceinline__ void load_row(const __nv_bfloat16 *p, float *v) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p + i));
+    v[i] = __uint_as_float(x.x << 16); v[i + 1] = __uint_as_float(x.x & 0xffff0000u);
+    v[i + 2] = __uint_as_float(x.y << 16); v[i + 3] = __uint_as_float(x.y & 0xffff0000u);
+  }
 }
 __device__ __forceinline__ void store1(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
@@ -128,6 +144,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   constexpr int Terms = P::Terms, WK = P::WK, Stages = P::Stages;
   constexpr bool Flush = sizeof(T) == 4;         // each 16 keys summed apart
   constexpr uint32_t Live = PACK ? 4 : P::Rows;  // rows of an item
+  // threads of a row where it is read and where its state is joined
+  constexpr uint32_t PerRow = Live <= 4 ? 32 : Live <= 8 ? 16 : 8;
   extern __shared__ __align__(16) uint8_t smem[];
   float *row_f = reinterpret_cast<float *>(smem);                    // factor of a row's scores
   float *row_sum = row_f + P::Rows;                                  // sum of its query
@@ -218,24 +236,24 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
       next = find(t0 + i + 1);
     }
 
-    // ---- the query rows, as operand fragments: 8 threads a row ----
-    // (threads past the rows go through with the first: the shuffles are whole)
-    for (uint32_t i0 = threadIdx.x / 8; i0 < P::Rows || i0 < kTreeThreads / 8;
-         i0 += kTreeThreads / 8) {
-      constexpr int Per = HD / 8;
-      const uint32_t r = i0 < Live ? i0 : 0, part = threadIdx.x % 8, row = row0 + r;
+    // ---- the query rows, as operand fragments ----
+    for (uint32_t r = threadIdx.x / PerRow; r < Live; r += kTreeThreads / PerRow) {
+      constexpr int Per = HD / PerRow;
+      const uint32_t part = threadIdx.x % PerRow, row = row0 + r;
       const bool live = row < a.rows;
       const uint32_t node = live ? row / a.group : 0;
       const T *q = (const T *)a.q + ((uint64_t)b * a.nodes + node) * a.q_stride +
                    (uint64_t)(head * a.group + (live ? row % a.group : 0)) * HD + part * Per;
+      const uint64_t mask = live ? a.mask[(uint64_t)b * a.nodes + node] & used : 0;
       float v[Per], top = 0.0f, sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < Per; i++) {
-        v[i] = live ? load1(q + i) : 0.0f;
-        top = fmaxf(top, fabsf(v[i]));
-      }
+      for (int i = 0; i < Per; i++) v[i] = 0.0f;
+      if (live) load_row<Per>(q, v);
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int i = 0; i < Per; i++) top = fmaxf(top, fabsf(v[i]));
+#pragma unroll
+      for (int o = PerRow / 2; o > 0; o >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       // the power of two that brings the largest value to [2^13, 2^14)
       int up = 140 - (int)(__float_as_uint(top) >> 23);
       if (top == 0.0f || !(top < INFINITY)) up = 0;
@@ -256,9 +274,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
           *reinterpret_cast<__half *>(qf + fragment(r + 4, step, quad) + p * 4 + half * 2) = low;
       }
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int o = PerRow / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (part == 0) {
-        const uint64_t mask = live ? a.mask[(uint64_t)b * a.nodes + node] & used : 0;
 #pragma unroll
         for (uint32_t c = r; c < P::Rows; c += PACK ? 4 : P::Rows) {
           // never zero: a factor of zero would make NaN of a masked score
@@ -581,9 +598,9 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
         }
     }
     __syncthreads();
-    for (uint32_t r = threadIdx.x / 8; r < Live; r += kTreeThreads / 8) {
-      constexpr int Per = HD / 8;
-      const uint32_t part = threadIdx.x % 8, row = row0 + r;
+    for (uint32_t r = threadIdx.x / PerRow; r < Live; r += kTreeThreads / PerRow) {
+      constexpr int Per = HD / PerRow;
+      const uint32_t part = threadIdx.x % PerRow, row = row0 + r;
       float top = -INFINITY, sum = 0.0f, c[WK];
 #pragma unroll
       for (int w = 0; w < WK; w++) top = fmaxf(top, ml[w * P::Rows + r].x);
@@ -603,7 +620,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
       const uint64_t out_row = (uint64_t)b * a.nodes + node;
 #pragma unroll
       for (int i = 0; i < Per; i++) {
-        const uint32_t d = i * 8 + part;
+        const uint32_t d = i * PerRow + part;
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < WK; w++)
