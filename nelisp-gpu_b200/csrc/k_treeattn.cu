@@ -2,6 +2,8 @@
 // the quantised paged cache.  The kernels are in tree_attn.cuh, compiled per
 // head size in k_treeattn_h*.cu.
 
+#include <algorithm>
+
 #include "tree_work.cuh"
 
 namespace nl {
@@ -73,6 +75,13 @@ extern "C" int nl_tree_attn_dev(const nl_tree_attn_args *args, void *stream) {
   const uint32_t umma_rows = tree_umma_rows(a, bf16);
   a.rows_at_once = umma_rows ? umma_rows : tree_rows_at_once(a.rows, head_dim);
   a.row_tiles = (a.rows + a.rows_at_once - 1) / a.rows_at_once;
+  // The list of the work, in tiles of at least 32 keys, is counted in 32 bits.
+  const uint64_t most = std::min((uint64_t)x.max_blocks * block_size, (uint64_t)INT32_MAX + nodes);
+  const unsigned __int128 places =
+      (unsigned __int128)(most / 32 + 1 + kTreeMaxItemCost) * kv_heads * a.row_tiles * batch;
+  if (places > UINT32_MAX)
+    return set_error(NL_ERROR, "%s: %u sequences of up to %llu tokens: too much for one call", what,
+                     batch, (unsigned long long)most);
   a.block_shift = 32;
   for (uint32_t s = 0; s < 32; s++)
     if (block_size == 1u << s) a.block_shift = s;

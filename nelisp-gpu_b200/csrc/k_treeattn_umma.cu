@@ -257,7 +257,7 @@ template <bool SUM> __device__ __forceinline__ float across(uint32_t (&v)[H]) {
 
 // The walk over the parts of items that a CTA has, the same in every role.
 struct Walk {
-  uint64_t at, end, before;
+  uint32_t at, end, before;
   uint32_t b, items;
   uint32_t head, row0, t0, t1, tiles;
   __device__ __forceinline__ bool begin(const TreeArgs &a) {
@@ -273,13 +273,13 @@ struct Walk {
     while (at < end) {
       tiles = tiles_of(a, b);
       const uint32_t cost = tiles + a.item_cost;
-      if (at >= before + (uint64_t)cost * items) {
-        before += (uint64_t)cost * items;
+      if (at >= before + cost * items) {
+        before += cost * items;
         b++;
         continue;
       }
-      const uint32_t item = (uint32_t)((at - before) / cost), c0 = (uint32_t)((at - before) % cost);
-      const uint32_t c1 = end - at < cost - c0 ? c0 + (uint32_t)(end - at) : cost;
+      const uint32_t item = (at - before) / cost, c0 = (at - before) % cost;
+      const uint32_t c1 = end - at < cost - c0 ? c0 + (end - at) : cost;
       at += c1 - c0;
       if (c1 <= a.item_cost) continue;
       t0 = c0 > a.item_cost ? c0 - a.item_cost : 0;

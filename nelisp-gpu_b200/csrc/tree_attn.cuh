@@ -160,13 +160,12 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t wr = warp % WR, wk = warp / WR;
   const List list = list_of(a);
-  const uint64_t total = list.total;
-  const uint32_t workers = list.workers;
+  const uint32_t total = list.total, workers = list.workers;
   if (blockIdx.x >= workers) return;
-  uint64_t at = share(total, workers, blockIdx.x);
-  const uint64_t end = share(total, workers, blockIdx.x + 1);
+  uint32_t at = share(total, workers, blockIdx.x);
+  const uint32_t end = share(total, workers, blockIdx.x + 1);
   uint32_t b;
-  uint64_t before;
+  uint32_t before;
   locate(a, at, &b, &before);
   const uint32_t items = a.pool.kv_heads * a.row_tiles;
   uint8_t *mine = ring + wk * (Stages * G::Stage);
@@ -182,13 +181,13 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   while (at < end) {
     // ---- the next item, or part of one ----
     const uint32_t tiles = tiles_of(a, b), cost = tiles + a.item_cost;
-    if (at >= before + (uint64_t)cost * items) {
-      before += (uint64_t)cost * items;
+    if (at >= before + cost * items) {
+      before += cost * items;
       b++;
       continue;
     }
-    const uint32_t item = (uint32_t)((at - before) / cost), c0 = (uint32_t)((at - before) % cost);
-    const uint32_t c1 = end - at < cost - c0 ? c0 + (uint32_t)(end - at) : cost;
+    const uint32_t item = (at - before) / cost, c0 = (at - before) % cost;
+    const uint32_t c1 = end - at < cost - c0 ? c0 + (end - at) : cost;
     at += c1 - c0;
     if (c1 <= a.item_cost) continue;             // its share ends before the first tile
     const uint32_t t0 = c0 > a.item_cost ? c0 - a.item_cost : 0, t1 = c1 - a.item_cost;
@@ -660,21 +659,20 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
   // Whatever wrote the lengths is done: the attention kernel lets this one start
   // once it has waited for that itself.
   const List list = list_of(a);
-  const uint64_t total = list.total;
-  const uint32_t workers = list.workers, cut = blockIdx.x + 1;
+  const uint32_t total = list.total, workers = list.workers, cut = blockIdx.x + 1;
   // (Every block waits, also where it has nothing to join: once this grid is
   // done, whatever follows it takes the attention kernel to be done.)
   if (cut >= workers) {
     pdl_wait();
     return;
   }
-  const uint64_t at = share(total, workers, cut);
+  const uint32_t at = share(total, workers, cut);
   uint32_t b;
-  uint64_t before;
+  uint32_t before;
   locate(a, at, &b, &before);
   const uint32_t tiles = tiles_of(a, b), cost = tiles + a.item_cost;
-  const uint32_t off = (uint32_t)((at - before) % cost), item = (uint32_t)((at - before) / cost);
-  const uint64_t s0 = at - off + a.item_cost;     // the item's first tile
+  const uint32_t off = (at - before) % cost, item = (at - before) / cost;
+  const uint32_t s0 = at - off + a.item_cost;     // the item's first tile
   const bool cuts = off > a.item_cost && share(total, workers, cut - 1) <= s0;
   const uint32_t c0 = cut - 1, c1 = owner(total, workers, s0 + tiles - 1);
   const uint32_t head = item / a.row_tiles, row0 = item % a.row_tiles * a.rows_at_once;

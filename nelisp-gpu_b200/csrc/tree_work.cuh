@@ -12,6 +12,7 @@
 namespace nl {
 
 constexpr uint32_t kTreeMaxCtas = 148 * 4;
+constexpr uint32_t kTreeMaxItemCost = 16;
 
 struct TreeArgs {
   const void *q;
@@ -64,23 +65,20 @@ __device__ __forceinline__ uint32_t tiles_of(const TreeArgs &a, uint32_t b) {
   return n ? (n + a.tile - 1) / a.tile : 1u;
 }
 
-__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+// (The entry point refuses lists of 2^32 places and more: in 64 bits the
+// divisions here took a microsecond of a call with a few keys, and registers of
+// the others.)
 // The list's length -- an item counts its tiles and its own cost -- and the CTAs
 // it is divided among.  Where all sequences are equally long, a number of CTAs
 // that the items divide evenly gives every CTA a part of one item only (8 x 32
 // items of 33 tiles on 256 of 296 CTAs instead of one and a part of another
 // each); it is taken if it leaves no more than 15% of the CTAs without work.
 struct List {
-  uint64_t total;
-  uint32_t workers;
+  uint32_t total, workers;
 };
 __device__ __forceinline__ List list_of(const TreeArgs &a) {
   const uint32_t lane = threadIdx.x & 31;
-  uint64_t sum = 0;
+  uint32_t sum = 0;
   uint32_t least = ~0u, most = 0;
   for (uint32_t b = lane; b < a.batch; b += 32) {
     const uint32_t t = tiles_of(a, b);
@@ -90,29 +88,29 @@ __device__ __forceinline__ List list_of(const TreeArgs &a) {
   }
   List l;
   const uint32_t items = a.pool.kv_heads * a.row_tiles;
-  l.total = warp_sum(sum) * items;
-  l.workers = l.total < a.ctas ? (uint32_t)l.total : a.ctas;
-  const uint64_t all = (uint64_t)items * a.batch;
+  l.total = __reduce_add_sync(0xffffffffu, sum) * items;
+  l.workers = min(l.total, a.ctas);
+  const uint32_t all = items * a.batch;
   if (__reduce_min_sync(0xffffffffu, least) == __reduce_max_sync(0xffffffffu, most) &&
       all <= l.workers) {
-    const uint32_t even = l.workers / (uint32_t)all * (uint32_t)all;
+    const uint32_t even = l.workers / all * all;
     if (even * 20 >= l.workers * 17) l.workers = even;
   }
   return l;
 }
 // The sequence that place AT of the list falls into, and the places before it.
-__device__ __forceinline__ void locate(const TreeArgs &a, uint64_t at, uint32_t *b_out,
-                                       uint64_t *before_out) {
+__device__ __forceinline__ void locate(const TreeArgs &a, uint32_t at, uint32_t *b_out,
+                                       uint32_t *before_out) {
   const uint32_t lane = threadIdx.x & 31;
-  const uint64_t items = (uint64_t)a.pool.kv_heads * a.row_tiles;
-  uint64_t before = 0;
+  const uint32_t items = a.pool.kv_heads * a.row_tiles;
+  uint32_t before = 0;
   for (uint32_t base = 0; base < a.batch; base += 32) {
-    const uint64_t mine =
+    const uint32_t mine =
         base + lane < a.batch ? (tiles_of(a, base + lane) + a.item_cost) * items : 0;
-    uint64_t end = mine;
+    uint32_t end = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t up = __shfl_up_sync(0xffffffffu, end, o);
+      const uint32_t up = __shfl_up_sync(0xffffffffu, end, o);
       if (lane >= (uint32_t)o) end += up;
     }
     end += before;
@@ -129,11 +127,11 @@ __device__ __forceinline__ void locate(const TreeArgs &a, uint64_t at, uint32_t 
   *before_out = before;
 }
 // CTA c of w takes the places [share(c), share(c + 1)).
-__device__ __forceinline__ uint64_t share(uint64_t total, uint32_t w, uint32_t c) {
-  return total / w * c + total % w * c / w;
+__device__ __forceinline__ uint32_t share(uint32_t total, uint32_t w, uint32_t c) {
+  return total / w * c + total % w * c / w;      // w is at most kTreeMaxCtas
 }
-__device__ __forceinline__ uint32_t owner(uint64_t total, uint32_t w, uint64_t at) {
-  uint32_t c = (uint32_t)((double)at * w / (double)total);
+__device__ __forceinline__ uint32_t owner(uint32_t total, uint32_t w, uint32_t at) {
+  uint32_t c = (uint32_t)((float)at * ((float)w / (float)total));      // or a neighbour of it
   if (c >= w) c = w - 1;
   while (c + 1 < w && share(total, w, c + 1) <= at) c++;
   while (c > 0 && share(total, w, c) > at) c--;

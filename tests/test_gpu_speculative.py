@@ -921,6 +921,7 @@ def test_library_refusals(dev, torch):
              ("nl_tree_attn_dev", tree(cache(), o=8), "aligned"),
              ("nl_tree_attn_dev", tree(cache(), mask=0), "null"),
              ("nl_tree_attn_dev", tree(cache(), wsb=100), "workspace"),
+             ("nl_tree_attn_dev", tree(cache(bs=1 << 16), batch=64, mb=1 << 16), "too much"),
              ("nl_tree_attn_dev", tree(cache(fmt=6)), "format"),
              ("nl_tree_attn_dev", tree(cache(kc=4)), "unaligned")]
     cases += [(name, None, "null") for name in
