@@ -460,10 +460,10 @@ int nl_kv_move_dev(const nl_kv_move_args *args, void *stream);
  * them, node j as token LEN[b] + j; token t is offset t % block_size of block
  * TABLE[b][t / block_size] (int32 [batch][max_blocks]; a block outside the
  * pool, or past max_blocks, holds no keys).  A call's tables span fewer than
- * 2^32 runs of 32 tokens over its sequences and key heads.  Node i attends to every prefix
- * token and to the nodes j whose bit j of MASK[b][i] is set: its ancestors
- * and itself.  A mask of 0 marks an unused node: its output is zeros and its
- * LSE -inf, as for a node that finds no key.
+ * 2^32 runs of 32 tokens over its sequences and key heads.  Node i attends
+ * to every prefix token and to the nodes j whose bit j of MASK[b][i] is set:
+ * its ancestors and itself.  A mask of 0 marks an unused node: its output is
+ * zeros and its LSE -inf, as for a node that finds no key.
  *   O[b,i,h] = sum_t softmax_t(SCALE q.k_t) v_t,
  *   LSE[b,i,h] = log sum_t exp(SCALE q.k_t)
  * Q and O are rows (b, i) of heads*head_dim elements of DTYPE, 16-byte

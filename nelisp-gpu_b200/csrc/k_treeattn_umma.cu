@@ -29,17 +29,17 @@
 //               thread's branch the issue of a tile took longer than its work.
 // The registers of the launch are shared out anew among the roles.
 //
-// What bounds it: a tile takes about 3,150 cycles (131,071 keys, 16 nodes of 4
-// heads, 8 bits: 107 us, 2.6 TB/s, 321 TF/s) with the tensor cores 17% busy, issue 58%, and shared memory -- codes in and out, values
-// out and in again, weights, the rows' factors and references -- about 80%.  No
-// role is the one: each is 2,000 to 2,300 cycles busy a tile at 5 to 8 cycles an
-// instruction, and waits the rest of it for another.  Measured and not taken: two
-// streams of score warps on alternate tiles (32 rows, 4 bits: 68 us, not 62), the
-// vote by a barrier that is waited for after the exponentials (125, not 110), the
-// scores' columns released before the weights (113), deeper batches of loads in
-// the conversions (110 to 115).
-// The stages run on over the end of an item: the next item's codes are on
-// their way and converted while the last one's output is written.
+// What bounds it: a tile takes about 3,000 cycles (131,071 keys, 16 nodes of 4
+// heads, 8 bits: 102 us, 2.7 TB/s, 336 TF/s) with the tensor cores 17% busy,
+// issue 58%, and shared memory -- codes in and out, values out and in again,
+// weights, the rows' factors and references -- about 80%.  No role is the one:
+// each is 2,000 to 2,300 cycles busy a tile at 5 to 8 cycles an instruction, and
+// waits the rest of it for another.  Registers matter: with the list of work in
+// 64 bits, which spilled, the same took 107.  Measured and not taken: two streams
+// of score warps on alternate tiles (32 rows, 4 bits: 64.3 us, not 63.2), the vote
+// by a barrier that is waited for after the exponentials (15% slower), the scores'
+// columns released before the weights (5%), deeper batches of loads in the
+// conversions (1 to 5%).
 //
 // Every wait is bounded.  One that gives up sets the library's wait flag, and
 // its thread then waits no more but runs on to the end: no barrier of the CTA

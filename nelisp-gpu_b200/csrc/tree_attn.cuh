@@ -30,7 +30,7 @@
 // else synchronises the CTA until an item ends.
 //
 // What bounds it: with few rows the loads.  8 sequences of 4,096 keys, 32 heads
-// of 128, float32, 8 bits: 62.6 us for 277 MB, 0.67 of a copy's rate; the same
+// of 128, float32, 8 bits: 61.0 us for 277 MB, 0.69 of a copy's rate; the same
 // without the products 50, the join 3.  With many rows the issue of products and
 // weights: the table at start_rows; in bfloat16 the tcgen05 form
 // (k_treeattn_umma.cu) takes over there.
@@ -801,7 +801,7 @@ cudaError_t start_rows(TreeArgs &a, cudaStream_t st) {
   constexpr int Most = HD == 256 ? 2 : 4;
   constexpr int Part = sizeof(T) == 4 && HD == 128 && BITS == 8 ? 2 : Most;
   // Up to four rows of float32: both terms in one 8-row tile (8 sequences of 4,096
-  // keys, 32 heads, 8 bits: 62.6 us; as two tiles 72.8).
+  // keys, 32 heads, 8 bits: 62.6 us where as two tiles it took 72.8).
   if constexpr (sizeof(T) == 4) {
     if (a.rows <= 4) return start<T, HD, BITS, 1, 1, true>(a, st);
   }
