@@ -460,7 +460,7 @@ int rows_call(const char *what, bool append, const nl_kv_rows_args *args, void *
   if ((rc = kv_check_pool(what, fmt, p))) return rc;
   if (n == 0) return NL_OK;
   if (!r.slot) return set_error(NL_ERROR, "%s: null slots", what);
-  if (p.kv_heads > INT32_MAX)      // twice as many are counted in 32 bits
+  if (p.kv_heads > 1u << 30)       // twice as many, and a step more, are counted in 32 bits
     return set_error(NL_ERROR, "%s: %u kv heads", what, p.kv_heads);
   const uint32_t unit = dtype == NL_BF16 ? 8 : 4;
   for (int i = 0; i < 2; i++) {
