@@ -84,7 +84,9 @@ template <int HD, int BITS, int N> struct Plan {
   static constexpr int Warp = Offs + N * 8;                   // [4][N]
   static constexpr int Base = Warp + 4 * N * 4;               // [4][N] (4 bits)
   static constexpr int Words = Base + (BITS == 4 ? 4 * N * 4 : 0);   // [4][128] uint4
-  static constexpr int Bars = Words + 4 * kTileKeys * 16;
+  static constexpr int Scale = Words + 4 * kTileKeys * 16;    // [4][N]
+  static constexpr int Lim = Scale + 4 * N * 4;
+  static constexpr int Bars = Lim + N * 4;
   static constexpr int Used = Bars + 256 + 1024;
   static constexpr int Bytes = Used > 120 * 1024 ? Used : 120 * 1024;   // one CTA per SM (TMEM)
   // TMEM columns: two stages of keys and of scores, the output
@@ -309,6 +311,8 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
   uint64_t *offs = reinterpret_cast<uint64_t *>(sm + L::Offs);
   float *warp_part = reinterpret_cast<float *>(sm + L::Warp);
   float *warp_base = reinterpret_cast<float *>(sm + L::Base);
+  float *warp_scale = reinterpret_cast<float *>(sm + L::Scale);   // largest scale a row sees
+  uint32_t *lim = reinterpret_cast<uint32_t *>(sm + L::Lim);      // of a row so far, if apart
   const uint32_t bars = s0 + L::Bars;
   const uint32_t full = bars, empty = bars + 24, kready = bars + 48, qkdone = bars + 80,
                  sfree = bars + 96, vready = bars + 112, pready = bars + 128, pvdone = bars + 144,
@@ -614,7 +618,10 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
 #pragma unroll
         for (int i = 0; i < H / 2; i++) l[i] = base[i % NB] = 0;
         float vs = 1.0f;
-        uint32_t vlimit = 0;
+        uint32_t vlimit = kTreeNone;
+        // Rows see different nodes, so there a row has a limit of its own, and where
+        // the limits differ (VLIMIT is kTreeOwn) its reference is moved by as many
+        // powers of two: a node that a row does not see costs its weights no bits.
 
         for (uint32_t tile = w.t0; tile < w.t1; tile++, it++) {
           const uint32_t st = it & 1, ph = it >> 1 & 1;
@@ -628,12 +635,20 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           const float mk = middle_of(kw);
           const Pair sk2 = pair(sk, sk), mk2 = pair(mk, mk);
           const float sv = scale_of<BITS>(vw);
-          // (a value that is NaN reaches the output by its weight alone)
-          const float mv = BITS == 4 && sv == sv ? middle_of(vw) : 0.0f;
+          // (a value that is not finite reaches the output by its weight alone)
+          const float mid = BITS == 4 ? middle_of(vw) : 0.0f;
+          const bool finite = fabsf(mid) < INFINITY;
+          const float mv = finite ? mid : 0.0f;
           const uint32_t vbits = __float_as_uint(sv) < 0x7f800000u ? __float_as_uint(sv) : 0u;
           const uint32_t key = tile * kTileKeys + mykey;
           // tiles of prefix keys that all exist need no masks
           const bool whole = __all_sync(0xffffffffu, have && key < prefix);
+          const bool nodes_here = (tile + 1) * kTileKeys > prefix;
+          auto sees = [&](int i) {
+            const uint64_t m = masks[n0 + i];
+            const uint32_t node = key - prefix;
+            return have && (key < prefix ? m != 0 : node < 64 && (m >> node & 1));
+          };
           // the scores of the group's rows on this key, in powers of two: over the
           // rows' references, or as they are
           auto score = [&](uint32_t (&s)[H], bool over_ref) {
@@ -659,13 +674,8 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             }
             if (!whole) {
 #pragma unroll
-              for (int i = 0; i < H; i++) {
-                const uint64_t m = masks[n + i];
-                const uint32_t node = key - prefix;
-                const bool seen =
-                    have && (key < prefix ? m != 0 : node < 64 && (m >> node & 1));
-                if (!seen) s[i] = 0xff800000u;             // -inf
-              }
+              for (int i = 0; i < H; i++)
+                if (!sees(i)) s[i] = 0xff800000u;          // -inf
             }
           };
           const uint32_t ts = tmem + (quad << 16) + L::TS + st * N + n0;
@@ -676,30 +686,58 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < H; i++) top = fmaxf(top, __uint_as_float(s[i]));
-            const bool over = top > 8.0f || (vbits >= vlimit && vbits != 0);
+            const bool over = top > 8.0f || vbits >= vlimit;
             if (again || !group_any(group, over)) break;
             // ---- new references: the maxima of the keys so far ----
+            const bool apart = vlimit == kTreeOwn;
+            const uint32_t before = vlimit == kTreeNone ? 0 : 261u - (__float_as_uint(vs) >> 23);
             tmem_ld16(ts, s);
             score(s, false);
             const float mine = across<false>(s);
             if (lane < H) warp_part[(warp & 3) * N + n0 + lane] = mine;
-            if (quad == 0 && lane == 0) *vote = 0;
+            if (nodes_here) {
+#pragma unroll
+              for (int i = 0; i < H; i++) s[i] = sees(i) ? vbits : 0u;
+              const float scale = across<false>(s);
+              if (lane < H) warp_scale[(warp & 3) * N + n0 + lane] = scale;
+            }
+            if (quad == 0 && lane == 0) *vote = before << 23;
             group_sync(group);
-            const uint32_t top_bits = __reduce_max_sync(0xffffffffu, vbits);
-            if (lane == 0) atomicMax(vote, top_bits);
+            if (!nodes_here) {
+              const uint32_t top_bits = __reduce_max_sync(0xffffffffu, vbits);
+              if (lane == 0 && top_bits >= vlimit) atomicMax(vote, limit_of(top_bits) << 23);
+            }
             if (mykey < H) {
-              const float *p = warp_part + n0 + mykey;
+              const uint32_t n = n0 + mykey;
+              const float *p = warp_part + n;
               const float most = fmaxf(fmaxf(p[0], p[N]), fmaxf(p[2 * N], p[3 * N]));
-              const float old = -ref[n0 + mykey];            // -kFar: no key met yet
-              keep[n0 + mykey] = most > old ? ex2(old - most) : 1.0f;
-              if (most > old) ref[n0 + mykey] = -most;
+              int was = 0, now = 0;                          // powers of two of the reference
+              if (nodes_here) {
+                const float *z = warp_scale + n;
+                const float scale = fmaxf(fmaxf(z[0], z[N]), fmaxf(z[2 * N], z[3 * N]));
+                const uint32_t had = apart ? lim[n] : before;
+                const uint32_t own =
+                    max(had, scale > 0.0f ? limit_of(__float_as_uint(scale)) : 0u);
+                const uint32_t e = common_limit(before, __reduce_min_sync(0xffffu, own ? own : ~0u),
+                                                __reduce_max_sync(0xffffu, own));
+                const bool differ = __any_sync(0xffffu, own != e);
+                was = apart_by(before, had);
+                now = apart_by(e, own);
+                lim[n] = own;
+                if (mykey == 0) *vote = e << 23 | (differ ? 1u : 0u);
+              }
+              // (kFar: no key met yet)
+              const float old = ref[n] == kFar ? -kFar : (float)was - ref[n];
+              keep[n] = (most > old ? ex2(old - most) : 1.0f) *
+                        __uint_as_float((uint32_t)(127 + now - was) << 23);
+              if (most > old) ref[n] = (float)now - most;
+              else if (ref[n] != kFar) ref[n] = (float)now - old;
             }
             group_sync(group);
             float ratio = 1.0f;
-            const uint32_t big = *vote;
-            if (big >= vlimit && big != 0) {
-              const uint32_t e = (big >> 23) + 1;            // scales below 2^(e - 127)
-              vlimit = e << 23;
+            const uint32_t e = *vote >> 23;                  // scales below 2^(e - 127)
+            vlimit = *vote & 1u ? kTreeOwn : e ? e << 23 : kTreeNone;
+            if (e != before) {
               const float next_vs = __uint_as_float((261u - e) << 23);   // to below 2^7
               ratio = next_vs / vs;
               vs = next_vs;
@@ -726,7 +764,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
           // ---- the weights ----
           const float wv = sv * vs;
           // an unseen key's value may be NaN
-          const bool odd = !(fabsf(wv) < INFINITY);
+          const bool odd = !(fabsf(wv) < INFINITY && finite);
           const Pair wv2 = pair(wv, wv), mv2 = pair(mv, mv);
           bar_wait(pvdone + 8 * st, ph ^ 1, alive, err);       // the buffer's last reader
           uint8_t *pt = sm + L::P + st * L::PTile + mykey * 128;

@@ -107,8 +107,8 @@ template <typename T, int HD, int BITS, int NR, int WR, bool PACK> struct Plan {
   static constexpr int Ring = WK * Stages * G::Stage;
   static constexpr int Pitch = HD + 4;                     // floats of a row when states are joined
   static constexpr int Join = WK * Rows * Pitch * 4;        // over the fragments and the ring
-  // row factors, row sums, masks, per-warp (max, sum)
-  static constexpr int Small = Rows * 4 + Rows * 4 + Rows * 8 + WK * Rows * 8;
+  // row factors, row sums, masks, per-warp (max, sum), per-warp limits
+  static constexpr int Small = Rows * 4 + Rows * 4 + Rows * 8 + WK * Rows * 8 + WK * Rows * 4;
   static constexpr int Bytes = Small + (Q + Ring > Join ? Q + Ring : Join);
 };
 
@@ -151,7 +151,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   float *row_sum = row_f + P::Rows;                                  // sum of its query
   uint64_t *row_mask = reinterpret_cast<uint64_t *>(row_sum + P::Rows);
   float2 *ml = reinterpret_cast<float2 *>(row_mask + P::Rows);       // [WK][Rows]
-  uint8_t *qf = reinterpret_cast<uint8_t *>(ml + WK * P::Rows);
+  uint32_t *row_lim = reinterpret_cast<uint32_t *>(ml + WK * P::Rows);  // [WK][Rows], if apart
+  uint8_t *qf = reinterpret_cast<uint8_t *>(row_lim + WK * P::Rows);
   uint8_t *ring = qf + P::Q;
   float *join = reinterpret_cast<float *>(qf);
 
@@ -256,7 +257,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
       // the power of two that brings the largest value to [2^13, 2^14)
       int up = 140 - (int)(__float_as_uint(top) >> 23);
       if (top == 0.0f || !(top < INFINITY)) up = 0;
-      up = min(up, 126);
+      up = min(up, kTreeUp);
       const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
       for (int i = 0; i < Per; i++) {
@@ -277,9 +278,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
       if (part == 0) {
 #pragma unroll
         for (uint32_t c = r; c < P::Rows; c += PACK ? 4 : P::Rows) {
-          // never zero: a factor of zero would make NaN of a masked score
-          row_f[c] = fmaxf(a.scale * __uint_as_float((uint32_t)(127 - up) << 23),
-                           1.17549435e-38f);
+          row_f[c] = fmaxf(a.scale * __uint_as_float((uint32_t)(127 - up) << 23), kTreeFactor);
           row_sum[c] = sum;
           row_mask[c] = mask;
         }
@@ -299,7 +298,12 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
 #pragma unroll
       for (int r = 0; r < 2; r++) m[n][r] = -INFINITY, l[n][r] = base[n][r] = 0.0f;
     float vs = 1.0f;               // the weights are p s vs
-    uint32_t vlimit = 0;           // scales below these bits fit vs
+    uint32_t vlimit = kTreeNone;   // scales below these bits fit vs
+    // Rows see different nodes, so there a row has a limit of its own, and where
+    // the limits differ (VLIMIT is kTreeOwn) its reference M is not the maximum so
+    // far but off it by as many powers of two: a node that a row does not see costs
+    // it no bits.
+    uint32_t *lim = row_lim + wk * P::Rows + r0;
 
     for (uint32_t tile = t0; tile < t1; tile++) {
       copy_wait<Stages - 2>();
@@ -449,12 +453,62 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
       uint32_t big = BITS == 8 ? vw[lane] : vw[lane] << 16;
       big = __reduce_max_sync(0xffffffffu, big < 0x7f800000u ? big : 0u);
       float ratio = 1.0f;
-      if (big >= vlimit && big != 0) {
-        const uint32_t e = (big >> 23) + 1;             // scales below 2^(e - 127)
-        vlimit = e << 23;
-        const float next_vs = __uint_as_float((269u - e) << 23);   // to below 2^15
-        ratio = next_vs / vs;
-        vs = next_vs;
+      if (big >= vlimit) {
+        const bool apart = vlimit == kTreeOwn;
+        const uint32_t before = vlimit == kTreeNone ? 0 : 269u - (__float_as_uint(vs) >> 23);
+        uint32_t e = limit_of(big);
+        if (k0 + kTreeKeys > prefix) {                  // some keys are nodes
+          uint32_t own[NR][2], most = 0, least = ~0u;
+#pragma unroll
+          for (int n = 0; n < NR; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+              uint32_t v = 0;
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const uint32_t at = 16 * (i >> 1) + 2 * (i & 1);
+                const uint32_t w = __float_as_uint(scale_of<BITS>(vw[at + krow]));
+                if ((see[n][r] >> at & 1) && w < 0x7f800000u) v = max(v, w);
+              }
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, x));
+              own[n][r] = max(apart ? lim[8 * n + r] : before, v ? limit_of(v) : 0u);
+              most = max(most, own[n][r]);
+              if (own[n][r]) least = min(least, own[n][r]);
+            }
+          most = __reduce_max_sync(0xffffffffu, most);
+          least = __reduce_min_sync(0xffffffffu, least);
+          e = common_limit(before, least, most);
+          bool differ = false;
+#pragma unroll
+          for (int n = 0; n < NR; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+              // the maximum so far, and the reference that many powers of two off it
+              float v = fmaxf(fmaxf(s[0][n][r], s[0][n][2 + r]), fmaxf(s[1][n][r], s[1][n][2 + r]));
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+              const int was = apart ? apart_by(before, lim[8 * n + r]) : 0;
+              const float one = 1.0f / f[n][r];
+              if (m[n][r] != -INFINITY) v = fmaxf(v, fmaf((float)was, one, m[n][r]));
+              top[n][r] = v == -INFINITY ? v : fmaf((float)-apart_by(e, own[n][r]), one, v);
+              differ |= own[n][r] != e;
+            }
+          __syncwarp();                                 // every lane has read the limits
+#pragma unroll
+          for (int n = 0; n < NR; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) lim[8 * n + r] = own[n][r];   // of all lanes the same
+          __syncwarp();
+          vlimit = __any_sync(0xffffffffu, differ) ? kTreeOwn : e ? e << 23 : kTreeNone;
+        } else {
+          vlimit = e << 23;
+        }
+        if (e) {
+          const float next_vs = __uint_as_float((269u - e) << 23);   // to below 2^15
+          ratio = next_vs / vs;
+          vs = next_vs;
+        }
         moved = true;
       }
       if (__any_sync(0xffffffffu, moved)) {

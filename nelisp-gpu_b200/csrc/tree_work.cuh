@@ -209,6 +209,33 @@ __device__ __forceinline__ uint32_t codes4_high(uint32_t w) {
   return h2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), as_h2(0x2c002c00u),
                     as_h2(0xd480d480u)));   // (1024 + 16 c) / 16 - 64 - 8
 }
+// The limits of value scales, as exponents: scales below 2^(e - 127), 0 before
+// any was met.  Where the rows' own limits differ, E is the one the common power of
+// two of the weights goes by -- that of the keys before, or the least, unless the
+// largest is more than kTreeApart above it -- and a row's weights are raised over
+// it by the powers of two that apart_by says.  (Largest cases: 2^60 up or down
+// leaves sums of weights their whole range, and what is cut at 2^60 comes out of the
+// 15 bits that float16 has to spare.)
+constexpr int kTreeApart = 60;
+// What stands for a limit before any scale was met, and where rows have their own:
+// less than any scale's bits but zero's, so that a scale met is looked at.
+constexpr uint32_t kTreeNone = 1, kTreeOwn = 2;
+__device__ __forceinline__ uint32_t limit_of(uint32_t scale) {
+  return max((scale >> 23) + 1, 16u);            // the least scale is 2^-112
+}
+__device__ __forceinline__ uint32_t common_limit(uint32_t before, uint32_t least, uint32_t most) {
+  const int from = before ? (int)before : most ? (int)least : 0;
+  return (uint32_t)max(from, (int)most - kTreeApart);
+}
+__device__ __forceinline__ int apart_by(uint32_t e, uint32_t own) {
+  return own ? max(-kTreeApart, min((int)e - (int)own, kTreeApart)) : 0;
+}
+// A query row is raised by at most 2^kTreeUp to float16's range (below, what it
+// loses is less than 2^-100 of a score), and its factor is at least kTreeFactor:
+// a factor of zero would make NaN of a masked score, and 2^kTreeApart over it has to
+// be finite.
+constexpr int kTreeUp = 100;
+constexpr float kTreeFactor = 7.70371978e-34f;   // 2^-110
 // Scale and offset of a parameter word.  Four-bit codes are used less 8, so
 // the offset is that of the middle of the range: with it at the low end the
 // two sums q.c and lo sum(q) would be large and of opposite signs.
