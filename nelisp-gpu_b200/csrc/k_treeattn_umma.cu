@@ -257,11 +257,15 @@ template <bool SUM> __device__ __forceinline__ float across(uint32_t (&v)[H]) {
   return join(r, __shfl_xor_sync(0xffffffffu, r, 16));
 }
 
-// The walk over the parts of items that a CTA has, the same in every role.
+// The walk over the parts of items that a CTA has, the same in every role.  A part
+// is taken in runs of at most kTreeRunUmma tiles, each joined with the state that the
+// one before (RESUMED) left in the workspace.
 struct Walk {
   uint32_t at, end, before;
   uint32_t b, items;
   uint32_t head, row0, t0, t1, tiles;
+  bool any, resumed, more;
+  bool from0;                    // the part begins the item
   __device__ __forceinline__ bool begin(const TreeArgs &a) {
     const List list = list_of(a);
     if (blockIdx.x >= list.workers) return false;
@@ -269,6 +273,7 @@ struct Walk {
     end = share(list.total, list.workers, blockIdx.x + 1);
     items = a.pool.kv_heads * a.row_tiles;
     locate(a, at, &b, &before);
+    any = false;
     return true;
   }
   __device__ __forceinline__ bool next(const TreeArgs &a) {
@@ -281,11 +286,16 @@ struct Walk {
         continue;
       }
       const uint32_t item = (at - before) / cost, c0 = (at - before) % cost;
-      const uint32_t c1 = end - at < cost - c0 ? c0 + (end - at) : cost;
+      const uint32_t all = end - at < cost - c0 ? c0 + (end - at) : cost;
+      const uint32_t c1 = min(all, max(c0, a.item_cost) + kTreeRunUmma);
+      resumed = any && c0 != 0;
+      more = c1 < all;
       at += c1 - c0;
+      any = true;
       if (c1 <= a.item_cost) continue;
       t0 = c0 > a.item_cost ? c0 - a.item_cost : 0;
       t1 = c1 - a.item_cost;
+      if (!resumed) from0 = t0 == 0;
       head = item / a.row_tiles;
       row0 = item % a.row_tiles * a.rows_at_once;
       return true;
@@ -799,8 +809,8 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         }
 
         // ---- the end of the item: sums over the keys, and the output ----
-        const bool part_of = !(w.t0 == 0 && w.t1 == w.tiles);
-        const uint32_t slot = 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0);
+        const bool part_of = w.more || !(w.from0 && w.t1 == w.tiles);
+        const uint32_t slot = 2 * blockIdx.x + (w.from0 ? 1 : 0);
         {
           uint32_t v[H];
 #pragma unroll
@@ -826,19 +836,31 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         if (mykey < H) {
           const uint32_t n = n0 + mykey, row = w.row0 + n;
           const float *p = warp_part + n, *q = warp_base + n;
-          const float sum = (p[0] + p[N]) + (p[2 * N] + p[3 * N]);
+          float sum = (p[0] + p[N]) + (p[2 * N] + p[3 * N]);
+          float top = ref[n] == kFar ? -INFINITY : -ref[n];
+          float *ml = a.part_ml + ((uint64_t)slot * N + n) * 2;
+          // what this run and those before it weigh (one of NaN may have no maximum)
+          float now = 1.0f, old = 0.0f;
+          if (w.resumed) {
+            const float x = ml[0], y = ml[1], both = fmaxf(top, x);
+            now = top == both ? 1.0f : ex2(top - both);
+            old = x == both ? 1.0f : ex2(x - both);
+            sum = now * sum + old * y;
+            top = both;
+          }
           const bool empty = masks[n] == 0 || sum == 0.0f;
-          const float top = ref[n] == kFar ? -INFINITY : -ref[n];
           if (part_of) {
-            a.part_ml[((uint64_t)slot * N + n) * 2] = top;
-            a.part_ml[((uint64_t)slot * N + n) * 2 + 1] = sum;
+            ml[0] = top;
+            ml[1] = sum;
           } else if (row < a.rows && a.lse) {
             a.lse[((uint64_t)w.b * a.nodes + row / a.group) * a.heads + w.head * a.group +
                   row % a.group] = empty ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
           }
           // what the output is multiplied by, 0 for a row without keys, and what
           // the offsets add to it
-          const float by = part_of ? 1.0f : empty ? 0.0f : 1.0f / sum;
+          float by = part_of ? 1.0f : empty ? 0.0f : 1.0f / sum;
+          factor[n] = by * old;
+          by *= now;
           keep[n] = by / vs;
           qsum[n] = BITS == 4 && by != 0.0f ? by * ((q[0] + q[N]) + (q[2 * N] + q[3 * N])) : 0.0f;
         }
@@ -855,7 +877,8 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             for (int i = 0; i < H; i++) {
               const uint32_t n = n0 + i;
               const float k = keep[n];
-              const float v = k == 0.0f ? 0.0f : fmaf(__uint_as_float(o[i]), k, qsum[n]);
+              float v = k == 0.0f ? 0.0f : fmaf(__uint_as_float(o[i]), k, qsum[n]);
+              if (w.resumed && factor[n] != 0.0f) v = fmaf(part[i * HD], factor[n], v);
               const uint64_t at = offs[n];
               if (part_of) part[i * HD] = v;
               else if (at != ~0ull) ((__nv_bfloat16 *)a.o)[at + d] = __float2bfloat16_rn(v);

@@ -164,6 +164,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   const uint32_t total = list.total, workers = list.workers;
   if (blockIdx.x >= workers) return;
   uint32_t at = share(total, workers, blockIdx.x);
+  const uint32_t begin = at;
+  uint32_t part0 = 0;            // the first tile of this CTA's part of an item, over its runs
   const uint32_t end = share(total, workers, blockIdx.x + 1);
   uint32_t b;
   uint32_t before;
@@ -188,10 +190,20 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
       continue;
     }
     const uint32_t item = (at - before) / cost, c0 = (at - before) % cost;
-    const uint32_t c1 = end - at < cost - c0 ? c0 + (end - at) : cost;
+    uint32_t c1 = end - at < cost - c0 ? c0 + (end - at) : cost;
+    // Where the sums stay in the tensor core's accumulator a part is taken in
+    // runs, each joined with the state that the one before left in the workspace.
+    bool resumed = false, more = false;
+    if constexpr (!Flush) {
+      const uint32_t most = max(c0, a.item_cost) + kTreeRun;
+      resumed = c0 != 0 && at != begin;
+      more = c1 > most;
+      c1 = min(c1, most);
+    }
     at += c1 - c0;
     if (c1 <= a.item_cost) continue;             // its share ends before the first tile
     const uint32_t t0 = c0 > a.item_cost ? c0 - a.item_cost : 0, t1 = c1 - a.item_cost;
+    if (Flush || !resumed) part0 = t0;
     const uint32_t head = item / a.row_tiles, row0 = item % a.row_tiles * Live;
     const uint32_t prefix = prefix_of(a, b), keys = keys_of(a, b);
 
@@ -657,6 +669,19 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
       float top = -INFINITY, sum = 0.0f, c[WK];
 #pragma unroll
       for (int w = 0; w < WK; w++) top = fmaxf(top, ml[w * P::Rows + r].x);
+      const bool part_of = more || !(part0 == 0 && t1 == tiles);
+      const uint32_t slot = 2 * blockIdx.x + (part0 == 0 ? 1 : 0);
+      float run = 0.0f;              // what the runs before weigh
+      if constexpr (!Flush) {
+        if (resumed) {
+          const float2 before =
+              *reinterpret_cast<const float2 *>(a.part_ml + ((uint64_t)slot * P::Rows + r) * 2);
+          top = fmaxf(top, before.x);
+          run = before.x == -INFINITY ? (before.y != before.y ? 1.0f : 0.0f) : ex2(before.x - top);
+          sum = run * before.y;
+        }
+        __syncwarp();                // the row's threads have read it
+      }
 #pragma unroll
       for (int w = 0; w < WK; w++) {
         const float2 v = ml[w * P::Rows + r];
@@ -665,8 +690,6 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
         if (v.x == -INFINITY && v.y != v.y) c[w] = 1.0f;
         sum = fmaf(c[w], v.y, sum);
       }
-      const bool part_of = !(t0 == 0 && t1 == tiles);
-      const uint32_t slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
       const bool empty = row_mask[r] == 0 || sum == 0.0f;
       const float inv = 1.0f / sum;
       const uint32_t node = row / a.group, h = head * a.group + row % a.group;
@@ -675,6 +698,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
       for (int i = 0; i < Per; i++) {
         const uint32_t d = i * PerRow + part;
         float v = 0.0f;
+        if (!Flush && run != 0.0f) v = run * a.part_o[((uint64_t)slot * P::Rows + r) * HD + d];
 #pragma unroll
         for (int w = 0; w < WK; w++)
           if (c[w] != 0.0f) {

@@ -179,9 +179,19 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
-// o += codes x weights.  The tensor core cuts, not rounds, what it adds to an
-// accumulator, and over a long context that drifts; where the output is
-// float32 each 16 keys are summed apart and added in float32.
+// The tensor core cuts, not rounds, what it adds to an accumulator: with values of
+// one sign the sum falls behind by 0.5e-7 of itself an addition here, 1e-7 by
+// tcgen05 (measured; 8 bits, 100,000 keys in one part: mean error -3.0e-4 and
+// -6.5e-4).  Where the output is float32 each 16 keys are summed apart and added in
+// float32.  Where it is bfloat16, whose rounding is 2^-9, a part longer than
+// kTreeRun tiles of 32 keys (two additions each) or kTreeRunUmma of 128 (eight each)
+// is taken in runs of that many, joined in float32: at most 2,048 additions and
+// 2^-12.  (Sums taken out of the accumulator within the loop over the tiles made
+// every call of the tcgen05 form 8 to 12% slower, however rare and small the code; a
+// run costs about seven tiles, 3% of a long part.)
+constexpr uint32_t kTreeRun = 512, kTreeRunUmma = 256;
+
+// o += codes x weights.
 template <int Terms, int NR, bool Flush>
 __device__ __forceinline__ void weigh(float (&o)[4], const uint4 &c,
                                       const uint32_t (&p)[Terms][NR][2], int n) {

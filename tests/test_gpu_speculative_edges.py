@@ -80,3 +80,99 @@ def test_whatever_an_unused_node_holds(dev, torch, name, M, H, d, bits):  # noqa
         if want is None:
             want = got
         assert np.array_equal(got, want)                # to the bit what it is without them
+
+
+# ---- long contexts in one part ---------------------------------------------------------
+#
+# 160 sequences over the same pages give every CTA items of its own, so a part is
+# as long as the context.
+
+def long_case(torch, name, M, H, d, bits, bs, n, B, shape):  # noqa: F811
+    """Q, cache, table, lengths, masks, and keys and values as float64: scores
+    gamma_row a_t that are flat, or rise or fall along the keys, and positive values
+    whose mean goes with the score."""
+    g = torch.Generator(device="cuda").manual_seed(n + d + M)
+    nb = -(-(n + M) // bs)
+    N = nb * bs
+    u = torch.randn(d, device="cuda", generator=g)
+    u /= u.norm()
+    a = torch.randn(N, device="cuda", generator=g)
+    along = torch.arange(N, device="cuda") / N
+    trend = {"flat": 0 * along, "rising": 8 * along, "falling": -8 * along}[shape]
+    V = 1.5 + torch.rand(d, device="cuda", generator=g) * torch.tanh(a)[:, None] \
+        + 0.3 * torch.rand(N, d, device="cuda", generator=g)
+    if shape != "flat":
+        V = V * torch.exp2(2 * along)[:, None]
+    parts = []
+    for x in ((a + trend)[:, None] * u * d ** 0.5, V):
+        code, word = S.quantise(x.cpu().numpy(), bits)
+        y = torch.from_numpy(S.values(code, word, bits)).double().cuda()
+        parts.append((torch.from_numpy(S.pack(code, bits)).cuda().view(nb, 1, bs, -1).contiguous(),
+                      torch.from_numpy(word.view(np.int32)).cuda().view(nb, 1, bs).contiguous(), y))
+    (kc, kp, k), (vc, vp, v) = parts
+    rows = B * M * H
+    gamma = torch.linspace(-1, 1, rows, device="cuda")
+    gamma = gamma[torch.randperm(rows, device="cuda", generator=g)]
+    if shape != "flat":
+        gamma = 0.75 + gamma / 4
+    q = (gamma[:, None] * u).view(B * M, H * d).to(S.dtype_of(torch, name))
+    table = torch.arange(nb, dtype=torch.int32, device="cuda").expand(B, nb).contiguous()
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    mask = torch.tensor(S.chain(M), dtype=torch.int64, device="cuda").expand(B, M).contiguous()
+    return q, (kc, kp, vc, vp), table, lens, mask, k, v
+
+
+def long_check(dev, torch, name, M, H, d, bits, bs, n, shape, B=160):  # noqa: F811
+    """The relative error of the outputs of four sequences."""
+    q, cache, table, lens, mask, k, v = long_case(torch, name, M, H, d, bits, bs, n, B, shape)
+    o, lse = torch.empty_like(q), torch.empty(B * M, H, device="cuda")
+    dev.tree_attn(q, *cache, table, lens, mask, o, d, lse=lse)
+    off = []
+    for b in range(0, B, B // 4):
+        for i in range(M):
+            row, see = b * M + i, n + i + 1
+            x = q[row].view(H, d).double()
+            s = x @ k[:see].T * d ** -0.5
+            want = torch.softmax(s, -1) @ v[:see]
+            far = (x.abs() @ k[:see].abs().T).amax(-1) * d ** -0.5
+            ls = torch.logsumexp(s, -1)
+            assert ((lse[row].double() - ls).abs() <=
+                    2 ** -20 * far + 2 ** -19 + 2 ** -20 * ls.abs()).all()
+            vmax = v[:see].abs().max()
+            tol = (2 ** -20 * far + 2 ** -19)[:, None] * vmax
+            if name == "bf16":                  # the weights' rounding, and the output's
+                tol = tol + 2 ** -11 * vmax + 2 ** -8 * want.abs()
+            got = o[row].view(H, d).double()
+            assert ((got - want).abs() <= tol).all()
+            off.append(((got - want) / want).flatten())
+    from nelisp_cuda import _lib as L
+    assert L.load().nl_wait_status() == L.NL_OK
+    return torch.cat(off)
+
+
+# One node of 8 and 16 heads, 128 rows with pages that the tcgen05 form does not
+# take, heads of 256; the tcgen05 form with 20, 64 and 128 rows, heads of 64 and 128.
+@pytest.mark.parametrize("M,H,d,bits,bs,n", [
+    (1, 8, 128, 8, 64, 300000), (1, 16, 128, 4, 64, 150000), (32, 4, 128, 8, 40, 200000),
+    (16, 4, 256, 8, 64, 200000), (20, 1, 128, 8, 64, 100000), (16, 4, 128, 8, 64, 100000),
+    (16, 4, 128, 8, 64, 300000), (16, 4, 64, 8, 64, 100000), (32, 4, 128, 4, 64, 100000),
+])
+def test_long_contexts_do_not_drift(dev, torch, M, H, d, bits, bs, n):  # noqa: F811
+    """The tensor core cuts what it adds to an accumulator: positive values lose
+    a little at every addition, 1e-7 at most.  The sums are taken out of it after
+    2,048 additions, 2^-12; the mean of at least 4,096 roundings to bfloat16 (2^-9 /
+    sqrt 3 each) stays within 2^-14."""
+    B = 600 if M == 1 else 160                  # for parts as long as the context
+    off = long_check(dev, torch, "bf16", M, H, d, bits, bs, n, "flat", B)
+    assert off.numel() >= 4096 and off.mean().abs() <= 2 ** -12 + 2 ** -14, off.mean()
+
+
+@pytest.mark.parametrize("shape", ["rising", "falling"])
+@pytest.mark.parametrize("name,M,H,d,bs", [
+    ("bf16", 1, 8, 128, 64), ("bf16", 32, 4, 128, 40), ("bf16", 4, 2, 256, 64),
+    ("bf16", 20, 1, 128, 64), ("bf16", 16, 4, 64, 64), ("f32", 2, 2, 128, 64)])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_long_contexts_with_a_trend(dev, torch, name, M, H, d, bits, bs, shape):  # noqa: F811
+    """Maxima and value scales that move after sums were taken out, and that do
+    not."""
+    long_check(dev, torch, name, M, H, d, bits, bs, 100000, shape, 600 if M == 1 else 160)
