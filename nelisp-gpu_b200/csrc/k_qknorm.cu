@@ -295,7 +295,9 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
             vb[i] = fma2(x0, sa[i], mul2(x1, cb[i % (BWD ? 1 : P)]));
           }
         } else {
-          // t = u x: dg += r t, and dx = r g u - x r^3 mean(g t)
+          // t = u x: dg += r t, and dx = r (g u - x r^2 mean(g t)), in an order in which
+          // nothing leaves float32's range that the gradient does not leave: r^3, or
+          // the mean times it, did for rows of a size of 1e14
           Pair ua[P], ub[P], dot = 0;
           split<T, HALF>(w[u][CH - 2], w[u][CH - 1], ua, ub);
 #pragma unroll
@@ -308,12 +310,12 @@ qk_norm_rope_kernel(const __grid_constant__ QkArgs a) {
             db[i] = fma2(t1, r2, db[i]);
             dot = fma2(t1, gb[i], fma2(t0, ga[i], dot));
           }
-          const float k = -(r * r) * r * (group_sum<G>(dot) * inv_d);
+          const float k = -r * (r * (group_sum<G>(dot) * inv_d));
           const Pair k2 = pair(k, k);
 #pragma unroll
           for (int i = 0; i < P; i++) {
-            va[i] = fma2(va[i], k2, mul2(mul2(ua[i], ga[i]), r2));
-            vb[i] = fma2(vb[i], k2, mul2(mul2(ub[i], gb[i]), r2));
+            va[i] = mul2(fma2(va[i], k2, mul2(ua[i], ga[i])), r2);
+            vb[i] = mul2(fma2(vb[i], k2, mul2(ub[i], gb[i])), r2);
           }
         }
         if (p.live && hh < h1) {

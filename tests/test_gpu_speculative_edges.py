@@ -176,3 +176,38 @@ def test_long_contexts_with_a_trend(dev, torch, name, M, H, d, bits, bs, shape):
     """Maxima and value scales that move after sums were taken out, and that do
     not."""
     long_check(dev, torch, name, M, H, d, bits, bs, 100000, shape, 600 if M == 1 else 160)
+
+
+# ---- the gradient of large and of small rows ----------------------------------------------
+
+@pytest.mark.parametrize("pairs", ["half", "adjacent"])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("size,eps", [(1e14, 1e-5), (1e17, 1e-5), (1e18, 1e-5), (1e-14, 0.0),
+                                      (1e-17, 0.0), (1e-3, 0.0)])
+@pytest.mark.parametrize("grad", [1e-8, 1.0, 1e6])
+def test_norm_rope_gradient_of_any_size(dev, torch, name, pairs, size, eps, grad):  # noqa: F811
+    """Wherever the sum of squares is a float32, so is the gradient, to the bound
+    that it has for rows of ordinary size (relative: nothing is added to it).  Some
+    vectors of size 1e18 are past that: their 1 / rms is 0, and so is what they give."""
+    n, h, k, d, _ = shape = (7, 3, 2, 128, 64)
+    rng = np.random.default_rng(4)
+    x, gq, gk, co, si, pos = S.norm_inputs(torch, rng, shape, name)
+    x *= size
+    dq = torch.from_numpy(rng.standard_normal((n, h * d)) * grad).to("cuda", x.dtype)
+    dk = torch.from_numpy(rng.standard_normal((n, k * d)) * grad).to("cuda", x.dtype)
+    dx = torch.full_like(x, 7.0)
+    dgq, dgk = torch.empty(d, device="cuda"), torch.empty(d, device="cuda")
+    dev.qk_norm_rope_bwd(x, gq, gk, co, si, pos, dq, dk, dx, dgq, dgk, eps=eps, pairs=pairs)
+    g = np.concatenate([np.tile(gq.cpu().numpy(), (h, 1)), np.tile(gk.cpu().numpy(), (k, 1))])
+    want, mag, dg, dgm = S.norm_rope_grad64(
+        S.heads64(x, n, h + k, d), g.astype(float), co.cpu().numpy().astype(float),
+        si.cpu().numpy().astype(float), pos.cpu().numpy(),
+        np.concatenate([S.heads64(dq, n, h, d), S.heads64(dk, n, k, d)], 1), float(np.float32(eps)),
+        pairs)
+    over = ((S.heads64(x, n, h + k, d) ** 2).sum(-1) > np.finfo(np.float32).max)[..., None]
+    assert over.any() == (size == 1e18)
+    want, mag, dg, dgm = (np.where(over, 0, t) for t in (want, mag, dg, dgm))
+    assert S.within(torch, S.heads64(dx, n, h + k, d), want, 128 * S.U * mag, name).all()
+    for have, part in ((dgq, slice(0, h)), (dgk, slice(h, h + k))):
+        assert (np.abs(have.cpu().numpy() - dg[:, part].sum((0, 1)))
+                <= 96 * S.U * dgm[:, part].sum((0, 1))).all()
