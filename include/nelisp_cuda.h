@@ -445,8 +445,9 @@ int nl_kv_read_dev(const nl_kv_rows_args *args, void *stream);
  * path of a draft tree to the end of its prefix: for each of BATCH sequences
  * COUNT (at most 64) slots SRC -> DST (int32 [batch][count]).  All sources of
  * a sequence are read before any of its destinations is written; a pair with
- * a slot outside the pool is skipped; different sequences must not share
- * slots.  Does not synchronise. */
+ * a slot outside the pool is skipped; of pairs with the same destination the
+ * last is kept; different sequences must not share slots.  Does not
+ * synchronise. */
 typedef struct {
   nl_kv_cache cache;
   const int32_t *src, *dst;

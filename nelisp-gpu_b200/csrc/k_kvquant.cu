@@ -376,7 +376,8 @@ kv_read_kernel(const __grid_constant__ KvRows r, const __grid_constant__ KvPool 
 }
 
 // Rows moved inside the pool, one block per (sequence, head): every source is
-// in shared memory before the first destination is written.
+// in shared memory before the first destination is written, and of pairs with one
+// destination the last alone is written, as one after the other would leave it.
 __global__ void __launch_bounds__(kThreads)
 kv_move_kernel(const __grid_constant__ KvPool p, const int32_t *src, const int32_t *dst,
                uint32_t count) {
@@ -388,6 +389,12 @@ kv_move_kernel(const __grid_constant__ KvPool p, const int32_t *src, const int32
   dst += (uint64_t)blockIdx.y * count;
   const uint32_t chunks = p.head_dim * p.bits / 128, per = chunks + 1;   // and the parameter
   const uint64_t bytes = (uint64_t)chunks * 16;
+  __shared__ uint32_t target[64], kept[64];      // the pairs' destinations, or ~0
+  if (threadIdx.x < count) {
+    const uint32_t from = (uint32_t)src[threadIdx.x], to = (uint32_t)dst[threadIdx.x];
+    const bool both = from / p.block_size < p.num_blocks && to / p.block_size < p.num_blocks;
+    target[threadIdx.x] = both ? to : ~0u;
+  }
   for (uint32_t i = threadIdx.x; i < count * per; i += kThreads) {
     const uint32_t slot = (uint32_t)src[i / per], block = slot / p.block_size, k = i % per;
     uint4 v = make_uint4(0, 0, 0, 0);
@@ -399,11 +406,17 @@ kv_move_kernel(const __grid_constant__ KvPool p, const int32_t *src, const int32
     held[i] = v;
   }
   __syncthreads();
+  if (threadIdx.x < count) {
+    const uint32_t to = target[threadIdx.x];
+    bool later = false;
+    for (uint32_t k = threadIdx.x + 1; k < count; k++) later |= target[k] == to;
+    kept[threadIdx.x] = later ? ~0u : to;
+  }
+  __syncthreads();
   for (uint32_t i = threadIdx.x; i < count * per; i += kThreads) {
-    const uint32_t from = (uint32_t)src[i / per], to = (uint32_t)dst[i / per], k = i % per;
-    const uint32_t block = to / p.block_size;
-    if (from / p.block_size >= p.num_blocks || block >= p.num_blocks) continue;
-    const uint32_t at = kv_row(p, block, to % p.block_size, head);
+    const uint32_t to = kept[i / per], k = i % per;
+    if (to == ~0u) continue;
+    const uint32_t at = kv_row(p, to / p.block_size, to % p.block_size, head);
     if (k < chunks) reinterpret_cast<uint4 *>(p.code[kv] + at * bytes)[k] = held[i];
     else p.param[kv][at] = held[i].x;
   }

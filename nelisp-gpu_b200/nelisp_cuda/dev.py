@@ -198,7 +198,8 @@ def kv_read(SLOT, KC, KP, VC, VP, K, V, stream=None):
 
 def kv_move(SRC, DST, KC, KP, VC, VP, head_dim, stream=None):
     """Move tokens between slots without requantising them: SRC, DST int32
-    [batch, count]; per sequence every source is read before any write."""
+    [batch, count]; per sequence every source is read before any write, and of
+    pairs with one destination the last is kept."""
     if stream is not None:
         return _on(stream, kv_move, SRC, DST, KC, KP, VC, VP, head_dim)
     rc = (_module or _load_serving()).kv_move(SRC, DST, KC, KP, VC, VP, head_dim)

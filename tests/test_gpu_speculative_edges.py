@@ -211,3 +211,31 @@ def test_norm_rope_gradient_of_any_size(dev, torch, name, pairs, size, eps, grad
     for have, part in ((dgq, slice(0, h)), (dgk, slice(h, h + k))):
         assert (np.abs(have.cpu().numpy() - dg[:, part].sum((0, 1)))
                 <= 96 * S.U * dgm[:, part].sum((0, 1))).all()
+
+
+# ---- equal slots ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits,d", [(8, 128), (4, 256), (8, 64)])
+def test_kv_move_to_equal_destinations(dev, torch, bits, d):  # noqa: F811
+    """Of pairs with one destination the last that is inside the pool is kept,
+    whole: codes and word."""
+    kvh, bs, nb, count = 2, 7, 40, 64
+    for seed in range(8):
+        rng = np.random.default_rng(seed)
+        cache = dev.kv_cache(nb, bs, kvh, d, bits)
+        for c in cache:
+            c.copy_(torch.from_numpy(rng.integers(0, 256, tuple(c.shape))).to(c.dtype))
+        perm = rng.permutation(nb * bs).astype(np.int32)
+        src = np.stack([perm[:count], perm[100:100 + count]])
+        dst = np.stack([rng.choice(src[0][:3], count), rng.choice(perm[200:205], count)])
+        src[0, -1], dst[1, -1], src[1, -2] = -1, nb * bs, 1 << 30      # skipped, though last
+        want = [c.cpu().numpy().copy() for c in cache]
+        old = [w.copy() for w in want]
+        for w, o in zip(want, old):
+            for b in range(2):
+                for a, z in zip(src[b], dst[b]):
+                    if 0 <= a < nb * bs and 0 <= z < nb * bs:
+                        w[z // bs, :, z % bs] = o[a // bs, :, a % bs]
+        dev.kv_move(torch.from_numpy(src).cuda(), torch.from_numpy(dst).cuda(), *cache, d)
+        for c, w in zip(cache, want):
+            assert np.array_equal(c.cpu().numpy(), w)
