@@ -423,9 +423,11 @@ typedef struct {
 
 /* nl_kv_append_dev quantises N tokens' keys and values (rows of
  * kv_heads*head_dim elements of DTYPE, 16-byte aligned, K_STRIDE and V_STRIDE
- * apart) into slots SLOT[i].  A slot outside the pool is skipped; of tokens
- * with the same slot one is kept, its key and value heads not necessarily of
- * the same token.  nl_kv_read_dev reads the slots back as values into the
+ * apart) into slots SLOT[i].  A slot outside the pool is skipped (-1, say, for
+ * rows of padding).  The slots inside it must differ: what a slot given to
+ * two tokens of one call holds afterwards is not defined (codes of one may
+ * stand under the word of the other); other slots are not affected.
+ * nl_kv_read_dev reads the slots back as values into the
  * rows of K and V; a slot outside the pool reads as zeros.  Neither
  * synchronises. */
 typedef struct {

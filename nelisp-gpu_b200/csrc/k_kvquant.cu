@@ -143,7 +143,10 @@ __device__ __forceinline__ float bf16_up(float x) {   // of a positive finite x
   return __uint_as_float((__float_as_uint(x) + 0xffffu) & 0xffff0000u);
 }
 
-// A warp's job: some of a token's heads, the values' after the keys'.
+// A warp's job: some of a token's heads, the values' after the keys'.  Nothing orders
+// the jobs, nor a vector's codes and its word: two tokens of one append with one slot
+// leave a mixture there, which the caller is told.  (One owner a slot would take
+// either a word per slot of the pool or every token's slot compared with all others.)
 struct Job {
   uint32_t token, h0, h1;
   uint32_t row;                  // of head 0 in the pool, or ~0

@@ -179,7 +179,8 @@ def kv_cache(num_blocks, block_size, kv_heads, head_dim, bits, device="cuda"):
 
 def kv_append(K, V, SLOT, KC, KP, VC, VP, stream=None):
     """Quantise the rows K and V ([n, kv_heads * hd], f32 or bf16, may be
-    strided) into the cache's token slots SLOT (int32 [n]; outside: skipped)."""
+    strided) into the cache's token slots SLOT (int32 [n]; outside: skipped; those
+    inside must differ, or a slot given twice holds a mixture)."""
     if stream is not None:
         return _on(stream, kv_append, K, V, SLOT, KC, KP, VC, VP)
     rc = (_module or _load_serving()).kv_append(K, V, SLOT, KC, KP, VC, VP)

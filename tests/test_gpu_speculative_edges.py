@@ -239,3 +239,27 @@ def test_kv_move_to_equal_destinations(dev, torch, bits, d):  # noqa: F811
         dev.kv_move(torch.from_numpy(src).cuda(), torch.from_numpy(dst).cuda(), *cache, d)
         for c, w in zip(cache, want):
             assert np.array_equal(c.cpu().numpy(), w)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_kv_append_to_a_slot_given_twice(dev, torch, bits, name):  # noqa: F811
+    """What such a slot holds is not defined; all others hold what they would."""
+    n, kvh, d, bs = 1500, 3, 128, 16
+    rng = np.random.default_rng(bits)
+    x = torch.from_numpy(rng.standard_normal((2, n, kvh * d))).to("cuda", S.dtype_of(torch, name))
+    nb = n // bs + 3
+    slot = rng.permutation(nb * bs)[:n].astype(np.int32)
+    alone = dev.kv_cache(nb, bs, kvh, d, bits)
+    dev.kv_append(x[0], x[1], torch.from_numpy(slot).cuda(), *alone)
+    twice = slot.copy()
+    twice[100:200] = slot[300:400]                  # and 100 slots get none
+    twice[7] = twice[8] = twice[9] = -1
+    cache = dev.kv_cache(nb, bs, kvh, d, bits)
+    dev.kv_append(x[0], x[1], torch.from_numpy(twice).cuda(), *cache)
+    other = np.setdiff1d(slot, np.concatenate([slot[300:400], slot[100:200], slot[7:10]]))
+    none = np.setdiff1d(np.arange(nb * bs), twice)
+    for c, a in zip(cache, alone):
+        c, a = c.cpu().numpy(), a.cpu().numpy()
+        assert np.array_equal(c[other // bs, :, other % bs], a[other // bs, :, other % bs])
+        assert not c[none // bs, :, none % bs].any()
