@@ -50,7 +50,7 @@ struct Api {
   decltype(&nl_tree_attn_dev) tree;
   c10::DeviceIndex device;
 } bound;
-PyObject *binder;                // binds them, on the first call whose tensors pass
+PyObject *binder;                // binds them, on the first call with a CUDA tensor
 
 Api &api() {
   if (!bound.tree) {
@@ -68,11 +68,17 @@ const Tensor &tensor(PyObject *o) {
   if (!THPVariable_Check(o)) refuse("expected a tensor, not ", Py_TYPE(o)->tp_name);
   return THPVariable_Unpack(o);
 }
+// The kernels run on the library's device.
+void on_device(const Tensor &t) {
+  if (t.get_device() != api().device)
+    refuse("a tensor on ", t.device(), ": the library's device is cuda:", (int)api().device);
+}
 const Tensor &flat(PyObject *o, ScalarType type) {
   const Tensor &t = tensor(o);
   if (t.scalar_type() != type || !t.is_cuda() || !t.is_contiguous())
     refuse("expected a contiguous CUDA tensor of ", type, ", not ", t.scalar_type(), " ", t.sizes(),
            " with strides ", t.strides(), " on ", t.device());
+  on_device(t);
   return t;
 }
 int row_type(const Tensor &t) {
@@ -87,6 +93,7 @@ const Tensor &rows(PyObject *o, ScalarType type) {
       (t.stride(1) != 1 && t.size(1) > 1))
     refuse("expected CUDA rows of ", type, " (2-D, unit inner stride), not ", t.scalar_type(), " ",
            t.sizes(), " with strides ", t.strides(), " on ", t.device());
+  on_device(t);
   return t;
 }
 uint32_t u32(int64_t v) {
@@ -103,7 +110,11 @@ float real(PyObject *o) {
   if (v == -1.0 && PyErr_Occurred()) throw Raised{};
   return (float)v;
 }
-void *stream() { return c10::cuda::getCurrentCUDAStream(api().device).stream(); }
+// The call, on the library's device and torch's current stream there.
+template <typename A> int launch(int (*entry)(const A *, void *), const A &args) {
+  const c10::cuda::CUDAGuard guard(api().device);
+  return entry(&args, c10::cuda::getCurrentCUDAStream(api().device).stream());
+}
 
 // WORKSPACE as given, or of the caching allocator: it belongs to the current
 // stream, so that calls on different streams never share one.
@@ -115,6 +126,7 @@ struct Workspace {
     if (given != Py_None) {
       const Tensor &t = tensor(given);
       if (!t.is_cuda() || !t.is_contiguous()) refuse("workspace: a contiguous CUDA tensor");
+      on_device(t);
       at = t.data_ptr();
       bytes = t.nbytes();
       return;
@@ -194,7 +206,7 @@ int norm_rope(PyObject *const *o) {
   x.q_stride = q.stride(0);
   x.k = k.data_ptr();
   x.k_stride = k.stride(0);
-  return api().norm_rope(&x, stream());
+  return launch(api().norm_rope, x);
 }
 
 // QKV GQ GK CO SI POS DQ DK DQKV DGQ DGK eps pairs workspace
@@ -222,7 +234,7 @@ int norm_rope_bwd(PyObject *const *o) {
   const Workspace ws(o[13], api().norm_rope_bwd_bytes(x.head_dim), qkv);
   x.workspace = ws.at;
   x.ws_bytes = ws.bytes;
-  return api().norm_rope_bwd(&x, stream());
+  return launch(api().norm_rope_bwd, x);
 }
 
 // ---- the cache ------------------------------------------------------------------
@@ -252,13 +264,13 @@ nl_kv_rows_args rows_of(PyObject *ko, PyObject *vo, PyObject *slots, PyObject *c
 // K V SLOT KC KP VC VP
 int kv_append(PyObject *const *o) {
   const nl_kv_rows_args x = rows_of(o[0], o[1], o[2], o + 3);
-  return api().kv_append(&x, stream());
+  return launch(api().kv_append, x);
 }
 
 // SLOT KC KP VC VP K V
 int kv_read(PyObject *const *o) {
   const nl_kv_rows_args x = rows_of(o[5], o[6], o[0], o + 1);
-  return api().kv_read(&x, stream());
+  return launch(api().kv_read, x);
 }
 
 // SRC DST KC KP VC VP head_dim
@@ -267,7 +279,7 @@ int kv_move(PyObject *const *o) {
   if (src.dim() != 2 || src.sizes() != dst.sizes()) refuse("SRC and DST: [batch, count] each");
   const nl_kv_move_args x = {cache_of(o + 2, integer(o[6])), (const int32_t *)src.data_ptr(),
                              (const int32_t *)dst.data_ptr(), u32(src.size(0)), u32(src.size(1))};
-  return api().kv_move(&x, stream());
+  return launch(api().kv_move, x);
 }
 
 // ---- tree attention ---------------------------------------------------------------
@@ -312,7 +324,7 @@ int tree_attn(PyObject *const *o) {
                      q);
   x.workspace = ws.at;
   x.ws_bytes = ws.bytes;
-  return api().tree(&x, stream());
+  return launch(api().tree, x);
 }
 
 // ---- the module -----------------------------------------------------------------

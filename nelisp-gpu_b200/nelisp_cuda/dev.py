@@ -132,8 +132,12 @@ def _load_serving():
 
 
 def _on(stream, function, *args):
-    """FUNCTION with STREAM as the current one."""
+    """FUNCTION with STREAM, one of the library's device, as the current one."""
     import torch
+    _lib()
+    if stream.device_index != _device:
+        raise ValueError(f"a stream of cuda:{stream.device_index}: the library's device is "
+                         f"cuda:{_device}")
     with torch.cuda.stream(stream):
         return function(*args)
 

@@ -263,3 +263,42 @@ def test_kv_append_to_a_slot_given_twice(dev, torch, bits, name):  # noqa: F811
         c, a = c.cpu().numpy(), a.cpu().numpy()
         assert np.array_equal(c[other // bs, :, other % bs], a[other // bs, :, other % bs])
         assert not c[none // bs, :, none % bs].any()
+
+
+# ---- tensors and streams of another device -------------------------------------------------
+
+def test_tensors_of_another_device_are_refused(dev, torch):  # noqa: F811
+    """The mismatch is made on the host: the module is told that the library is
+    on the next device, so that these tensors are the foreign ones.  Nothing is
+    launched."""
+    x, gq, gk, co, si, pos = S.norm_inputs(torch, np.random.default_rng(1), (4, 2, 1, 64, 64), "f32")
+    q, k = torch.empty(4, 128, device="cuda"), torch.empty(4, 64, device="cuda")
+    cache = dev.kv_cache(2, 16, 1, 64, 8)
+    slot = torch.arange(4, dtype=torch.int32, device="cuda")
+    one = torch.ones(4, 1, dtype=torch.int64, device="cuda")
+    calls = [lambda: dev.qk_norm_rope(x, gq, gk, co, si, pos, q, k),
+             lambda: dev.qk_norm_rope_bwd(x, gq, gk, co, si, pos, q, k, x.clone(), gq.clone(),
+                                          gk.clone()),
+             lambda: dev.kv_append(k, k, slot, *cache),
+             lambda: dev.kv_read(slot, *cache, k, k.clone()),
+             lambda: dev.kv_move(slot.view(2, 2), slot.view(2, 2), *cache, 64),
+             lambda: dev.tree_attn(k, *cache, slot.view(4, 1) % 2, slot, one, k.clone(), 64)]
+    for call in calls:
+        call()
+    device = dev._device
+    try:
+        dev._device = device + 1
+        dev._bind()
+        before = dev.launch_count()
+        for call in calls:
+            with pytest.raises(ValueError, match="device"):
+                call()
+        with pytest.raises(ValueError, match="stream"):
+            dev.kv_append(k, k, slot, *cache, stream=torch.cuda.current_stream())
+        assert dev.launch_count() == before
+    finally:
+        dev._device = device
+        dev._bind()
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
