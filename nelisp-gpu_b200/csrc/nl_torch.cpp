@@ -96,6 +96,11 @@ const Tensor &rows(PyObject *o, ScalarType type) {
   on_device(t);
   return t;
 }
+// Elements from a row to the next.  One row may have any stride (torch calls it
+// contiguous all the same), and none is used.
+uint64_t stride_of(const Tensor &t) {
+  return t.size(0) > 1 ? (uint64_t)t.stride(0) : ((uint64_t)t.size(1) + 7) / 8 * 8;
+}
 uint32_t u32(int64_t v) {
   if (v < 0 || v > (int64_t)UINT32_MAX) refuse("a size of ", v, " does not fit 32 bits");
   return (uint32_t)v;
@@ -179,7 +184,7 @@ void norm_rope_fields(A &x, PyObject *const *o, const Tensor &qkv, const Tensor 
   else
     refuse("pairs: 'half' or 'adjacent'");
   x.qkv = qkv.data_ptr();
-  x.x_stride = qkv.stride(0);
+  x.x_stride = stride_of(qkv);
   x.gq = (const float *)gq.data_ptr();
   x.gk = (const float *)gk.data_ptr();
   x.co = (const float *)co.data_ptr();
@@ -203,9 +208,9 @@ int norm_rope(PyObject *const *o) {
   const Tensor &qkv = rows(o[0], type), &q = rows(o[6], type), &k = rows(o[7], type);
   norm_rope_fields(x, o, qkv, q, k, o[8], o[9]);
   x.q = q.data_ptr();
-  x.q_stride = q.stride(0);
+  x.q_stride = stride_of(q);
   x.k = k.data_ptr();
-  x.k_stride = k.stride(0);
+  x.k_stride = stride_of(k);
   return launch(api().norm_rope, x);
 }
 
@@ -224,11 +229,11 @@ int norm_rope_bwd(PyObject *const *o) {
   if (dqkv.size(0) != x.n || dqkv.size(1) < dq.size(1) + dk.size(1))
     refuse("DQKV of ", dqkv.sizes(), " for ", x.n, " rows");
   x.dq = dq.data_ptr();
-  x.dq_stride = dq.stride(0);
+  x.dq_stride = stride_of(dq);
   x.dk = dk.data_ptr();
-  x.dk_stride = dk.stride(0);
+  x.dk_stride = stride_of(dk);
   x.dqkv = dqkv.data_ptr();
-  x.dx_stride = dqkv.stride(0);
+  x.dx_stride = stride_of(dqkv);
   x.dgq = (float *)dgq.data_ptr();
   x.dgk = (float *)dgk.data_ptr();
   const Workspace ws(o[13], api().norm_rope_bwd_bytes(x.head_dim), qkv);
@@ -255,9 +260,9 @@ nl_kv_rows_args rows_of(PyObject *ko, PyObject *vo, PyObject *slots, PyObject *c
   x.n = u32(k.size(0));
   x.slot = (const int32_t *)slot.data_ptr();
   x.k = k.data_ptr();
-  x.k_stride = k.stride(0);
+  x.k_stride = stride_of(k);
   x.v = v.data_ptr();
-  x.v_stride = v.stride(0);
+  x.v_stride = stride_of(v);
   return x;
 }
 
@@ -314,12 +319,12 @@ int tree_attn(PyObject *const *o) {
   x.max_blocks = u32(table.size(1));
   x.scale = o[10] == Py_None ? (float)(1.0 / std::sqrt((double)head_dim)) : real(o[10]);
   x.q = q.data_ptr();
-  x.q_stride = q.stride(0);
+  x.q_stride = stride_of(q);
   x.table = (const int32_t *)table.data_ptr();
   x.len = (const int32_t *)len.data_ptr();
   x.mask = (const uint64_t *)mask.data_ptr();
   x.o = out.data_ptr();
-  x.o_stride = out.stride(0);
+  x.o_stride = stride_of(out);
   const Workspace ws(o[12], api().tree_bytes(x.nodes, x.heads, x.cache.kv_heads, x.cache.head_dim),
                      q);
   x.workspace = ws.at;

@@ -302,3 +302,44 @@ def test_tensors_of_another_device_are_refused(dev, torch):  # noqa: F811
     for call in calls:
         call()
     torch.cuda.synchronize()
+
+
+# ---- one row, whatever its stride -------------------------------------------------------------
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_one_row_of_any_stride(dev, torch, name):  # noqa: F811
+    """A single row has no stride that matters: that of a transposed column is 1,
+    of an expanded vector 0."""
+    t = S.dtype_of(torch, name)
+    h, k, d = 4, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+
+    def odd(x, stride):
+        return x.clone().as_strided((1, x.numel()), (stride, 1))
+
+    def rows(stride):
+        g.manual_seed(1)
+        x = odd(torch.randn(1, (h + 2 * k) * d, device="cuda", generator=g).to(t), stride)
+        gq, gk = torch.rand(2, d, device="cuda", generator=g).unbind()
+        gq, gk = gq.contiguous(), gk.contiguous()
+        co, si = torch.rand(2, 5, d // 2, device="cuda", generator=g).unbind()
+        pos = torch.tensor([3], dtype=torch.int32, device="cuda")
+        q, kk = (odd(torch.zeros(1, m * d, device="cuda", dtype=t), stride) for m in (h, k))
+        dev.qk_norm_rope(x, gq, gk, co, si, pos, q, kk)
+        dx = odd(torch.zeros_like(x), stride)
+        dev.qk_norm_rope_bwd(x, gq, gk, co, si, pos, q, kk, dx, gq.clone(), gk.clone())
+        cache = dev.kv_cache(2, 16, k, d, 8)
+        slot = torch.tensor([5], dtype=torch.int32, device="cuda")
+        v = odd(x[:, (h + k) * d:], stride)
+        dev.kv_append(kk, v, slot, *cache)
+        ko, vo = (odd(torch.zeros(1, k * d, device="cuda", dtype=t), stride) for _ in range(2))
+        dev.kv_read(slot, *cache, ko, vo)
+        o = odd(torch.zeros_like(q), stride)
+        dev.tree_attn(q, *cache, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), slot,
+                      torch.ones(1, 1, dtype=torch.int64, device="cuda"), o, d)
+        return [x.clone() for x in (q, kk, dx, *cache, ko, vo, o)]
+
+    want = rows(1 << 12)
+    assert all(x.float().abs().sum() > 0 for x in want[-3:])
+    for stride in (0, 1, 3):
+        assert all(torch.equal(a, b) for a, b in zip(rows(stride), want))
