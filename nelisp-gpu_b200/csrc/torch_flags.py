@@ -1,5 +1,17 @@
 """Prints the compiler flags of an extension of the torch that this interpreter
-has: its headers, Python's and CUDA's, and torch's libraries."""
+has: its headers, Python's and CUDA's, and torch's libraries.  With --which, prints
+which interpreter and torch these are instead, without importing it, and nothing
+where there is none."""
+import sys
+
+if sys.argv[1:] == ["--which"]:
+    import importlib.metadata
+    import importlib.util
+    spec = importlib.util.find_spec("torch")
+    if spec is not None and spec.origin:
+        print(sys.implementation.cache_tag, spec.origin, importlib.metadata.version("torch"))
+    sys.exit(0)
+
 import sysconfig
 
 from torch.utils import cpp_extension
