@@ -164,6 +164,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
       : "r"(at));
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
+__device__ __forceinline__ float tmem_ld1(uint32_t at) {
+  uint32_t v;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n"
+               "tcgen05.wait::ld.sync.aligned;\n" : "=r"(v) : "r"(at) : "memory");
+  return __uint_as_float(v);
+}
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
@@ -705,24 +711,33 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             score(s, false);
             const float mine = across<false>(s);
             if (lane < H) warp_part[(warp & 3) * N + n0 + lane] = mine;
-            if (nodes_here) {
-#pragma unroll
-              for (int i = 0; i < H; i++) s[i] = sees(i) ? vbits : 0u;
-              const float scale = across<false>(s);
-              if (lane < H) warp_scale[(warp & 3) * N + n0 + lane] = scale;
-            }
-            if (quad == 0 && lane == 0) *vote = before << 23;
+            uint32_t *low_vote = votes + 4 + group, *met = votes + 8 + group;
+            if (quad == 0 && lane == 0) *vote = before << 23, *low_vote = ~0u, *met = 0;
             group_sync(group);
-            if (!nodes_here) {
-              const uint32_t top_bits = __reduce_max_sync(0xffffffffu, vbits);
-              if (lane == 0 && top_bits >= vlimit) atomicMax(vote, limit_of(top_bits) << 23);
+            const uint32_t high = __reduce_max_sync(0xffffffffu, vbits);
+            if (lane == 0 && high != 0) atomicMax(vote, limit_of(high) << 23);
+            bool rows = false;                 // limits looked at row by row
+            if (nodes_here) {
+              const uint32_t low = __reduce_min_sync(0xffffffffu, vbits ? limit_of(vbits) : ~0u);
+              if (lane == 0) atomicMin(low_vote, low);
+              if (vbits != 0 && key < prefix) *met = 1;
+              group_sync(group);
+              rows = apart ||
+                     rows_apart(before, *low_vote, *vote >> 23, *met || tile + 1 == w.t1);
+              if (rows) {
+#pragma unroll
+                for (int i = 0; i < H; i++) s[i] = sees(i) ? vbits : 0u;
+                const float scale = across<false>(s);
+                if (lane < H) warp_scale[(warp & 3) * N + n0 + lane] = scale;
+                group_sync(group);
+              }
             }
             if (mykey < H) {
               const uint32_t n = n0 + mykey;
               const float *p = warp_part + n;
               const float most = fmaxf(fmaxf(p[0], p[N]), fmaxf(p[2 * N], p[3 * N]));
               int was = 0, now = 0;                          // powers of two of the reference
-              if (nodes_here) {
+              if (rows) {
                 const float *z = warp_scale + n;
                 const float scale = fmaxf(fmaxf(z[0], z[N]), fmaxf(z[2 * N], z[3 * N]));
                 const uint32_t had = apart ? lim[n] : before;
@@ -868,7 +883,21 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
         bar_wait(pvdone + 8 * (it - 1 & 1), (it - 1) >> 1 & 1, alive, err);
         fence_after();
         const uint32_t d = natural<BITS>(mykey);       // the value this TMEM lane holds
-        {
+        if (w.resumed) {
+          float *part = a.part_o + ((uint64_t)slot * N + n0) * HD + d;
+#pragma unroll 1
+          for (int i = 0; i < H; i++) {
+            const uint32_t n = n0 + i;
+            const float x = tmem_ld1(tmem + (quad << 16) + L::TO + n), k = keep[n], f = factor[n];
+            if (HD == 128 || quad < 64) {
+              float v = k == 0.0f ? 0.0f : fmaf(x, k, qsum[n]);
+              if (f != 0.0f) v = fmaf(part[i * HD], f, v);
+              const uint64_t at = offs[n];
+              if (part_of) part[i * HD] = v;
+              else if (at != ~0ull) ((__nv_bfloat16 *)a.o)[at + d] = __float2bfloat16_rn(v);
+            }
+          }
+        } else {
           uint32_t o[H];
           tmem_ld16(tmem + (quad << 16) + L::TO + n0, o);
           if (HD == 128 || quad < 64) {
@@ -877,8 +906,7 @@ tree_umma_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUt
             for (int i = 0; i < H; i++) {
               const uint32_t n = n0 + i;
               const float k = keep[n];
-              float v = k == 0.0f ? 0.0f : fmaf(__uint_as_float(o[i]), k, qsum[n]);
-              if (w.resumed && factor[n] != 0.0f) v = fmaf(part[i * HD], factor[n], v);
+              const float v = k == 0.0f ? 0.0f : fmaf(__uint_as_float(o[i]), k, qsum[n]);
               const uint64_t at = offs[n];
               if (part_of) part[i * HD] = v;
               else if (at != ~0ull) ((__nv_bfloat16 *)a.o)[at + d] = __float2bfloat16_rn(v);

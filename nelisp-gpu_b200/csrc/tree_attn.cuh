@@ -462,14 +462,21 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
         }
       }
       // the largest finite scale of the values decides the weights' power of two
-      uint32_t big = BITS == 8 ? vw[lane] : vw[lane] << 16;
-      big = __reduce_max_sync(0xffffffffu, big < 0x7f800000u ? big : 0u);
+      uint32_t one = BITS == 8 ? vw[lane] : vw[lane] << 16;
+      one = one < 0x7f800000u ? one : 0u;
+      const uint32_t big = __reduce_max_sync(0xffffffffu, one);
       float ratio = 1.0f;
       if (big >= vlimit) {
         const bool apart = vlimit == kTreeOwn;
         const uint32_t before = vlimit == kTreeNone ? 0 : 269u - (__float_as_uint(vs) >> 23);
         uint32_t e = limit_of(big);
+        bool rows = false;                              // looked at one by one
         if (k0 + kTreeKeys > prefix) {                  // some keys are nodes
+          const uint32_t low = __reduce_min_sync(0xffffffffu, one ? limit_of(one) : ~0u);
+          const bool met = __any_sync(0xffffffffu, one != 0 && k0 + lane < prefix);
+          rows = apart || rows_apart(before, low, e, met || tile + 1 == t1);
+        }
+        if (rows) {
           uint32_t own[NR][2], most = 0, least = ~0u;
 #pragma unroll
           for (int n = 0; n < NR; n++)
@@ -501,9 +508,9 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
 #pragma unroll
               for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
               const int was = apart ? apart_by(before, lim[8 * n + r]) : 0;
-              const float one = 1.0f / f[n][r];
-              if (m[n][r] != -INFINITY) v = fmaxf(v, fmaf((float)was, one, m[n][r]));
-              top[n][r] = v == -INFINITY ? v : fmaf((float)-apart_by(e, own[n][r]), one, v);
+              const float unit = 1.0f / f[n][r];
+              if (m[n][r] != -INFINITY) v = fmaxf(v, fmaf((float)was, unit, m[n][r]));
+              top[n][r] = v == -INFINITY ? v : fmaf((float)-apart_by(e, own[n][r]), unit, v);
               differ |= own[n][r] != e;
             }
           __syncwarp();                                 // every lane has read the limits
@@ -690,6 +697,17 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
         if (v.x == -INFINITY && v.y != v.y) c[w] = 1.0f;
         sum = fmaf(c[w], v.y, sum);
       }
+      if constexpr (!Flush) {
+        if (resumed) {               // the runs before join the first warp's state
+#pragma unroll 1
+          for (int i = 0; i < Per; i++) {
+            float *x = join + r * P::Pitch + i * PerRow + part;
+            const float before = a.part_o[((uint64_t)slot * P::Rows + r) * HD + i * PerRow + part];
+            *x = (c[0] != 0.0f ? c[0] * *x : 0.0f) + (run != 0.0f ? run * before : 0.0f);
+          }
+          c[0] = 1.0f;
+        }
+      }
       const bool empty = row_mask[r] == 0 || sum == 0.0f;
       const float inv = 1.0f / sum;
       const uint32_t node = row / a.group, h = head * a.group + row % a.group;
@@ -698,7 +716,6 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
       for (int i = 0; i < Per; i++) {
         const uint32_t d = i * PerRow + part;
         float v = 0.0f;
-        if (!Flush && run != 0.0f) v = run * a.part_o[((uint64_t)slot * P::Rows + r) * HD + d];
 #pragma unroll
         for (int w = 0; w < WK; w++)
           if (c[w] != 0.0f) {

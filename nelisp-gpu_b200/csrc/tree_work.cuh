@@ -240,6 +240,16 @@ constexpr uint32_t kTreeNone = 1, kTreeOwn = 2;
 __device__ __forceinline__ uint32_t limit_of(uint32_t scale) {
   return max((scale >> 23) + 1, 16u);            // the least scale is 2^-112
 }
+// Whether that has to be looked at row by row, for a tile of nodes whose scales lie
+// in [LOW, E]: 2^kTreeSpare of difference fits the bits that float16 has to spare, and
+// then one limit serves all rows, unless a row may meet its first scale later (not
+// ALL: a prefix key that all rows see has one, or the tile is the last).  (Most calls
+// run the code for that nowhere: with it in every first tile of nodes 16 ragged
+// sequences of 32 rows took 5 us more.)
+constexpr uint32_t kTreeSpare = 10;
+__device__ __forceinline__ bool rows_apart(uint32_t before, uint32_t low, uint32_t e, bool all) {
+  return before ? e > before + kTreeSpare : !all || e > low + kTreeSpare;
+}
 __device__ __forceinline__ uint32_t common_limit(uint32_t before, uint32_t least, uint32_t most) {
   const int from = before ? (int)before : most ? (int)least : 0;
   return (uint32_t)max(from, (int)most - kTreeApart);

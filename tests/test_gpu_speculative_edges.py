@@ -59,6 +59,23 @@ def test_large_and_small_values_across_node_tiles(dev, torch, name, M, H, d, bit
         S.check_tree(dev, torch, q, kv, table, lens, m, bits, H, d)
 
 
+@pytest.mark.parametrize("name,M,H,d", [("f32", 60, 1, 128), ("bf16", 60, 1, 128),
+                                        ("bf16", 20, 1, 64), ("bf16", 60, 2, 64)])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_rows_that_meet_their_first_value_late(dev, torch, name, M, H, d, bits):  # noqa: F811
+    """No prefix key (its pages are outside the pool), and nodes over several
+    tiles: the first ones, of ordinary size, are seen by themselves alone, and the
+    last by themselves and small."""
+    rng = np.random.default_rng(6)
+    mask = [1 << i for i in range(M)]
+    for L in (112, 96):
+        q, kv, table, lens, m = S.attn_inputs(torch, rng, 1, M, H, 1, d, bits, 16, [L], [mask], name)
+        table[0, :L // 16] = -1
+        for i in range(M):
+            put(kv, table, L + i, rng.standard_normal(d) * (1.0 if i < M // 2 else 1e-12), bits)
+        S.check_tree(dev, torch, q, kv, table, lens, m, bits, H, d)
+
+
 @pytest.mark.parametrize("name,M,H,d", FORMS)
 @pytest.mark.parametrize("bits", [8, 4])
 def test_whatever_an_unused_node_holds(dev, torch, name, M, H, d, bits):  # noqa: F811
