@@ -30,7 +30,7 @@
 // else synchronises the CTA until an item ends.
 //
 // What bounds it: with few rows the loads.  8 sequences of 4,096 keys, 32 heads
-// of 128, float32, 8 bits: 61.0 us for 277 MB, 0.69 of a copy's rate; the same
+// of 128, float32, 8 bits: 61.5 us for 277 MB, 0.69 of a copy's rate; the same
 // without the products 50, the join 3.  With many rows the issue of products and
 // weights: the table at start_rows; in bfloat16 the tcgen05 form
 // (k_treeattn_umma.cu) takes over there.
@@ -874,7 +874,11 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
   }
   a.ctas = 148u * per_sm;
   a.tile = P::Tile;
-  a.item_cost = 4 * WR;          // about 512 keys
+  // About 512 keys.  (With WR, 2 WR, 4 WR, 8 WR, us: 16 sequences of 1,000 keys, 8 key
+  // heads, 4 rows, f32 17.4, 17.4, 19.0, 20.4; 3 of 4,096, 32 heads 29.9, 30.4, 31.4,
+  // 33.3; but 30 of 700, 8 heads, 4 rows, bf16, 4 bits 24.5, 23.6, 23.2, 20.2; one of
+  // 4,000, 64 rows, f32 42.1, 42.2, 42.4, 39.8; long or many items within 2%.)
+  a.item_cost = 4 * WR;
   cudaError_t e = launch_pdl(tree_attn_kernel<T, HD, BITS, NR, WR, PACK>, dim3(a.ctas),
                              dim3(kTreeThreads), (size_t)P::Bytes, st, a);
   count_launches(1);
@@ -886,24 +890,25 @@ cudaError_t start_rows(TreeArgs &a, cudaStream_t st) {
   // shares keys converts their codes again (us, 4 sequences of 32,768 keys, 8 key
   // heads of 128, 8 bits / 4 bits):
   //   rows               16         32         64         128
-  //   bf16  4 a warp   68/ 72    104/110    181/197    334/371
-  //         half       87/100    115/128    216/240    418/468
-  //   f32   4 a warp   90/ 90    225/158    312/293    561/562
-  //         half      111/117    155/164    297/321    622/677
-  // (half: 1 of 16 rows, 2 of more).  With both terms of float32 four tiles of 8
-  // bits spill, which only the joint reading of 128 rows makes up for; in 4 bits a
-  // step has one lane part of codes to hold, not two.
+  //   bf16  4 a warp   69/ 73    100/106    176/193    330/367
+  //         half       85/ 98    114/129    209/235    383/424
+  //   f32   4 a warp   88/ 87    193/148    274/286    508/550
+  //         half      108/112    159/156    293/304    544/565
+  // (half: 1 of 16 rows, 2 of more, 128 as two items of 64.)  32 rows of float32 in 8
+  // bits are the exception: one warp with four tiles holds both terms of both
+  // products and shares its keys with no other.  (Four tiles take all 255 registers
+  // and spill up to 100 bytes, as do two of 256 values, up to 190.)
   constexpr int Most = HD == 256 ? 2 : 4;
   constexpr int Part = sizeof(T) == 4 && HD == 128 && BITS == 8 ? 2 : Most;
   // Up to four rows of float32: both terms in one 8-row tile (8 sequences of 4,096
-  // keys, 32 heads, 8 bits: 62.6 us where as two tiles it took 72.8).
+  // keys, 32 heads, 8 bits: 61.6 us where as two tiles it took 69.0).
   if constexpr (sizeof(T) == 4) {
     if (a.rows <= 4) return start<T, HD, BITS, 1, 1, true>(a, st);
   }
   if (a.rows_at_once == 8) return start<T, HD, BITS, 1, 1>(a, st);
   if (a.rows_at_once == 16) return start<T, HD, BITS, 2, 1>(a, st);
   if (a.rows_at_once == 32) return start<T, HD, BITS, Part, 4 / Part>(a, st);
-  if (a.rows_at_once == 64) return start<T, HD, BITS, Part, 8 / Part>(a, st);
+  if (a.rows_at_once == 64) return start<T, HD, BITS, Most, 8 / Most>(a, st);
   if constexpr (Most == 4) return start<T, HD, BITS, Most, 4>(a, st);
   return cudaErrorInvalidValue;
 }
