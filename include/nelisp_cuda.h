@@ -471,8 +471,16 @@ int nl_kv_move_dev(const nl_kv_move_args *args, void *stream);
  *   LSE[b,i,h] = log sum_t exp(SCALE q.k_t)
  * Q and O are rows (b, i) of heads*head_dim elements of DTYPE, 16-byte
  * aligned, Q_STRIDE and O_STRIDE apart; query head h reads key head
- * h / (heads/kv_heads); LSE is f32 [batch*nodes][heads] or NULL.  Products
- * are exact in the codes and sums f32.  WORKSPACE holds at least
+ * h / (heads/kv_heads); LSE is f32 [batch*nodes][heads] or NULL.  The products
+ * take the codes exactly.  Their other operand, the queries and the softmax
+ * weights times the values' scales, is float16 after a power of two: one
+ * term, 11 bits, where DTYPE is bf16 (whose queries that holds exactly, and
+ * whose outputs' 8 bits cover the weights' rounding), two, 22 bits, where it
+ * is f32.  A node's value that a row does not see costs its weights nothing,
+ * whatever its size up to 2^120 times the others'.  Sums are f32 on the tensor
+ * cores, which cut what they add: at most 16 keys (f32) or 2,048 additions
+ * (bf16; 2^-12 of a sum of one sign) before they are joined in plain f32; the
+ * softmax's sums and maxima are plain f32.  WORKSPACE holds at least
  * nl_tree_attn_workspace_bytes(nodes, heads, kv_heads, head_dim) bytes,
  * 16-byte aligned, or is NULL for the library's own (calls that overlap in
  * time must then not share it).  Does not synchronise; with bf16 and more

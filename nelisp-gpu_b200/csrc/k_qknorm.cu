@@ -17,11 +17,13 @@
 // key heads with the row's products of gain, cosine and sine in registers;
 // blocks belong to one of the two parts, so a thread holds one gain (and one
 // set of gain gradients).  The next vectors are on their way to shared memory
-// meanwhile, in runs of whole vectors whatever the pairs.  Arithmetic is two floats an instruction, all in 32 bits; the one
-// rounding to the output type is at the store.  8,192 rows of 40 heads of 128,
-// bfloat16, one row in twenty padding: 30.6 us, 5.6 TB/s, 0.86 of a copy;
-// backward, 8,191 rows of 40 heads of 64: 28.4 us, 4.5 TB/s, bound by the latency
-// of a step that few warps hide.
+// meanwhile, in runs of whole vectors whatever the pairs.  Arithmetic is two
+// floats an instruction, all in 32 bits; the one rounding to the output type is
+// at the store.  8,192 rows of 40 heads of 128, bfloat16, one row in twenty
+// padding: 30.9 us, 5.6 TB/s, 0.85 of a copy; backward, 8,191 rows of 40 heads of
+// 64: 28.4 us, 4.5 TB/s, bound by the latency of a step that few warps hide.  A part
+// with fewer heads than a warp holds at a time leaves the other lanes idle: 8,192
+// rows of 8 heads and 1 of 64, bfloat16, take 11.6 us where 32 and 8 take 15.9.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

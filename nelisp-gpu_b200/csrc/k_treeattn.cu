@@ -91,8 +91,8 @@ extern "C" int nl_tree_attn_dev(const nl_tree_attn_args *args, void *stream) {
     for (int i = 0; i < 2; i++)
       a.pool.code[i] = (uint8_t *)workspace, a.pool.param[i] = (uint32_t *)workspace;
   a.part_o = (float *)workspace;
-  // sized by the rows of tree_rows_at_once; the tcgen05 form's 2 x 148 items of
-  // up to 128 rows, of more than 16, fit its 2 x 592 of at least 32
+  // Sized for 2 x 592 parts of tree_rows_at_once rows; the tcgen05 form has 2 x 148 of
+  // 32 rows (of 17 to 32, which that rounds to 32) or of 64 (of more: 64 or 128).
   a.part_ml = a.part_o +
               (size_t)2 * kTreeMaxCtas * tree_rows_at_once(a.rows, head_dim) * head_dim;
   cudaError_t e = umma_rows         ? tree_umma_start(a, st)
