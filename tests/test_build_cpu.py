@@ -34,6 +34,19 @@ def test_an_interpreter_without_torch(tmp_path):
     assert "_serving.so" not in plan(f"PYTHON={exe}")
 
 
+def test_a_torch_without_cuda_or_without_metadata(tmp_path):
+    """Without CUDA its headers would not do; without metadata it is torch all the
+    same."""
+    (tmp_path / "torch" / "lib").mkdir(parents=True)
+    (tmp_path / "torch" / "__init__.py").write_text("")
+    exe = tmp_path / "python"
+    exe.write_text(f'#!/bin/sh\nexec env PYTHONPATH="{tmp_path}" "{sys.executable}" -S "$@"\n')
+    exe.chmod(0o755)
+    assert "_serving.so" not in plan(f"PYTHON={exe}")
+    (tmp_path / "torch" / "lib" / "libc10_cuda.so").write_text("")
+    assert "_serving.so" in plan(f"PYTHON={exe}")
+
+
 def test_with_torch_the_module_is_built_by_that_interpreter():
     out = plan(f"PYTHON={sys.executable}")
     line = next(x for x in out.split("\n") if "-o nelisp_cuda/_serving.so" in x)
