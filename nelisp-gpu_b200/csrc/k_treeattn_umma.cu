@@ -29,9 +29,9 @@
 //               thread's branch the issue of a tile took longer than its work.
 // The registers of the launch are shared out anew among the roles.
 //
-// What bounds it: a tile takes about 3,100 cycles (131,071 keys, 16 nodes of 4
-// heads, 8 bits: 107 us, 2.6 TB/s, 321 TF/s) with the tensor cores 17% busy,
-// issue 58%, and shared memory -- codes in and out, values out and in again,
+// What bounds it: a tile takes about 3,000 cycles (131,071 keys, 16 nodes of 4
+// heads, 8 bits: 102 us, 2.7 TB/s, 336 TF/s) with the tensor cores 18% busy,
+// issue 67%, and shared memory -- codes in and out, values out and in again,
 // weights, the rows' factors and references -- about 80%.  No role is the one:
 // each is 2,000 to 2,300 cycles busy a tile at 5 to 8 cycles an instruction, and
 // waits the rest of it for another.  Registers matter: the list of work in 64
@@ -983,9 +983,9 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
   }
   a.ctas = 148;
   a.tile = kTileKeys;
-  // (With 3, 5, 7, 10, us: 16 ragged sequences to 8,192 keys, 32 rows, 4 bits 88, 66, 64,
-  // 65; 4 ragged to 16,384, 256 rows 169, 124, 104, 108; 8 of 2,000, 64 rows 32.3, 33.8,
-  // 35.3, 36.7; 32 of 500 45.0, 44.4, 42.7, 42.0.)
+  // (With 5, 7, 10, us: 16 ragged sequences to 8,192 keys, 32 rows, 4 bits 64.7, 62.7,
+  // 61.9, with 3 88; 4 ragged to 16,384, 256 rows 123, 100, 103, with 3 169; 8 of 2,000,
+  // 64 rows 33.6, 35.1, 36.4; 32 of 500 44.4, 42.7, 42.3.)
   a.item_cost = 7;
   int *err = wait_flag_device();
   if (!err) return cudaErrorMemoryAllocation;
@@ -997,25 +997,25 @@ cudaError_t start(TreeArgs &a, cudaStream_t st) {
 }  // namespace
 
 // The rows of an item of this form, 0 where the other one serves.  It takes
-// about 3,100 cycles a tile whatever the rows, the other one a time that grows
+// about 3,000 cycles a tile whatever the rows, the other one a time that grows
 // with them and with the head size, so this one is for many (us, 4 sequences of
 // 32,768 keys, 8 key heads, 8 bits / 4 bits):
 //   rows            8        16       20        32         48        64
 //   128 values
-//     this form   78/90    78/89    79/ 90    79/ 90    102/109   103/109
-//     the other   57/59    69/72    97/102   100/106    173/189   176/193
+//     this form   82/85    81/86    82/ 85    82/ 85     97/111    99/112
+//     the other   57/59    69/73    97/103   100/106    174/190   177/194
 //   64 values
-//     this form   92/101   92/102   93/102    93/102     93/102    95/104
-//     the other   40/40    47/50    62/ 71    65/ 73    115/128   117/131
+//     this form   91/102   91/102   91/102    91/103     92/102    93/105
+//     the other   40/40    47/50    63/ 71    65/ 73    115/128   118/131
 // More than 16 rows of 128 values, then, or 32 of 64.  Few and short sequences
 // would have it otherwise (8 bits, 128 values, 8 key heads; this form / the other):
 //   keys                     500          1,000        2,000        4,000
-//   1 sequence, 24 rows   16.1/14.8    17.7/15.8    16.7/18.5    18.7/24.6
-//   64 rows               21.8/21.7    23.2/25.3    21.2/31.7    22.8/39.2
-//   8 sequences, 24 rows  19.8/22.5    23.9/24.1    27.3/30.0    36.3/40.7
-//   64 rows               22.2/32.3    31.9/38.2    35.7/49.2    46.9/71.1
+//   1 sequence, 24 rows   16.3/14.4    17.9/15.9    17.0/18.5    18.8/24.6
+//   64 rows               21.8/21.8    23.3/25.4    21.4/31.7    23.0/39.3
+//   8 sequences, 24 rows  19.9/22.6    24.1/24.0    27.8/30.3    37.1/40.8
+//   64 rows               22.6/32.3    32.0/38.3    35.6/49.4    46.2/71.3
 // but the lengths are on the device, and the rule goes by what the host knows: a
-// single sequence of up to 1,000 keys pays 1 to 23% for it.  (256 values have no room
+// single sequence of up to 1,000 keys and 17 to 32 rows pays 13 to 25% for it.  (256 values have no room
 // in TMEM and shared memory; a run of a page that is no multiple of 16 keys has
 // no copy of whole boxes; float32 needs its sums out of the tensor core often.)
 uint32_t tree_umma_rows(const TreeArgs &a, bool bf16) {

@@ -892,7 +892,7 @@ cudaError_t start_rows(TreeArgs &a, cudaStream_t st) {
   //   rows               16         32         64         128
   //   bf16  4 a warp   69/ 73    100/106    176/193    330/367
   //         half       85/ 98    114/129    209/235    383/424
-  //   f32   4 a warp   88/ 87    193/148    274/286    508/550
+  //   f32   4 a warp   88/ 87    193/149    275/287    510/552
   //         half      108/112    159/156    293/304    544/565
   // (half: 1 of 16 rows, 2 of more, 128 as two items of 64.)  32 rows of float32 in 8
   // bits are the exception: one warp with four tiles holds both terms of both

@@ -72,12 +72,11 @@ __device__ __forceinline__ uint32_t tiles_of(const TreeArgs &a, uint32_t b) {
 // it is divided among.  Where all sequences are equally long, a number of CTAs
 // that the items divide evenly gives every CTA a part of one item only, which saves
 // it an item's own cost, and leaves some CTAs without work: it is taken where a
-// CTA's part grows by no more than that.  (Even / by places, us: 32 items of 8 rows of
-// 64 values, bf16, 32,768 keys, on 576 or 592 CTAs, 39.3 / 51.5; 128
-// items of 32 rows, bf16, 4 bits, on 128 or 148 CTAs, 500 keys 20.1 / 26.0, 2,000:
-// 35.9 / 40.5, 8,192: 101.1 / 96.3, 32,768: 374 / 322; 64 rows, 8 bits, 1,000 keys
-// 28.8 / 36.0, 8,000: 110.6 / 106.9; 256 items of a row, f32, 4,096 keys, on 256 or
-// 296: 61.7 / 61.4.)
+// CTA's part grows by no more than that.  (Even / by places, us: 32 items of 8 rows
+// of 64 values, bf16, 32,768 keys, on 576 or 592 CTAs, 39.8 / 52.9; 128 items of 32
+// rows, bf16, 4 bits, on 128 or 148, 500 keys 19.8 / 25.7, 2,000: 34.9 / 39.0, 64 rows,
+// 8 bits, 1,000 keys 28.4 / 35.3; but 128 of 32 rows, 8,192 keys 101 / 96, 32,768: 374 /
+// 322; 256 of a row, f32, 4,096 keys, on 256 or 296 61.7 / 61.4.)
 struct List {
   uint32_t total, workers;
 };
